@@ -58,6 +58,9 @@ SIGNATURES = {
     "granite4_kernel_rope_kv_int8_paged": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_int, C.c_int,
                                                      C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                                      _vp, _vp, _vp, _vp, _vp]),
+    "granite4_kernel_qk_norm_rope_kv_paged": (C.c_int, [_vp, _vp, _vp, C.c_float, _vp, _vp, _vp, _vp] + [C.c_int] * 7 +
+                                              [_vp, _vp, _vp, _vp, _vp]),
+    "granite4_kernel_kv_read_paged": (C.c_int, [_vp, _vp, _vp, _vp, _vp] + [C.c_int] * 5 + [_vp, _vp]),
     "granite4_kernel_argmax_rows": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp]),
     "granite4_kernel_multi_scatter_advance": (C.c_int, [_vp, _vp]),
     "granite4_kernel_argmax_advance": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp]),
@@ -109,6 +112,10 @@ SIGNATURES = {
     "granite4_attn_split_int8": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_float, C.c_int, C.c_int, C.c_int, C.c_int,
                                            _vp, C.c_int, C.c_int, _vp, C.c_longlong, _vp, _vp, C.c_int, _vp, _vp,
                                            _vp, C.c_int, _vp, _vp, C.c_int]),
+    "granite4_attn_decode_int4_scratch_bytes": (C.c_longlong, [C.c_int] * 6),
+    "granite4_kernel_attn_decode_int4_paged": (C.c_int, [_vp] * 8 + [C.c_int] * 8 + [C.c_float, _vp, C.c_longlong, _vp]),
+    "granite4_prefill_attention_int4_scratch_bytes": (C.c_longlong, [C.c_int] * 5),
+    "granite4_prefill_attention_int4": (C.c_int, [_vp, C.c_float] + [C.c_int] * 6 + [_vp] * 7 + [C.c_longlong]),
     "granite4_gemm_fp8_workspace_bytes": (C.c_longlong, [C.c_int, C.c_int, C.c_int]),
     "granite4_kernel_gemm_fp8": (C.c_int, [C.c_int, _vp, C.c_longlong, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp,
                                            C.c_longlong]),

@@ -1,0 +1,671 @@
+// Attention of new tokens over the 4-bit paged KV pool: one token or a few rows of every sequence (decode,
+// verify), split over the length of the cache and joined; and prompt chunks.
+//
+//   query row r at position pos[r] sees cache positions t in (pos - window, pos] (window 0: [0, pos]);
+//   position t lives in pool row table[t]; k_t = code * k_scale, v_t = code * v_scale, codes c in [-7, 7]
+//   l_t = scale * q . k_t,   out = sum_t softmax(l)_t v_t,   no position seen: out = 0
+//
+// A position costs d + 8 bytes a kv head and 4 d multiply-adds a query head: memory bounds it as long as the
+// conversion of the codes stays cheap, so nothing is converted that need not be:
+//  * A nibble u = c + 8 masked out of a word IS an fp16 number: bits 0-3 of a half are the subnormal u 2^-24,
+//    bits 4-7 the value u 2^-20. One AND gives two mma operand elements. The 2^-24 (and the factor 16 of the odd
+//    dims: folded into q for the logits, taken out of the output rows for V) are powers of two, hence exact.
+//  * The 8 of u = c + 8 is one number per column: sum_d q_d (u_d - 8) = sum q u - 8 sum q, and
+//    sum_t p_t (u_t - 8) = sum p u - 8 sum p, with sum p from one more mma against ones.
+//  * The row scales multiply a logit (K) and a probability (V), never an element.
+//  * Both contractions have the cache positions on the 16-row side (S^T = K Q^T) or the 16-deep side (O^T = V^T P^T)
+//    of mma.sync m16n8k16 and the (query row, head) pairs on the 8-column side. Which dims a lane's fragment
+//    elements stand for is free as long as q's match, so a lane's K elements are 16 consecutive bytes of a row and
+//    its V elements 8: both are loaded from global memory straight into the registers the masks are applied to.
+// P is rounded to fp16 (11 bits; everything else is f32) after the multiplication with v_scale and a power of two
+// that puts the largest v_scale seen at 2^12, so values of any magnitude keep the format's precision.
+//
+// Work split: the (group, kv head, column block) segments' tiles of 32 positions form one line, cut into equal
+// shares, one CTA each, whatever the sequences' lengths (read on the device). A CTA's four warps take every fourth
+// tile of a segment's piece, each with its own running (max, sum, O); they merge in shared memory. Pieces of a
+// segment that more than one CTA worked on are joined by a second small kernel, in order of the CTAs.
+#include "g4_host.h"
+#include "g4_math.cuh"
+
+#include "../../include/granite4_b200.h"
+
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+namespace g4 {
+
+// kv_read.cu
+int widen_int4(const char* fn, const uint8_t* ck, const uint8_t* cv, const float* ks, const float* vs, const int* pt,
+               int Hk, long long stride, long long n, int8_t* ok, int8_t* ov, float* oks, float* ovs);
+
+namespace {
+
+constexpr int kTile = 32;     // positions a warp works on at a time
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMaxGroups = 1024;  // of a launch that splits the line of tiles
+constexpr int kMaxColumns = 64;   // rows of a group x query heads of a kv head
+
+struct Int4AttnParams {
+  const uint16_t* q;
+  const uint8_t* ck;
+  const uint8_t* cv;
+  const float* ks;
+  const float* vs;
+  const int* row_pos;  // NULL: row r is at base_pos + r
+  int base_pos;
+  const int* const* row_pt;
+  const int* pt;
+  uint16_t* out;
+  float* part_o;   // [slots][columns][D]
+  float* part_ml;  // [slots][columns][2]
+  int* prefix;     // [groups + 1] tiles before each group
+  int rows, per, groups, Hq, Hk, G, blocks;  // blocks: column blocks of a segment
+  long long stride;
+  int max_len, window;
+  float scale_log2;
+  int split;  // the line of tiles is cut into gridDim.x shares (0: a CTA per segment)
+};
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t halves(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// First and last position that any row of a group sees; last < first: none.
+__device__ __forceinline__ void group_span(const Int4AttnParams& p, int grp, int& lo, int& hi) {
+  lo = INT_MAX, hi = -1;
+  const int r0 = grp * p.per, nr = min(p.per, p.rows - r0);
+  for (int j = 0; j < nr; ++j) {
+    const int raw = p.row_pos != nullptr ? __ldg(p.row_pos + r0 + j) : p.base_pos + r0 + j;
+    if (raw < 0) continue;
+    const int pos = min(raw, p.max_len - 1);
+    hi = max(hi, pos);
+    lo = min(lo, p.window > 0 ? max(0, pos + 1 - p.window) : 0);
+  }
+}
+__device__ __forceinline__ int group_tiles(const Int4AttnParams& p, int grp) {
+  int lo, hi;
+  group_span(p, grp, lo, hi);
+  return hi < 0 ? 0 : hi / kTile - lo / kTile + 1;
+}
+
+// s_prefix[g] = tiles of the groups before g, s_prefix[groups] = all.
+__device__ void scan_groups(const Int4AttnParams& p, int* s_prefix) {
+  __shared__ int s_warp[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = (p.groups + kThreads - 1) / kThreads, g0 = threadIdx.x * each;
+  int sum = 0;
+  for (int i = 0; i < each; ++i)
+    if (g0 + i < p.groups) sum += group_tiles(p, g0 + i);
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  int before = inc - sum;
+  for (int w = 0; w < warp; ++w) before += s_warp[w];
+  for (int i = 0; i < each; ++i)
+    if (g0 + i < p.groups) s_prefix[g0 + i] = before, before += group_tiles(p, g0 + i);
+  if (threadIdx.x == kThreads - 1) s_prefix[p.groups] = s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3];
+  __syncthreads();
+}
+
+// CTAs that a line of `all` tiles is cut for: every share has a tile at least, and one for each warp where there are so many.
+__device__ __forceinline__ long long shares_of(long long all, int shares) {
+  return min(static_cast<long long>(shares), (all + kWarps - 1) / kWarps);
+}
+
+// The codes and scales of one tile as a lane holds them. K: rows g, g + 8, g + 16, g + 24 of the tile, a quarter of
+// the dims each; V: rows 2t, 2t + 1, 2t + 8, 2t + 9 (+ 16), an eighth of the dims each; scales of row `lane`.
+template <int D>
+struct Tile {
+  uint32_t k[4][D / 32];
+  uint32_t v[8][D / 64];
+  float sk, sv;
+};
+
+// NT column tiles of 8: column 8 nt + i of column block cb is (query row c / G, query head c % G), c = 8 NT cb + 8 nt + i.
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(const Int4AttnParams p) {
+  pdl_begin();
+  constexpr int kC = 8 * NT, kW = D / 32 /* K words of a row per lane */, kM = D / 16 /* 16-dim tiles of O^T */;
+  __shared__ int s_prefix[kMaxGroups + 1];
+  __shared__ __align__(16) float s_o[kWarps][kC][D + 4];
+  __shared__ float s_ml[kWarps][kC][2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int per_group = p.Hk * p.blocks;
+  long long x = 0, x_end = 0;  // this CTA's share of the line of tiles
+  int grp = 0, sub = 0;
+  if (p.split) {
+    scan_groups(p, s_prefix);
+    const long long all = static_cast<long long>(s_prefix[p.groups]) * per_group;
+    const long long shares = shares_of(all, gridDim.x);
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i <= p.groups; i += kThreads) p.prefix[i] = s_prefix[i];
+    if (blockIdx.x >= shares) return;
+    x = blockIdx.x * all / shares, x_end = (blockIdx.x + 1) * all / shares;
+    int lo = 0, hi = p.groups - 1;  // the last group that begins at or before x
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (static_cast<long long>(s_prefix[mid]) * per_group <= x) lo = mid;
+      else hi = mid - 1;
+    }
+    grp = lo;
+  }
+
+  while (true) {
+    int n_tiles, first_tile, piece_begin, piece_end;  // of this segment's tiles
+    int span_lo, span_hi;
+    if (p.split) {
+      if (x >= x_end) return;
+      while (static_cast<long long>(s_prefix[grp + 1]) * per_group <= x) ++grp;
+      n_tiles = s_prefix[grp + 1] - s_prefix[grp];
+      const long long in = x - static_cast<long long>(s_prefix[grp]) * per_group;
+      sub = static_cast<int>(in / n_tiles);
+      piece_begin = static_cast<int>(in % n_tiles);
+      piece_end = static_cast<int>(min(static_cast<long long>(n_tiles), piece_begin + (x_end - x)));
+      x += piece_end - piece_begin;
+    } else {
+      grp = blockIdx.x / per_group, sub = blockIdx.x % per_group;
+      piece_begin = 0;
+    }
+    group_span(p, grp, span_lo, span_hi);
+    first_tile = span_hi < 0 ? 0 : span_lo / kTile;
+    if (!p.split) n_tiles = piece_end = span_hi < 0 ? 0 : span_hi / kTile - first_tile + 1;
+    const int hkv = sub / p.blocks, c0 = (sub % p.blocks) * kC;
+    const int r0 = grp * p.per, nrows = min(p.per, p.rows - r0), columns = min(kC, nrows * p.G - c0);
+    const size_t head_row0 = static_cast<size_t>(hkv) * p.stride;
+    const uint8_t* ck = p.ck + head_row0 * (D / 2) + t * (D / 8);
+    const uint8_t* cv = p.cv + head_row0 * (D / 2) + g * (D / 16);
+    const float* ks = p.ks + head_row0;
+    const float* vs = p.vs + head_row0;
+    const int* pt = p.row_pt != nullptr ? p.row_pt[r0] : p.pt;
+
+    // pool row of the lane's position of a tile; positions that no row sees read pool row 0 and are masked
+    auto table_row = [&](int tile) -> int {
+      const int pos = tile * kTile + lane;
+      if (pos < span_lo || pos > span_hi) return 0;
+      const int row = pt != nullptr ? __ldg(pt + pos) : pos;
+      return min(max(row, 0), static_cast<int>(p.stride) - 1);
+    };
+    auto load = [&](Tile<D>& b, int row) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* src = ck + static_cast<size_t>(__shfl_sync(0xffffffffu, row, g + 8 * i)) * (D / 2);
+        if (D == 128) {
+          const uint4 w = __ldg(reinterpret_cast<const uint4*>(src));
+          b.k[i][0] = w.x, b.k[i][1] = w.y, b.k[i][kW - 2] = w.z, b.k[i][kW - 1] = w.w;
+        } else {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
+          b.k[i][0] = w.x, b.k[i][1] = w.y;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = 2 * t + (i & 1) + 8 * (i >> 1);
+        const uint8_t* src = cv + static_cast<size_t>(__shfl_sync(0xffffffffu, row, at)) * (D / 2);
+        if (D == 128) {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
+          b.v[i][0] = w.x, b.v[i][D / 64 - 1] = w.y;
+        } else {
+          b.v[i][0] = __ldg(reinterpret_cast<const uint32_t*>(src));
+        }
+      }
+      b.sk = __ldg(ks + row), b.sv = __ldg(vs + row);
+    };
+    const int tile_end = first_tile + piece_end;
+    int tile = first_tile + piece_begin + warp;
+    Tile<D> bufs[2];
+    int row_next = 0;
+    if (tile < tile_end) {
+      load(bufs[0], table_row(tile));
+      if (tile + kWarps < tile_end) row_next = table_row(tile + kWarps);
+    }
+
+    // q as the B operand, scaled by a power of two per column; the operand's elements follow the nibbles of K's
+    // words: dims 8w + {0, 4} | {1, 5} and {2, 6} | {3, 7} of the lane's quarter, the odd ones over 16
+    uint32_t qb[NT][2 * kW][2];
+    float l_scale[NT][2], l_off[NT][2];  // of the accumulator's columns 8 nt + 2 t + e
+    int pos_col[NT][2], lo_col[NT][2];
+    int all_lo = 0, all_hi = INT_MAX;  // positions that every column sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int c = c0 + 8 * nt + g;
+      const bool live = 8 * nt + g < columns;
+      const int j = live ? c / p.G : 0, hl = live ? c % p.G : 0;
+      const uint16_t* qrow = p.q + (static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + t * (D / 4);
+      float f[kW][8];
+      float top = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kW; ++w) {
+        unpack8(live ? __ldg(reinterpret_cast<const uint4*>(qrow) + w) : make_uint4(0u, 0u, 0u, 0u), f[w]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[w][e]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int ex = 0;
+      if (top > 0.0f && top < INFINITY) ex = min(max(((__float_as_int(top) >> 23) & 0xff) - 127 - 12, -100), 100);
+      const float down = __int_as_float((127 - ex) << 23), down16 = down * 0.0625f;
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kW; ++w) {
+        qb[nt][2 * w][0] = halves(f[w][0] * down, f[w][4] * down);
+        qb[nt][2 * w][1] = halves(f[w][1] * down16, f[w][5] * down16);
+        qb[nt][2 * w + 1][0] = halves(f[w][2] * down, f[w][6] * down);
+        qb[nt][2 * w + 1][1] = halves(f[w][3] * down16, f[w][7] * down16);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&qb[nt][2 * w + i][0]));
+          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&qb[nt][2 * w + i][1]));
+          sum += (a.x + a.y) + 16.0f * (b.x + b.y);
+        }
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const float up = p.scale_log2 * __int_as_float((127 + ex) << 23) * 16777216.0f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int cc = 8 * nt + 2 * t + e;
+        l_scale[nt][e] = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4);
+        l_off[nt][e] = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4) * (8.0f / 16777216.0f);
+        pos_col[nt][e] = INT_MAX, lo_col[nt][e] = 0;  // a column that is not there sees everything and is dropped
+        if (cc < columns) {
+          const int row = r0 + (c0 + cc) / p.G;
+          const int raw = p.row_pos != nullptr ? __ldg(p.row_pos + row) : p.base_pos + row;
+          const int pos = raw < 0 ? -1 : min(raw, p.max_len - 1);
+          pos_col[nt][e] = pos, lo_col[nt][e] = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+        }
+        all_hi = min(all_hi, pos_col[nt][e]), all_lo = max(all_lo, lo_col[nt][e]);
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      all_hi = min(all_hi, __shfl_xor_sync(0xffffffffu, all_hi, o));
+      all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, o));
+    }
+
+    float o[NT][kM][4], osum[NT][4], m_run[NT][2], l_run[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int b = 0; b < kM; ++b) o[nt][b][0] = o[nt][b][1] = o[nt][b][2] = o[nt][b][3] = 0.0f;
+      osum[nt][0] = osum[nt][1] = osum[nt][2] = osum[nt][3] = 0.0f;
+      m_run[nt][0] = m_run[nt][1] = -INFINITY, l_run[nt][0] = l_run[nt][1] = 0.0f;
+    }
+    float v_mult = 1.0f, v_cap = -1.0f;  // power of two on v_scale, and the largest v_scale it is good for
+
+    auto attend = [&](const Tile<D>& b, int t0) {
+      // S^T = K Q^T for the tile's two halves
+      float s[NT][2][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[nt][h][0] = s[nt][h][1] = s[nt][h][2] = s[nt][h][3] = 0.0f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int w = 0; w < kW; ++w) {
+          const uint32_t a = b.k[2 * h][w], c = b.k[2 * h + 1][w], a8 = a >> 8, c8 = c >> 8;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816(s[nt][h], a & 0x000f000fu, c & 0x000f000fu, a & 0x00f000f0u, c & 0x00f000f0u, qb[nt][2 * w][0],
+                     qb[nt][2 * w][1]);
+            mma16816(s[nt][h], a8 & 0x000f000fu, c8 & 0x000f000fu, a8 & 0x00f000f0u, c8 & 0x00f000f0u,
+                     qb[nt][2 * w + 1][0], qb[nt][2 * w + 1][1]);
+          }
+        }
+      const bool unmasked = t0 >= all_lo && t0 + kTile - 1 <= all_hi && t0 >= span_lo && t0 + kTile - 1 <= span_hi;
+      const float sv_lane = (t0 + lane >= span_lo && t0 + lane <= span_hi) ? b.sv : 0.0f;
+      float fk[4], fv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fk[i] = __shfl_sync(0xffffffffu, b.sk, g + 8 * i);
+      if (__any_sync(0xffffffffu, sv_lane > v_cap)) {
+        const float top = warp_max(sv_lane);
+        float mult = 1.0f;
+        v_cap = 0.0f;
+        if (top > 0.0f && top < INFINITY) {
+          const int ex = min(max(((__float_as_int(top) >> 23) & 0xff) - 127, -100), 100);
+          mult = __int_as_float((127 + 12 - ex) << 23);
+          v_cap = __int_as_float((127 + 3 + ex) << 23);  // 2^15 once multiplied
+        }
+        const float f = mult / v_mult;
+        v_mult = mult;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int m = 0; m < kM; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[nt][m][i] *= f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) osum[nt][i] *= f;
+        }
+      }
+      const float sv_mult = sv_lane * v_mult;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fv[i] = __shfl_sync(0xffffffffu, sv_mult, g + 8 * i);
+      uint32_t pb[NT][2][2];
+      bool moved = false;
+      float corr[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float pr[2][4];  // [column e][position g + 8 i]
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float l[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            l[i] = (s[nt][i >> 1][2 * (i & 1) + e] - l_off[nt][e]) * (fk[i] * l_scale[nt][e]);
+            if (!unmasked) {
+              const int pos = t0 + g + 8 * i;
+              if (pos > pos_col[nt][e] || pos < lo_col[nt][e]) l[i] = -INFINITY;
+            }
+          }
+          float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const float m_new = fmaxf(m_run[nt][e], top), base = m_new == -INFINITY ? 0.0f : m_new;
+          corr[nt][e] = exp2_fast(m_run[nt][e] - base);
+          moved |= m_new != m_run[nt][e];
+          m_run[nt][e] = m_new;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pr[e][i] = exp2_fast(l[i] - base);
+          l_run[nt][e] = l_run[nt][e] * corr[nt][e] + ((pr[e][0] + pr[e][1]) + (pr[e][2] + pr[e][3]));
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            pb[nt][h][u] = transpose8x8(halves(pr[0][2 * h + u] * fv[2 * h + u], pr[1][2 * h + u] * fv[2 * h + u]));
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int m = 0; m < kM; ++m) {
+            o[nt][m][0] *= corr[nt][0], o[nt][m][1] *= corr[nt][1];
+            o[nt][m][2] *= corr[nt][0], o[nt][m][3] *= corr[nt][1];
+          }
+          osum[nt][0] *= corr[nt][0], osum[nt][1] *= corr[nt][1];
+          osum[nt][2] *= corr[nt][0], osum[nt][3] *= corr[nt][1];
+        }
+      }
+      // O^T += V^T P^T: the halves of two positions' words side by side are four dims of both
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int w = 0; w < D / 64; ++w)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t sel = u ? 0x7632u : 0x5410u;
+            const uint32_t a = __byte_perm(b.v[4 * h][w], b.v[4 * h + 1][w], sel), a8 = a >> 8;
+            const uint32_t c = __byte_perm(b.v[4 * h + 2][w], b.v[4 * h + 3][w], sel), c8 = c >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816(o[nt][4 * w + 2 * u], a & 0x000f000fu, a & 0x00f000f0u, c & 0x000f000fu, c & 0x00f000f0u,
+                       pb[nt][h][0], pb[nt][h][1]);
+              mma16816(o[nt][4 * w + 2 * u + 1], a8 & 0x000f000fu, a8 & 0x00f000f0u, c8 & 0x000f000fu, c8 & 0x00f000f0u,
+                       pb[nt][h][0], pb[nt][h][1]);
+            }
+          }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma16816(osum[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[nt][h][0], pb[nt][h][1]);
+      }
+    };
+
+    while (tile < tile_end) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (tile < tile_end) {  // the same for the whole warp
+          if (tile + kWarps < tile_end) {
+            load(bufs[i ^ 1], row_next);
+            if (tile + 2 * kWarps < tile_end) row_next = table_row(tile + 2 * kWarps);
+          }
+          attend(bufs[i], tile * kTile);
+          tile += kWarps;
+        }
+      }
+    }
+
+    // the four warps' states meet in shared memory
+    const float back = 16777216.0f / v_mult;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float l = l_run[nt][e];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        const int c = 8 * nt + 2 * t + e;
+        if (g == 0) s_ml[warp][c][0] = m_run[nt][e], s_ml[warp][c][1] = l;
+        const float off = osum[nt][e] * (8.0f / 16777216.0f);
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+          *reinterpret_cast<float2*>(&s_o[warp][c][g * (D / 8) + 2 * m]) =
+              make_float2((o[nt][m][e] - off) * back, (o[nt][m][2 + e] * 0.0625f - off) * back);
+      }
+    }
+    __syncthreads();
+    const bool whole = piece_begin == 0 && piece_end == n_tiles;
+    const size_t slot = static_cast<size_t>(blockIdx.x) + static_cast<size_t>(grp) * per_group + sub;
+    for (int i = threadIdx.x; i < columns * D; i += kThreads) {
+      const int c = i / D, dim = i % D;
+      const float m = fmaxf(fmaxf(s_ml[0][c][0], s_ml[1][c][0]), fmaxf(s_ml[2][c][0], s_ml[3][c][0]));
+      float l = 0.0f, acc = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = s_ml[w][c][0] == -INFINITY ? 0.0f : exp2f(s_ml[w][c][0] - m);
+        l += f * s_ml[w][c][1], acc += f * s_o[w][c][dim];
+      }
+      if (whole) {
+        const int row = r0 + (c0 + c) / p.G, hl = (c0 + c) % p.G;
+        p.out[(static_cast<size_t>(row) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + dim] =
+            static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? acc / l : 0.0f));
+      } else {
+        p.part_o[(slot * kC + c) * D + dim] = acc;
+        if (dim == 0) p.part_ml[(slot * kC + c) * 2] = m, p.part_ml[(slot * kC + c) * 2 + 1] = l;
+      }
+    }
+    if (!p.split) return;
+    __syncthreads();
+  }
+}
+
+// Joins the pieces of segments that several CTAs worked on: a CTA per segment, in the CTAs' order.
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4AttnParams p, int max_shares) {
+  pdl_begin();
+  constexpr int kC = 8 * NT;
+  const int per_group = p.Hk * p.blocks, grp = blockIdx.x / per_group, sub = blockIdx.x % per_group;
+  const int hkv = sub / p.blocks, c0 = (sub % p.blocks) * kC, r0 = grp * p.per, nrows = min(p.per, p.rows - r0);
+  const int columns = min(kC, nrows * p.G - c0);
+  const int before = __ldcg(p.prefix + grp), n_tiles = __ldcg(p.prefix + grp + 1) - before;
+  const long long all = static_cast<long long>(__ldcg(p.prefix + p.groups)) * per_group;
+  const long long x0 = static_cast<long long>(before) * per_group + static_cast<long long>(sub) * n_tiles;
+  int i0 = 0, i1 = -1;  // the CTAs whose shares hold the segment's first and last tile
+  if (n_tiles > 0) {
+    const long long shares = shares_of(all, max_shares);
+    i0 = static_cast<int>(((x0 + 1) * shares - 1) / all), i1 = static_cast<int>(((x0 + n_tiles) * shares - 1) / all);
+    if (i0 == i1) return;  // written by that CTA
+  }
+  for (int i = threadIdx.x; i < columns * D; i += kThreads) {
+    const int c = i / D, dim = i % D;
+    float m = -INFINITY, l = 0.0f, acc = 0.0f;
+    for (int s = i0; s <= i1; ++s) {
+      const size_t at = (static_cast<size_t>(s) + blockIdx.x) * kC + c;
+      const float ms = __ldcg(p.part_ml + at * 2), ls = __ldcg(p.part_ml + at * 2 + 1);
+      if (ms == -INFINITY) continue;
+      const float mn = fmaxf(m, ms), f = m == -INFINITY ? 0.0f : exp2f(m - mn), fs = exp2f(ms - mn);
+      acc = acc * f + fs * __ldcg(p.part_o + at * D + dim), l = l * f + fs * ls, m = mn;
+    }
+    const int row = r0 + (c0 + c) / p.G, hl = (c0 + c) % p.G;
+    p.out[(static_cast<size_t>(row) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + dim] =
+        static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? acc / l : 0.0f));
+  }
+}
+
+// How a launch is cut: `shares` CTAs over the line of tiles, or a CTA per segment (shares 0).
+struct Int4Plan {
+  int nt, blocks, groups, shares;
+  long long segments, bytes;
+};
+
+Int4Plan plan_int4(int rows, int per, int Hq, int Hk, int d, int max_len) {
+  Int4Plan s{};
+  const int columns = per * (Hq / Hk);
+  s.nt = columns <= 8 ? 1 : 2;
+  s.blocks = (columns + 8 * s.nt - 1) / (8 * s.nt);
+  s.groups = (rows + per - 1) / per;
+  s.segments = static_cast<long long>(s.groups) * Hk * s.blocks;
+  const long long resident = static_cast<long long>(s.nt == 1 ? 3 : 2) * sm_count();
+  const long long tiles = s.segments * ((max_len + kTile - 1) / kTile);
+  // short caches: a segment is one tile per warp. Many segments: the CTAs balance one another, and each saves its
+  // neighbours the joining of a piece.
+  if (max_len <= kTile * kWarps || s.groups > kMaxGroups || s.segments >= 4 * resident) return s;
+  s.shares = static_cast<int>(std::min(resident, std::max(1ll, tiles / kWarps)));
+  const long long slots = s.shares + s.segments;
+  s.bytes = slots * 8 * s.nt * (d + 2) * 4 + (s.groups + 1 + 3) / 4 * 16;
+  return s;
+}
+
+bool int4_shape_ok(int Hq, int Hk, int d, int per) {
+  return (d == 64 || d == 128) && Hk > 0 && Hq > 0 && Hq % Hk == 0 && per > 0 && Hq / Hk <= kMaxColumns &&
+         static_cast<long long>(per) * (Hq / Hk) <= kMaxColumns;
+}
+
+template <int D, int NT>
+int launch_int4(const char* fn, const Int4AttnParams& p, const Int4Plan& s) {
+  const cudaStream_t st = current_stream();
+  if (s.segments > INT_MAX) return fail(fn, "too many rows");
+  const unsigned ctas = static_cast<unsigned>(p.split ? s.shares : s.segments);
+  G4_LAUNCH_PDL(fn, (attn_int4_kernel<D, NT>), dim3(ctas), dim3(kThreads), 0, st, p);
+  if (p.split)
+    G4_LAUNCH_PDL(fn, (attn_int4_join_kernel<D, NT>), dim3(static_cast<unsigned>(s.segments)), dim3(kThreads), 0, st, p, s.shares);
+  return 0;
+}
+
+// Checked arguments in; without scratch every segment is one CTA's.
+int attn_int4(const char* fn, Int4AttnParams p, int d, void* scratch, long long scratch_bytes, bool scratch_needed) {
+  p.G = p.Hq / p.Hk;
+  Int4Plan s = plan_int4(p.rows, p.per, p.Hq, p.Hk, d, p.max_len);
+  p.blocks = s.blocks, p.groups = s.groups;
+  const bool have = scratch != nullptr && scratch_bytes >= s.bytes && aligned16(scratch);
+  if (s.shares > 0 && !have) {
+    if (scratch_needed) return fail(fn, "scratch missing, misaligned or smaller than the size the scratch query returns");
+    s.shares = 0;
+  }
+  p.split = s.shares > 0;
+  if (p.split) {
+    p.part_o = static_cast<float*>(scratch);
+    const long long slots = s.shares + s.segments;
+    p.part_ml = p.part_o + slots * 8 * s.nt * d;
+    p.prefix = reinterpret_cast<int*>(p.part_ml + slots * 8 * s.nt * 2);
+  }
+  if (d == 128) return s.nt == 1 ? launch_int4<128, 1>(fn, p, s) : launch_int4<128, 2>(fn, p, s);
+  return s.nt == 1 ? launch_int4<64, 1>(fn, p, s) : launch_int4<64, 2>(fn, p, s);
+}
+
+// Chunks from this many rows on go through the tensor-core prefill kernels, which read an 8-bit pool.
+constexpr int kWidenRows = 32;
+bool widens(int rows, int Hq, int Hk, int d) { return rows >= kWidenRows && d == 128 && Hq == 4 * Hk; }
+int prefill_group(int Hq, int Hk) { return std::max(1, 16 / (Hq / Hk)); }
+long long widened_bytes(long long n, int Hk) { return (2 * n * Hk * (128 + 4) + 63) / 16 * 16; }
+
+}  // namespace
+}  // namespace g4
+
+extern "C" {
+
+long long granite4_attn_decode_int4_scratch_bytes(int rows, int rows_per_group, int Hq, int Hk, int d, int max_len) {
+  if (rows <= 0 || max_len <= 0 || !g4::int4_shape_ok(Hq, Hk, d, rows_per_group)) return -1;
+  return g4::plan_int4(rows, rows_per_group, Hq, Hk, d, max_len).bytes;
+}
+
+int granite4_kernel_attn_decode_int4_paged(const uint16_t* d_q, const uint8_t* d_cache_k, const uint8_t* d_cache_v,
+                                           const float* d_k_scale, const float* d_v_scale, const int* d_row_pos,
+                                           const int* const* d_row_pt, const int* d_pt, int rows, int rows_per_group,
+                                           int Hq, int Hk, int d, int stride, int max_len, int window, float scale,
+                                           void* d_scratch, long long scratch_bytes, uint16_t* d_out) {
+  const char* fn = "granite4_kernel_attn_decode_int4_paged";
+  if (d_q == nullptr || d_cache_k == nullptr || d_cache_v == nullptr || d_k_scale == nullptr || d_v_scale == nullptr ||
+      d_row_pos == nullptr || d_out == nullptr || rows <= 0 || stride <= 0 || max_len <= 0 ||
+      (d_row_pt == nullptr && d_pt == nullptr && max_len > stride) || window < 0 || !std::isfinite(scale))
+    return g4::fail(fn, "invalid arguments");
+  if (!g4::int4_shape_ok(Hq, Hk, d, rows_per_group))
+    return g4::fail(fn, "head dims of 64 and 128; Hq a multiple of Hk; at most 64 query rows x heads a kv head and group");
+  if (!g4::aligned16(d_q) || !g4::aligned16(d_cache_k) || !g4::aligned16(d_cache_v))
+    return g4::fail(fn, "q and the caches must be 16-byte aligned");
+  g4::Int4AttnParams p{};
+  p.q = d_q, p.ck = d_cache_k, p.cv = d_cache_v, p.ks = d_k_scale, p.vs = d_v_scale, p.out = d_out;
+  p.row_pos = d_row_pos, p.row_pt = d_row_pt, p.pt = d_pt;
+  p.rows = rows, p.per = rows_per_group, p.Hq = Hq, p.Hk = Hk, p.stride = stride, p.max_len = max_len, p.window = window;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  return g4::attn_int4(fn, p, d, d_scratch, scratch_bytes, true);
+}
+
+long long granite4_prefill_attention_int4_scratch_bytes(int rows, int base_pos, int Hq, int Hk, int d) {
+  if (rows <= 0 || base_pos < 0 || base_pos > INT_MAX - rows || !g4::int4_shape_ok(Hq, Hk, d, 1)) return -1;
+  if (g4::widens(rows, Hq, Hk, d)) return g4::widened_bytes(static_cast<long long>(base_pos) + rows, Hk);
+  return g4::plan_int4(rows, g4::prefill_group(Hq, Hk), Hq, Hk, d, base_pos + rows).bytes;
+}
+
+int granite4_prefill_attention_int4(const uint16_t* d_q_rot, float scale, int Hq, int Hk, int d, int base_pos, int rows,
+                                    int stride, uint16_t* d_out, const uint8_t* d_cache_k, const uint8_t* d_cache_v,
+                                    const float* d_k_scale, const float* d_v_scale, const int* d_pt, void* d_scratch,
+                                    long long scratch_bytes) {
+  const char* fn = "granite4_prefill_attention_int4";
+  if (d_q_rot == nullptr || d_cache_k == nullptr || d_cache_v == nullptr || d_k_scale == nullptr ||
+      d_v_scale == nullptr || d_out == nullptr || base_pos < 0 || rows <= 0 || base_pos > INT_MAX - rows || stride <= 0 ||
+      (d_pt == nullptr && base_pos + rows > stride) || !std::isfinite(scale))
+    return g4::fail(fn, "invalid arguments");
+  if (!g4::int4_shape_ok(Hq, Hk, d, 1))
+    return g4::fail(fn, "head dims of 64 and 128; Hq a multiple of Hk; at most 64 query heads a kv head");
+  if (!g4::aligned16(d_q_rot) || !g4::aligned16(d_cache_k) || !g4::aligned16(d_cache_v))
+    return g4::fail(fn, "q and the caches must be 16-byte aligned");
+  const int n = base_pos + rows;
+  if (g4::widens(rows, Hq, Hk, d)) {
+    if (d_scratch == nullptr || !g4::aligned16(d_scratch) || scratch_bytes < g4::widened_bytes(n, Hk))
+      return g4::fail(fn, "scratch missing, misaligned or smaller than the size the scratch query returns");
+    const size_t codes = static_cast<size_t>(n) * Hk * 128, scales = static_cast<size_t>(n) * Hk;
+    int8_t* ck = static_cast<int8_t*>(d_scratch);
+    int8_t* cv = ck + codes;
+    float* ks = reinterpret_cast<float*>(cv + codes);
+    float* vs = ks + scales;
+    if (g4::widen_int4(fn, d_cache_k, d_cache_v, d_k_scale, d_v_scale, d_pt, Hk, stride, n, ck, cv, ks, vs) != 0) return -1;
+    return granite4_prefill_attention_int8(d_q_rot, scale, Hq, Hk, d, base_pos, rows, n, d_out, ck, cv, ks, vs, nullptr,
+                                           nullptr, 0);
+  }
+  g4::Int4AttnParams p{};
+  p.q = d_q_rot, p.ck = d_cache_k, p.cv = d_cache_v, p.ks = d_k_scale, p.vs = d_v_scale, p.out = d_out;
+  p.base_pos = base_pos, p.pt = d_pt;
+  p.rows = rows, p.per = g4::prefill_group(Hq, Hk), p.Hq = Hq, p.Hk = Hk, p.stride = stride, p.max_len = n;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  return g4::attn_int4(fn, p, d, d_scratch, scratch_bytes, false);
+}
+
+}  // extern "C"

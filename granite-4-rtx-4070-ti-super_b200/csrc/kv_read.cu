@@ -1,0 +1,141 @@
+// Rows of the quantised paged pool read back: as bf16 values, or (for the prefill attention over a 4-bit
+// pool) as an 8-bit pool with the sequence's positions in order.
+//
+//   out[i][h][:] = bf16(code * scale) of pool row kv_rows[i]
+//
+// A 4-bit code is an 8-bit code as it stands (both mean code * scale), so the second form loses nothing.
+#include "g4_host.h"
+#include "g4_math.cuh"
+
+#include "../../include/granite4_b200.h"
+
+namespace g4 {
+namespace {
+
+constexpr int kReadThreads = 256;
+
+// Eight codes of a 4-bit word as signed bytes: nibble - 8 in each byte.
+__device__ __forceinline__ uint2 nibbles_to_bytes(uint32_t w) {
+  const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+  const uint32_t lo = __byte_perm(even, odd, 0x5140), hi = __byte_perm(even, odd, 0x7362);
+  // bytewise nibble - 8: the subtraction never borrows across bytes when the top bit is set first
+  return make_uint2(((lo | 0x80808080u) - 0x08080808u) ^ 0x80808080u, ((hi | 0x80808080u) - 0x08080808u) ^ 0x80808080u);
+}
+
+__device__ __forceinline__ float byte_value(uint32_t w, int i) {
+  return static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+}
+
+struct ReadParams {
+  const uint8_t* ck;
+  const uint8_t* cv;
+  const float* ks;
+  const float* vs;
+  const int* kv_rows;
+  uint16_t* k_out;
+  uint16_t* v_out;
+  int Hk;
+  long long stride, n;
+};
+
+// A thread reads eight codes and writes 16 bytes; consecutive threads follow the output.
+template <int D, int BITS>
+__global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const ReadParams p) {
+  pdl_begin();
+  constexpr int kParts = D / 8;
+  const long long items = p.n * p.Hk * kParts;
+  const long long i = static_cast<long long>(blockIdx.x) * kReadThreads + threadIdx.x;
+  if (i >= items) return;
+  const int part = static_cast<int>(i % kParts);
+  const long long rh = i / kParts;
+  const int h = static_cast<int>(rh % p.Hk);
+  const int row = __ldg(p.kv_rows + rh / p.Hk);
+  const bool have = row >= 0 && row < p.stride;
+  const size_t srow = static_cast<size_t>(h) * p.stride + (have ? row : 0);
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint8_t* cache = (kv ? p.cv : p.ck) + srow * (D * BITS / 8);
+    const float s = have ? __ldg((kv ? p.vs : p.ks) + srow) : 0.0f;
+    uint2 w = make_uint2(0u, 0u);
+    if (have) w = BITS == 4 ? nibbles_to_bytes(__ldg(reinterpret_cast<const uint32_t*>(cache) + part)) : __ldg(reinterpret_cast<const uint2*>(cache) + part);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = byte_value(e < 4 ? w.x : w.y, e & 3) * s;
+    st_stream(reinterpret_cast<uint4*>(kv ? p.v_out : p.k_out) + i, pack8(v));
+  }
+}
+
+struct WidenParams {
+  const uint8_t* ck;
+  const uint8_t* cv;
+  const float* ks;
+  const float* vs;
+  const int* pt;
+  int8_t* ok;
+  int8_t* ov;
+  float* oks;
+  float* ovs;
+  int Hk;
+  long long stride, n;
+};
+
+// Positions [0, n) of a sequence out of the 4-bit pool into an 8-bit pool [Hk][n][128] in their order.
+__global__ void __launch_bounds__(kReadThreads) kv_widen_kernel(const WidenParams p) {
+  pdl_begin();
+  constexpr int kParts = 128 / 16;  // a thread: 8 bytes in, 16 out
+  const long long i = static_cast<long long>(blockIdx.x) * kReadThreads + threadIdx.x;
+  if (i >= p.n * p.Hk * kParts) return;
+  const int part = static_cast<int>(i % kParts);
+  const long long hp = i / kParts, pos = hp % p.n;
+  const int h = static_cast<int>(hp / p.n);
+  long long row = p.pt != nullptr ? __ldg(p.pt + pos) : pos;
+  row = row < 0 ? 0 : (row >= p.stride ? p.stride - 1 : row);
+  const size_t srow = static_cast<size_t>(h) * p.stride + row;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>((kv ? p.cv : p.ck) + srow * 64) + part);
+    const uint2 a = nibbles_to_bytes(w.x), b = nibbles_to_bytes(w.y);
+    reinterpret_cast<uint4*>(kv ? p.ov : p.ok)[i] = make_uint4(a.x, a.y, b.x, b.y);
+    if (part == 0) (kv ? p.ovs : p.oks)[hp] = __ldg((kv ? p.vs : p.ks) + srow);
+  }
+}
+
+template <int D, int BITS>
+int launch_read(const char* fn, const ReadParams& p) {
+  const long long blocks = (p.n * p.Hk * (D / 8) + kReadThreads - 1) / kReadThreads;
+  if (blocks > INT_MAX) return fail(fn, "too many rows");
+  G4_LAUNCH_PDL(fn, (kv_read_kernel<D, BITS>), dim3(static_cast<unsigned>(blocks)), dim3(kReadThreads), 0, current_stream(), p);
+  return 0;
+}
+
+}  // namespace
+
+// Used by the prefill attention over a 4-bit pool (attn_int4.cu); out: codes [2][Hk][n][128], scales [2][Hk][n].
+int widen_int4(const char* fn, const uint8_t* ck, const uint8_t* cv, const float* ks, const float* vs, const int* pt,
+               int Hk, long long stride, long long n, int8_t* ok, int8_t* ov, float* oks, float* ovs) {
+  WidenParams p{ck, cv, ks, vs, pt, ok, ov, oks, ovs, Hk, stride, n};
+  const long long blocks = (n * Hk * 8 + kReadThreads - 1) / kReadThreads;
+  if (blocks > INT_MAX) return fail(fn, "too many positions");
+  G4_LAUNCH_PDL(fn, kv_widen_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kReadThreads), 0, current_stream(), p);
+  return 0;
+}
+
+}  // namespace g4
+
+extern "C" int granite4_kernel_kv_read_paged(const void* d_cache_k, const void* d_cache_v, const float* d_k_scale,
+                                             const float* d_v_scale, const int* d_kv_rows, int rows, int bits, int Hk,
+                                             int d, int stride, uint16_t* d_k_out, uint16_t* d_v_out) {
+  const char* fn = "granite4_kernel_kv_read_paged";
+  if (d_cache_k == nullptr || d_cache_v == nullptr || d_k_scale == nullptr || d_v_scale == nullptr ||
+      d_kv_rows == nullptr || d_k_out == nullptr || d_v_out == nullptr || rows <= 0 || Hk <= 0 || Hk > 65535 || stride <= 0)
+    return g4::fail(fn, "invalid arguments");
+  if ((d != 64 && d != 128) || (bits != 4 && bits != 8)) return g4::fail(fn, "head dims of 64 and 128, pools of 4 and 8 bits");
+  if (!g4::aligned16(d_cache_k) || !g4::aligned16(d_cache_v) || !g4::aligned16(d_k_out) || !g4::aligned16(d_v_out))
+    return g4::fail(fn, "pointers must be 16-byte aligned");
+  g4::ReadParams p{};
+  p.ck = static_cast<const uint8_t*>(d_cache_k), p.cv = static_cast<const uint8_t*>(d_cache_v);
+  p.ks = d_k_scale, p.vs = d_v_scale, p.kv_rows = d_kv_rows, p.k_out = d_k_out, p.v_out = d_v_out;
+  p.Hk = Hk, p.stride = stride, p.n = rows;
+  if (d == 128) return bits == 4 ? g4::launch_read<128, 4>(fn, p) : g4::launch_read<128, 8>(fn, p);
+  return bits == 4 ? g4::launch_read<64, 4>(fn, p) : g4::launch_read<64, 8>(fn, p);
+}

@@ -44,7 +44,8 @@ constexpr Types kU8 = type_bit(at::kByte), kI8 = type_bit(at::kChar);
   X(granite4_kernel_argmax_rows) X(granite4_kernel_argmax_advance) X(granite4_gpu_multi_embed)                  \
   X(granite4_kernel_multi_scatter_advance) X(granite4_kernel_attn_decode_int8_paged) X(granite4_attn_split_int8) \
   X(granite4_prefill_attention_int8) X(granite4_kernel_fp8_encode_with_amax) X(granite4_kernel_gemm_fp8)        \
-  X(granite4_prefill_silu_mul) X(granite4_kernel_swiglu_fp8)
+  X(granite4_prefill_silu_mul) X(granite4_kernel_swiglu_fp8) X(granite4_kernel_qk_norm_rope_kv_paged)           \
+  X(granite4_kernel_kv_read_paged) X(granite4_kernel_attn_decode_int4_paged) X(granite4_prefill_attention_int4)
 
 struct Api {
 #define X(name) decltype(&::name) name;
@@ -102,6 +103,23 @@ T* ptr(PyObject* o, Types types = kAny) {
     throw PyErrorSet{};
   }
   return static_cast<T*>(t.data_ptr());
+}
+
+// The same of a tensor on `dev` that holds at least n elements (n < 0: of sizes the launcher refuses).
+template <typename T = void>
+T* ptr_of(PyObject* o, Types types, c10::Device dev, long long n, const char* what) {
+  T* p = ptr<T>(o, types);
+  if (o == Py_None) return p;
+  const at::Tensor& t = tensor(o);
+  if (t.device() != dev) {
+    PyErr_Format(PyExc_ValueError, "%s is not on the device of the first tensor", what);
+    throw PyErrorSet{};
+  }
+  if (t.numel() < n) {
+    PyErr_Format(PyExc_ValueError, "%s holds %lld elements, %lld are needed", what, static_cast<long long>(t.numel()), n);
+    throw PyErrorSet{};
+  }
+  return p;
 }
 
 // A float32 table: a tensor or an integer device address.
@@ -412,6 +430,61 @@ OP(rope_kv_int8_paged, 16) {  // qkv, cos, sin, pos_rows, kv_rows, Hq, Hk, d, st
   });
 }
 
+OP(qk_norm_rope_kv_paged, 19) {
+  // qkv, q_norm, k_norm, eps, cos, sin, pos_rows, kv_rows, Hq, Hk, d, stride, max_pos, bits, q_rot, ck, cv, ks, vs
+  const at::Tensor& t = matrix(a[0]);
+  enter(t);
+  const auto dev = t.device();
+  const long long rows = t.size(0), Hq = num(a[8]), Hk = num(a[9]), d = num(a[10]), stride = num(a[11]), max_pos = num(a[12]);
+  const int bits = num(a[13]);
+  const float eps = real(a[3]);
+  const Types code = bits == 4 ? kU8 : kI8;
+  const long long codes = Hk * stride * d * bits / 8, half = max_pos * (d / 2);
+  const auto* qkv = ptr_of<const uint16_t>(a[0], kBf16, dev, rows * (Hq + 2 * Hk) * d, "qkv");
+  const auto* wq = ptr_of<const uint16_t>(a[1], kBf16, dev, d, "q_norm");
+  const auto* wk = ptr_of<const uint16_t>(a[2], kBf16, dev, d, "k_norm");
+  const float* c = PyLong_Check(a[4]) ? table(a[4]) : ptr_of<const float>(a[4], kF32, dev, half, "cos_tbl");
+  const float* s = PyLong_Check(a[5]) ? table(a[5]) : ptr_of<const float>(a[5], kF32, dev, half, "sin_tbl");
+  const auto* pos = ptr_of<const int>(a[6], kI32, dev, rows, "pos_rows");
+  const auto* kvr = ptr_of<const int>(a[7], kI32, dev, rows, "kv_rows");
+  auto* q = ptr_of<uint16_t>(a[14], kBf16, dev, rows * Hq * d, "q_rot");
+  auto* ck = ptr_of(a[15], code, dev, codes, "cache_k");
+  auto* cv = ptr_of(a[16], code, dev, codes, "cache_v");
+  auto* ks = ptr_of<float>(a[17], kF32, dev, Hk * stride, "k_scale");
+  auto* vs = ptr_of<float>(a[18], kF32, dev, Hk * stride, "v_scale");
+  return launched([&] {
+    return api.granite4_kernel_qk_norm_rope_kv_paged(qkv, wq, wk, eps, c, s, pos, kvr, static_cast<int>(rows),
+                                                     static_cast<int>(Hq), static_cast<int>(Hk), static_cast<int>(d),
+                                                     static_cast<int>(stride), static_cast<int>(max_pos), bits, q, ck, cv,
+                                                     ks, vs);
+  });
+}
+
+OP(kv_read_paged, 11) {  // ck, cv, ks, vs, kv_rows, bits, Hk, d, stride, k_out, v_out
+  const at::Tensor& t = tensor(a[0]);
+  enter(t);
+  const auto dev = t.device();
+  const int bits = num(a[5]);
+  const long long Hk = num(a[6]), d = num(a[7]), stride = num(a[8]), rows = tensor(a[4]).numel();
+  const Types code = bits == 4 ? kU8 : kI8;
+  const long long codes = Hk * stride * d * bits / 8;
+  const auto* ck = ptr_of(a[0], code, dev, codes, "cache_k");
+  const auto* cv = ptr_of(a[1], code, dev, codes, "cache_v");
+  const auto* ks = ptr_of<const float>(a[2], kF32, dev, Hk * stride, "k_scale");
+  const auto* vs = ptr_of<const float>(a[3], kF32, dev, Hk * stride, "v_scale");
+  const auto* kvr = ptr_of<const int>(a[4], kI32, dev, rows, "kv_rows");
+  auto* ko = ptr_of<uint16_t>(a[9], kBf16, dev, rows * Hk * d, "k_out");
+  auto* vo = ptr_of<uint16_t>(a[10], kBf16, dev, rows * Hk * d, "v_out");
+  if (rows > INT32_MAX) {
+    PyErr_SetString(PyExc_ValueError, "too many rows");
+    return nullptr;
+  }
+  return launched([&] {
+    return api.granite4_kernel_kv_read_paged(ck, cv, ks, vs, kvr, static_cast<int>(rows), bits, static_cast<int>(Hk),
+                                             static_cast<int>(d), static_cast<int>(stride), ko, vo);
+  });
+}
+
 // ---- decode-step glue -----------------------------------------------------------------------------
 OP(argmax_rows, 4) {  // logits, out, d_pos, vocab_map
   const at::Tensor& t = matrix(a[0]);
@@ -529,6 +602,54 @@ OP(prefill_attention_int8, 14) {  // q_rot, scale, Hq, Hk, d, base_pos, stride, 
   });
 }
 
+OP(attn_decode_int4_paged, 18) {
+  // q, ck, cv, ks, vs, row_pos, Hq, Hk, d, stride, max_len, scale, out, rows_per_group, row_pt, pt, window, scratch
+  const at::Tensor& t = matrix(a[0]);
+  enter(t);
+  const auto dev = t.device();
+  const long long rows = t.size(0), Hq = num(a[6]), Hk = num(a[7]), d = num(a[8]), stride = num(a[9]);
+  const int max_len = num(a[10]), per = num(a[13]), window = num(a[16]);
+  const float scale = real(a[11]);
+  const auto* q = ptr_of<const uint16_t>(a[0], kBf16, dev, rows * Hq * d, "q");
+  const auto* ck = ptr_of<const uint8_t>(a[1], kU8, dev, Hk * stride * d / 2, "cache_k");
+  const auto* cv = ptr_of<const uint8_t>(a[2], kU8, dev, Hk * stride * d / 2, "cache_v");
+  const auto* ks = ptr_of<const float>(a[3], kF32, dev, Hk * stride, "k_scale");
+  const auto* vs = ptr_of<const float>(a[4], kF32, dev, Hk * stride, "v_scale");
+  const auto* pos = ptr_of<const int>(a[5], kI32, dev, rows, "row_pos");
+  auto* out = ptr_of<uint16_t>(a[12], kBf16, dev, rows * Hq * d, "out");
+  const auto* row_pt = reinterpret_cast<const int* const*>(ptr_of<const int64_t>(a[14], kI64, dev, rows, "row_pt"));
+  const auto* pt = ptr_of<const int>(a[15], kI32, dev, max_len, "pt");
+  void* scr = ptr_of(a[17], kU8, dev, 0, "scratch");
+  const long long bytes = a[17] == Py_None ? 0 : tensor(a[17]).numel();
+  return launched([&] {
+    return api.granite4_kernel_attn_decode_int4_paged(q, ck, cv, ks, vs, pos, row_pt, pt, static_cast<int>(rows), per,
+                                                      static_cast<int>(Hq), static_cast<int>(Hk), static_cast<int>(d),
+                                                      static_cast<int>(stride), max_len, window, scale, scr, bytes, out);
+  });
+}
+
+OP(prefill_attention_int4, 14) {  // q_rot, scale, Hq, Hk, d, base_pos, stride, out, ck, cv, ks, vs, pt, scratch
+  const at::Tensor& t = matrix(a[0]);
+  enter(t);
+  const auto dev = t.device();
+  const float scale = real(a[1]);
+  const long long rows = t.size(0), Hq = num(a[2]), Hk = num(a[3]), d = num(a[4]), base = num(a[5]), stride = num(a[6]);
+  const auto* q = ptr_of<const uint16_t>(a[0], kBf16, dev, rows * Hq * d, "q_rot");
+  auto* out = ptr_of<uint16_t>(a[7], kBf16, dev, rows * Hq * d, "out");
+  const auto* ck = ptr_of<const uint8_t>(a[8], kU8, dev, Hk * stride * d / 2, "cache_k");
+  const auto* cv = ptr_of<const uint8_t>(a[9], kU8, dev, Hk * stride * d / 2, "cache_v");
+  const auto* ks = ptr_of<const float>(a[10], kF32, dev, Hk * stride, "k_scale");
+  const auto* vs = ptr_of<const float>(a[11], kF32, dev, Hk * stride, "v_scale");
+  const auto* pt = ptr_of<const int>(a[12], kI32, dev, base + rows, "pt");
+  void* scr = ptr_of(a[13], kU8, dev, 0, "scratch");
+  const long long bytes = a[13] == Py_None ? 0 : tensor(a[13]).numel();
+  return launched([&] {
+    return api.granite4_prefill_attention_int4(q, scale, static_cast<int>(Hq), static_cast<int>(Hk), static_cast<int>(d),
+                                               static_cast<int>(base), static_cast<int>(rows), static_cast<int>(stride),
+                                               out, ck, cv, ks, vs, pt, scr, bytes);
+  });
+}
+
 // ---- FP8 GEMM -----------------------------------------------------------------------------------------
 // The items of any iterable, as a tuple that this object owns.
 struct Items {
@@ -635,6 +756,7 @@ PyMethodDef methods[] = {
     FAST(rope_at_pos), FAST(rope_at_pos_batched), FAST(kv_append_batched), FAST(verify_qkv_stage),
     FAST(prefill_rope_split_append), FAST(rope_kv_int8_paged), FAST(argmax_rows), FAST(argmax_advance),
     FAST(gpu_multi_embed), FAST(multi_scatter_advance), FAST(attn_decode_int8_paged), FAST(attn_split_int8),
+    FAST(qk_norm_rope_kv_paged), FAST(kv_read_paged), FAST(attn_decode_int4_paged), FAST(prefill_attention_int4),
     FAST(prefill_attention_int8), FAST(gemm_fp8), FAST(prefill_silu_mul), FAST(swiglu_fp8), FAST(enter_device_of),
     {nullptr, nullptr, 0, nullptr}};
 

@@ -222,6 +222,22 @@ def rope_kv_int8_paged(qkv, cos_tbl, sin_tbl, pos_rows, kv_rows, Hq, Hk, d, stri
                                  q_rot, cache_k, cache_v, k_scale, v_scale)
 
 
+def qk_norm_rope_kv_paged(qkv, q_norm, k_norm, eps, cos_tbl, sin_tbl, pos_rows, kv_rows, Hq, Hk, d, stride, max_pos, bits,
+                          q_rot, cache_k, cache_v, k_scale, v_scale):
+    """granite4_kernel_qk_norm_rope_kv_paged: per-head RMSNorm of q and k (weights bf16 [d]; None: no norm),
+    rotation, K and V quantised into pool rows kv_rows. bits 4: uint8 pool [Hk][stride][d / 2], codes in
+    [-7, 7] kept as code + 8, the even dim in the low half of its byte; bits 8: the int8 pool [Hk][stride][d].
+    d 64 or 128. Rows whose position or pool row is out of range are skipped."""
+    return _n.qk_norm_rope_kv_paged(qkv, q_norm, k_norm, eps, cos_tbl, sin_tbl, pos_rows, kv_rows, Hq, Hk, d, stride, max_pos,
+                                    bits, q_rot, cache_k, cache_v, k_scale, v_scale)
+
+
+def kv_read_paged(cache_k, cache_v, k_scale, v_scale, kv_rows, bits, Hk, d, stride, k_out, v_out):
+    """granite4_kernel_kv_read_paged: k_out / v_out [rows][Hk][d] = bf16(code * scale) of the pool rows kv_rows
+    (4- or 8-bit pool); a row outside [0, stride) gives zeros."""
+    return _n.kv_read_paged(cache_k, cache_v, k_scale, v_scale, kv_rows, bits, Hk, d, stride, k_out, v_out)
+
+
 # ---- decode-step glue -----------------------------------------------------------------------
 def argmax_rows(logits, out, d_pos=None, vocab_map=None):
     """granite4_kernel_argmax_rows: first index of each row's maximum of bf16 logits [rows][V]."""
@@ -292,6 +308,41 @@ def prefill_attention_int8(q_rot, scale, Hq, Hk, d, base_pos, stride, out, cache
     attention of q_rot's rows at positions base_pos, base_pos + 1, ... of one sequence."""
     return _n.prefill_attention_int8(q_rot, scale, Hq, Hk, d, base_pos, stride, out, cache_k, cache_v, k_scale, v_scale,
                                      pt, scratch)
+
+
+def attn_decode_int4_scratch_bytes(rows, rows_per_group, Hq, Hk, d, max_len):
+    """Scratch of attn_decode_int4_paged on the current device (0: none wanted, -1: not built)."""
+    return capi.lib().granite4_attn_decode_int4_scratch_bytes(rows, rows_per_group, Hq, Hk, d, max_len)
+
+
+def attn_decode_int4_paged(q, cache_k, cache_v, k_scale, v_scale, row_pos, Hq, Hk, d, stride, max_len, scale, out,
+                           rows_per_group=1, row_pt=None, pt=None, window=0, scratch=None):
+    """granite4_kernel_attn_decode_int4_paged: attention of decode / verify rows over the 4-bit pool. Any Hq / Hk
+    with rows_per_group * Hq / Hk <= 64, d 64 or 128; window > 0: a row sees its last `window` positions. row_pt:
+    int64 CUDA tensor of per-row table addresses (a group uses its first row's), pt: one int32 table for every
+    row; scratch: uint8 CUDA tensor of at least attn_decode_int4_scratch_bytes(...) bytes (allocated here when
+    not given)."""
+    if scratch is None:
+        _n.enter_device_of(q)  # the size depends on the device
+        need = capi.lib().granite4_attn_decode_int4_scratch_bytes(q.shape[0], rows_per_group, Hq, Hk, d, max_len)
+        if need > 0:
+            scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    return _n.attn_decode_int4_paged(q, cache_k, cache_v, k_scale, v_scale, row_pos, Hq, Hk, d, stride, max_len, scale, out,
+                                     rows_per_group, row_pt, pt, window, scratch)
+
+
+def prefill_attention_int4(q_rot, scale, Hq, Hk, d, base_pos, stride, out, cache_k, cache_v, k_scale, v_scale,
+                           pt=None, scratch=None):
+    """granite4_prefill_attention_int4: causal attention of q_rot's rows at positions base_pos, base_pos + 1, ... of one
+    sequence over the 4-bit pool. scratch: uint8 CUDA tensor of at least
+    granite4_prefill_attention_int4_scratch_bytes(...) bytes (allocated here when not given)."""
+    if scratch is None:
+        _n.enter_device_of(q_rot)  # the size depends on the device
+        need = capi.lib().granite4_prefill_attention_int4_scratch_bytes(q_rot.shape[0], base_pos, Hq, Hk, d)
+        if need > 0:
+            scratch = torch.empty(need, dtype=torch.uint8, device=q_rot.device)
+    return _n.prefill_attention_int4(q_rot, scale, Hq, Hk, d, base_pos, stride, out, cache_k, cache_v, k_scale, v_scale, pt,
+                                     scratch)
 
 
 # ---- FP8 x FP8 GEMM -----------------------------------------------------------------------

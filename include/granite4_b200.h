@@ -279,6 +279,36 @@ int granite4_kernel_rope_kv_int8_paged(const uint16_t* d_qkv, const float* d_cos
                                        uint16_t* d_q_rot, int8_t* d_cache_k, int8_t* d_cache_v,
                                        float* d_k_scale, float* d_v_scale);
 
+/* Added: RMSNorm of every query and key head, RoPE, and K / V quantised into a
+ * paged pool, in one pass over the rows of a token-major qkv [rows][(Hq + 2 Hk) d]:
+ *   n = x * r * w, r = 1 / sqrt(mean(x^2) + eps) over the head's d values, with w =
+ *   d_q_norm / d_k_norm, bf16 [d] (either may be NULL: that side is not normed);
+ *   q_rot = bf16(rope(n)); K = rope(n) and V as it is are quantised per (row, head):
+ *   scale = float(amax / top), code = sign * floor(|x| / scale + 1/2).
+ * bits 8: top 127, the int8 pool [Hk][stride][d] of the entry points above. bits 4:
+ * top 7, uint8 [Hk][stride][d / 2], code + 8 in a nibble, the even dim in the low half
+ * of its byte. Scales are f32 [Hk][stride] for both. Codes are those of exact
+ * arithmetic on the bf16 inputs and the f32 tables (a row that holds an infinity
+ * or a NaN gets unspecified codes in [-top, top]). d is 64 or 128; eps > 0; norm weights,
+ * tables, qkv, q_rot and caches 16-byte aligned. d_pos_rows / d_kv_rows as in
+ * granite4_kernel_rope_kv_int8_paged: a row with an index out of range is skipped;
+ * pool rows of one call are distinct. For granite4_kernel_kv_move a 4-bit pool is one
+ * of bits 8 with d / 2 in the place of d. */
+int granite4_kernel_qk_norm_rope_kv_paged(const uint16_t* d_qkv, const uint16_t* d_q_norm,
+                                          const uint16_t* d_k_norm, float eps, const float* d_cos,
+                                          const float* d_sin, const int* d_pos_rows,
+                                          const int* d_kv_rows, int rows, int Hq, int Hk, int d,
+                                          int stride, int max_pos, int bits, uint16_t* d_q_rot,
+                                          void* d_cache_k, void* d_cache_v, float* d_k_scale,
+                                          float* d_v_scale);
+/* Added: pool rows read back. d_k_out / d_v_out [rows][Hk][d] = bf16(code * scale) of
+ * pool rows d_kv_rows[0 .. rows) of a 4- or 8-bit pool (bits); a row outside [0,
+ * stride) gives zeros. d is 64 or 128; caches and outputs 16-byte aligned. */
+int granite4_kernel_kv_read_paged(const void* d_cache_k, const void* d_cache_v,
+                                  const float* d_k_scale, const float* d_v_scale,
+                                  const int* d_kv_rows, int rows, int bits, int Hk, int d,
+                                  int stride, uint16_t* d_k_out, uint16_t* d_v_out);
+
 /* ------------------------------------------------------------------------ */
 /* Decode-step glue around the path: greedy pick, token chaining, KV moves   */
 /* ------------------------------------------------------------------------ */
@@ -501,6 +531,40 @@ int granite4_attn_split_int8(const uint16_t* d_q, const int8_t* d_cache_k8, cons
                              int max_len, const int* d_row_pos, const int* const* d_row_pt,
                              const int* d_row_grp, int ngroups, const int* d_row_tbase,
                              const int* d_row_tail, int window);
+
+/* Added: the decode / verify attention over the 4-bit pool of
+ * granite4_kernel_qk_norm_rope_kv_paged. Arguments as
+ * granite4_kernel_attn_decode_int8_paged, but: any Hq that is a multiple of Hk with
+ * rows_per_group * Hq / Hk <= 64, d 64 or 128; window > 0 lets row r see positions
+ * (pos - window, pos] only; d_out may lie on any 2-byte boundary. max_len bounds every
+ * position + 1 (a larger position counts as max_len - 1) and sizes the scratch; d_scratch
+ * must hold granite4_attn_decode_int4_scratch_bytes(...) bytes of the same device, 16-byte
+ * aligned (0: NULL will do), and belongs to one call at a time. The rows' table entries
+ * are read only for positions that some row of the group sees. A row with a negative
+ * position gets zeros; the rows of a group may have any positions. The cache is cut into
+ * equal shares whatever the sequences' lengths, and the order of every sum follows from
+ * the arguments and positions alone: the same call gives the same bits. */
+long long granite4_attn_decode_int4_scratch_bytes(int rows, int rows_per_group, int Hq, int Hk, int d,
+                                                  int max_len);
+int granite4_kernel_attn_decode_int4_paged(const uint16_t* d_q, const uint8_t* d_cache_k,
+                                           const uint8_t* d_cache_v, const float* d_k_scale,
+                                           const float* d_v_scale, const int* d_row_pos,
+                                           const int* const* d_row_pt, const int* d_pt, int rows,
+                                           int rows_per_group, int Hq, int Hk, int d, int stride,
+                                           int max_len, int window, float scale, void* d_scratch,
+                                           long long scratch_bytes, uint16_t* d_out);
+/* Added: granite4_prefill_attention_int8 over the 4-bit pool. Chunks of 32 rows or more
+ * with d 128 and Hq == 4 Hk widen the sequence's rows into an 8-bit pool in d_scratch
+ * (exact: a 4-bit code is an 8-bit code with the same scale; 264 bytes per position and kv
+ * head) and run the kernels of that entry point; everything else runs on the decode
+ * kernel, where d_scratch is optional (without it no range is split). d_scratch must hold
+ * granite4_prefill_attention_int4_scratch_bytes(...) bytes, 16-byte aligned. */
+long long granite4_prefill_attention_int4_scratch_bytes(int rows, int base_pos, int Hq, int Hk, int d);
+int granite4_prefill_attention_int4(const uint16_t* d_q_rot, float scale, int Hq, int Hk, int d,
+                                    int base_pos, int rows, int stride, uint16_t* d_out,
+                                    const uint8_t* d_cache_k, const uint8_t* d_cache_v,
+                                    const float* d_k_scale, const float* d_v_scale, const int* d_pt,
+                                    void* d_scratch, long long scratch_bytes);
 
 /* ------------------------------------------------------------------------ */
 /* a4. SwiGLU, bf16 and FP8 outputs                                          */
