@@ -16,13 +16,14 @@
 //  * Both contractions have the cache positions on the 16-row side (S^T = K Q^T) or the 16-deep side (O^T = V^T P^T)
 //    of mma.sync m16n8k16 and the (query row, head) pairs on the 8-column side. Which dims a lane's fragment
 //    elements stand for is free as long as q's match, so a lane's K elements are 16 consecutive bytes of a row and
-//    its V elements 8: both are loaded from global memory straight into the registers the masks are applied to.
+//    its V elements 8: both are loaded straight into the registers the masks are applied to.
 // P is rounded to fp16 (11 bits; everything else is f32) after the multiplication with v_scale and a power of two
 // that puts the largest v_scale seen at 2^12, so values of any magnitude keep the format's precision.
 //
 // Work split: the (group, kv head, column block) segments' tiles of 32 positions form one line, cut into equal
 // shares, one CTA each, whatever the sequences' lengths (read on the device). A CTA's four warps take every fourth
-// tile of a segment's piece, each with its own running (max, sum, O); they merge in shared memory. Pieces of a
+// tile of a segment's piece, each with its own ring of asynchronous copies and its own running (max, sum, O); they
+// merge in shared memory. Pieces of a
 // segment that more than one CTA worked on are joined by a second small kernel, in order of the CTAs.
 #include "g4_host.h"
 #include "g4_math.cuh"
@@ -32,6 +33,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 namespace g4 {
 
@@ -44,7 +46,8 @@ namespace {
 constexpr int kTile = 32;     // positions a warp works on at a time
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxGroups = 1024;  // of a launch that splits the line of tiles
+constexpr int kMaxGroups = 512;   // of a launch that splits the line of tiles
+constexpr int kMaxShares = 1024;  // it is cut into
 constexpr int kMaxColumns = 64;   // rows of a group x query heads of a kv head
 
 struct Int4AttnParams {
@@ -137,24 +140,47 @@ __device__ __forceinline__ long long shares_of(long long all, int shares) {
   return min(static_cast<long long>(shares), (all + kWarps - 1) / kWarps);
 }
 
-// The codes and scales of one tile as a lane holds them. K: rows g, g + 8, g + 16, g + 24 of the tile, a quarter of
-// the dims each; V: rows 2t, 2t + 1, 2t + 8, 2t + 9 (+ 16), an eighth of the dims each; scales of row `lane`.
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4_async(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A warp's ring of raw tiles: 32 K rows, 32 V rows, their scales, as they are in the pool (what no row sees: zeros).
+// Row r of a block of eight, as the mma operands count them, is position r (r < 4) or r ^ 1 of the block: with that
+// order, and the 16-byte pieces of V rows 2, 3, 6 and 7 of a block exchanged in pairs, the lanes' reads of either
+// operand meet no bank twice.
+constexpr int kStages = 3;
 template <int D>
-struct Tile {
-  uint32_t k[4][D / 32];
-  uint32_t v[8][D / 64];
-  float sk, sv;
-};
+constexpr int kRowBytes = D / 2;
+template <int D>
+constexpr int kStageBytes = 2 * kTile * kRowBytes<D> + 2 * kTile * 4;
+template <int D>
+constexpr int kWarpBytes = kStages * kStageBytes<D>;
+constexpr int kPad = 4;  // floats after a parked row of O
 
 // NT column tiles of 8: column 8 nt + i of column block cb is (query row c / G, query head c % G), c = 8 NT cb + 8 nt + i.
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(const Int4AttnParams p) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) attn_int4_kernel(const Int4AttnParams p) {
+  // a launch that splits the line is one resident wave: what comes next may be staged beside it
+  if (p.split) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   pdl_begin();
   constexpr int kC = 8 * NT, kW = D / 32 /* K words of a row per lane */, kM = D / 16 /* 16-dim tiles of O^T */;
+  constexpr int kRB = kRowBytes<D>, kVAt = kTile * kRB, kSAt = 2 * kTile * kRB;
+  static_assert(kWarpBytes<D> >= kC * (D + kPad) * 4 + kC * 8, "a warp parks its state in its ring");
   __shared__ int s_prefix[kMaxGroups + 1];
-  __shared__ __align__(16) float s_o[kWarps][kC][D + 4];
-  __shared__ float s_ml[kWarps][kC][2];
+  extern __shared__ __align__(128) unsigned char s_ring[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  unsigned char* const ring = s_ring + warp * kWarpBytes<D>;
+  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  const int pg = g < 4 ? g : g ^ 1;                                // position of row g
+  const int v_even = 2 * t + (t >> 1), v_odd = 2 * t + 1 - (t >> 1);  // positions of rows 2t, 2t + 1
   const int per_group = p.Hk * p.blocks;
   long long x = 0, x_end = 0;  // this CTA's share of the line of tiles
   int grp = 0, sub = 0;
@@ -197,51 +223,47 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(co
     const int hkv = sub / p.blocks, c0 = (sub % p.blocks) * kC;
     const int r0 = grp * p.per, nrows = min(p.per, p.rows - r0), columns = min(kC, nrows * p.G - c0);
     const size_t head_row0 = static_cast<size_t>(hkv) * p.stride;
-    const uint8_t* ck = p.ck + head_row0 * (D / 2) + t * (D / 8);
-    const uint8_t* cv = p.cv + head_row0 * (D / 2) + g * (D / 16);
+    const uint8_t* ck = p.ck + head_row0 * kRB;
+    const uint8_t* cv = p.cv + head_row0 * kRB;
     const float* ks = p.ks + head_row0;
     const float* vs = p.vs + head_row0;
     const int* pt = p.row_pt != nullptr ? p.row_pt[r0] : p.pt;
 
-    // pool row of the lane's position of a tile; positions that no row sees read pool row 0 and are masked
+    // pool row of the lane's position of a tile, -1 where no row of the group sees it
     auto table_row = [&](int tile) -> int {
       const int pos = tile * kTile + lane;
-      if (pos < span_lo || pos > span_hi) return 0;
+      if (pos < span_lo || pos > span_hi) return -1;
       const int row = pt != nullptr ? __ldg(pt + pos) : pos;
       return min(max(row, 0), static_cast<int>(p.stride) - 1);
     };
-    auto load = [&](Tile<D>& b, int row) {
+    auto fetch = [&](int stage, int row) {
+      constexpr int kPieces = kRB / 16, kRowsAtOnce = 32 / kPieces;
+      const uint32_t at = ring_at + stage * kStageBytes<D>;
+      const int piece = lane % kPieces, r_in = lane / kPieces;
+      // rows 2, 3, 6, 7 of a block (rows of kRowsAtOnce are whole blocks)
+      const int v_piece = D == 128 ? piece ^ (((r_in >> 1) & 1) << 1) : piece;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* src = ck + static_cast<size_t>(__shfl_sync(0xffffffffu, row, g + 8 * i)) * (D / 2);
-        if (D == 128) {
-          const uint4 w = __ldg(reinterpret_cast<const uint4*>(src));
-          b.k[i][0] = w.x, b.k[i][1] = w.y, b.k[i][kW - 2] = w.z, b.k[i][kW - 1] = w.w;
-        } else {
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
-          b.k[i][0] = w.x, b.k[i][1] = w.y;
-        }
+      for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
+        const int r = i * kRowsAtOnce + r_in;
+        const int pr = __shfl_sync(0xffffffffu, row, r);
+        const size_t off = static_cast<size_t>(max(pr, 0)) * kRB + piece * 16;
+        copy16_async(at + r * kRB + piece * 16, ck + off, pr >= 0);
+        copy16_async(at + kVAt + r * kRB + v_piece * 16, cv + off, pr >= 0);
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int at = 2 * t + (i & 1) + 8 * (i >> 1);
-        const uint8_t* src = cv + static_cast<size_t>(__shfl_sync(0xffffffffu, row, at)) * (D / 2);
-        if (D == 128) {
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
-          b.v[i][0] = w.x, b.v[i][D / 64 - 1] = w.y;
-        } else {
-          b.v[i][0] = __ldg(reinterpret_cast<const uint32_t*>(src));
-        }
-      }
-      b.sk = __ldg(ks + row), b.sv = __ldg(vs + row);
+      copy4_async(at + kSAt + lane * 4, ks + max(row, 0), row >= 0);
+      copy4_async(at + kSAt + kTile * 4 + lane * 4, vs + max(row, 0), row >= 0);
     };
     const int tile_end = first_tile + piece_end;
     int tile = first_tile + piece_begin + warp;
-    Tile<D> bufs[2];
-    int row_next = 0;
-    if (tile < tile_end) {
-      load(bufs[0], table_row(tile));
-      if (tile + kWarps < tile_end) row_next = table_row(tile + kWarps);
+    int row_next = -1;
+    {
+      const int row0 = tile < tile_end ? table_row(tile) : -1;
+      const int row1 = tile + kWarps < tile_end ? table_row(tile + kWarps) : -1;
+      if (tile + 2 * kWarps < tile_end) row_next = table_row(tile + 2 * kWarps);
+      if (tile < tile_end) fetch(0, row0);
+      copies_commit();
+      if (tile + kWarps < tile_end) fetch(1, row1);
+      copies_commit();
     }
 
     // q as the B operand, scaled by a power of two per column; the operand's elements follow the nibbles of K's
@@ -317,7 +339,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(co
     }
     float v_mult = 1.0f, v_cap = -1.0f;  // power of two on v_scale, and the largest v_scale it is good for
 
-    auto attend = [&](const Tile<D>& b, int t0) {
+    for (int stage = 0; tile < tile_end; tile += kWarps, stage = stage == kStages - 1 ? 0 : stage + 1) {
+      copies_wait<kStages - 2>();
+      __syncwarp();
+      if (tile + 2 * kWarps < tile_end) fetch(stage == 0 ? 2 : stage - 1, row_next);
+      copies_commit();
+      if (tile + 3 * kWarps < tile_end) row_next = table_row(tile + 3 * kWarps);
+      const unsigned char* const raw = ring + stage * kStageBytes<D>;
+      const float* const raw_ks = reinterpret_cast<const float*>(raw + kSAt);
+      const float* const raw_vs = raw_ks + kTile;
+      const int t0 = tile * kTile;
+
       // S^T = K Q^T for the tile's two halves
       float s[NT][2][4];
 #pragma unroll
@@ -325,10 +357,22 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(co
 #pragma unroll
         for (int h = 0; h < 2; ++h) s[nt][h][0] = s[nt][h][1] = s[nt][h][2] = s[nt][h][3] = 0.0f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        uint32_t k[2][kW];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const unsigned char* src = raw + (pg + 8 * i + 16 * h) * kRB + t * (D / 8);
+          if (D == 128) {
+            const uint4 w = *reinterpret_cast<const uint4*>(src);
+            k[i][0] = w.x, k[i][1] = w.y, k[i][kW - 2] = w.z, k[i][kW - 1] = w.w;
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(src);
+            k[i][0] = w.x, k[i][1] = w.y;
+          }
+        }
 #pragma unroll
         for (int w = 0; w < kW; ++w) {
-          const uint32_t a = b.k[2 * h][w], c = b.k[2 * h + 1][w], a8 = a >> 8, c8 = c >> 8;
+          const uint32_t a = k[0][w], c = k[1][w], a8 = a >> 8, c8 = c >> 8;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma16816(s[nt][h], a & 0x000f000fu, c & 0x000f000fu, a & 0x00f000f0u, c & 0x00f000f0u, qb[nt][2 * w][0],
@@ -337,11 +381,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(co
                      qb[nt][2 * w + 1][0], qb[nt][2 * w + 1][1]);
           }
         }
-      const bool unmasked = t0 >= all_lo && t0 + kTile - 1 <= all_hi && t0 >= span_lo && t0 + kTile - 1 <= span_hi;
-      const float sv_lane = (t0 + lane >= span_lo && t0 + lane <= span_hi) ? b.sv : 0.0f;
-      float fk[4], fv[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) fk[i] = __shfl_sync(0xffffffffu, b.sk, g + 8 * i);
+      }
+      const bool unmasked = t0 >= all_lo && t0 + kTile - 1 <= all_hi;
+      const float sv_lane = raw_vs[lane];
       if (__any_sync(0xffffffffu, sv_lane > v_cap)) {
         const float top = warp_max(sv_lane);
         float mult = 1.0f;
@@ -363,15 +405,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(co
           for (int i = 0; i < 4; ++i) osum[nt][i] *= f;
         }
       }
-      const float sv_mult = sv_lane * v_mult;
+      float fk[4], fv[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) fv[i] = __shfl_sync(0xffffffffu, sv_mult, g + 8 * i);
+      for (int i = 0; i < 4; ++i) fk[i] = raw_ks[pg + 8 * i], fv[i] = raw_vs[pg + 8 * i] * v_mult;
       uint32_t pb[NT][2][2];
       bool moved = false;
       float corr[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float pr[2][4];  // [column e][position g + 8 i]
+        float pr[2][4];  // [column e][position pg + 8 i]
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float l[4];
@@ -379,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(co
           for (int i = 0; i < 4; ++i) {
             l[i] = (s[nt][i >> 1][2 * (i & 1) + e] - l_off[nt][e]) * (fk[i] * l_scale[nt][e]);
             if (!unmasked) {
-              const int pos = t0 + g + 8 * i;
+              const int pos = t0 + pg + 8 * i;
               if (pos > pos_col[nt][e] || pos < lo_col[nt][e]) l[i] = -INFINITY;
             }
           }
@@ -416,13 +458,24 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(co
       // O^T += V^T P^T: the halves of two positions' words side by side are four dims of both
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        uint32_t v[4][D / 64];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = (i & 1 ? v_odd : v_even) + 8 * (i >> 1) + 16 * h;
+          if (D == 128) {
+            const uint2 w = *reinterpret_cast<const uint2*>(raw + kVAt + r * kRB + ((g * 8) ^ ((r & 2) << 4)));
+            v[i][0] = w.x, v[i][D / 64 - 1] = w.y;
+          } else {
+            v[i][0] = *reinterpret_cast<const uint32_t*>(raw + kVAt + r * kRB + g * 4);
+          }
+        }
 #pragma unroll
         for (int w = 0; w < D / 64; ++w)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const uint32_t sel = u ? 0x7632u : 0x5410u;
-            const uint32_t a = __byte_perm(b.v[4 * h][w], b.v[4 * h + 1][w], sel), a8 = a >> 8;
-            const uint32_t c = __byte_perm(b.v[4 * h + 2][w], b.v[4 * h + 3][w], sel), c8 = c >> 8;
+            const uint32_t a = __byte_perm(v[0][w], v[1][w], sel), a8 = a >> 8;
+            const uint32_t c = __byte_perm(v[2][w], v[3][w], sel), c8 = c >> 8;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               mma16816(o[nt][4 * w + 2 * u], a & 0x000f000fu, a & 0x00f000f0u, c & 0x000f000fu, c & 0x00f000f0u,
@@ -435,23 +488,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(co
         for (int nt = 0; nt < NT; ++nt)
           mma16816(osum[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[nt][h][0], pb[nt][h][1]);
       }
-    };
-
-    while (tile < tile_end) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (tile < tile_end) {  // the same for the whole warp
-          if (tile + kWarps < tile_end) {
-            load(bufs[i ^ 1], row_next);
-            if (tile + 2 * kWarps < tile_end) row_next = table_row(tile + 2 * kWarps);
-          }
-          attend(bufs[i], tile * kTile);
-          tile += kWarps;
-        }
-      }
     }
 
-    // the four warps' states meet in shared memory
+    // the four warps' states meet in shared memory, each parked in the warp's own ring
+    copies_wait<0>();
+    __syncwarp();
+    float* const park = reinterpret_cast<float*>(ring);  // [kC][D + kPad], then [kC][2] (max, sum)
     const float back = 16777216.0f / v_mult;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -462,11 +504,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(co
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int c = 8 * nt + 2 * t + e;
-        if (g == 0) s_ml[warp][c][0] = m_run[nt][e], s_ml[warp][c][1] = l;
+        if (g == 0) park[kC * (D + kPad) + 2 * c] = m_run[nt][e], park[kC * (D + kPad) + 2 * c + 1] = l;
         const float off = osum[nt][e] * (8.0f / 16777216.0f);
 #pragma unroll
         for (int m = 0; m < kM; ++m)
-          *reinterpret_cast<float2*>(&s_o[warp][c][g * (D / 8) + 2 * m]) =
+          *reinterpret_cast<float2*>(park + c * (D + kPad) + g * (D / 8) + 2 * m) =
               make_float2((o[nt][m][e] - off) * back, (o[nt][m][2 + e] * 0.0625f - off) * back);
       }
     }
@@ -475,12 +517,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(co
     const size_t slot = static_cast<size_t>(blockIdx.x) + static_cast<size_t>(grp) * per_group + sub;
     for (int i = threadIdx.x; i < columns * D; i += kThreads) {
       const int c = i / D, dim = i % D;
-      const float m = fmaxf(fmaxf(s_ml[0][c][0], s_ml[1][c][0]), fmaxf(s_ml[2][c][0], s_ml[3][c][0]));
-      float l = 0.0f, acc = 0.0f;
+      float mw[kWarps], m = -INFINITY, l = 0.0f, acc = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = s_ml[w][c][0] == -INFINITY ? 0.0f : exp2f(s_ml[w][c][0] - m);
-        l += f * s_ml[w][c][1], acc += f * s_o[w][c][dim];
+        mw[w] = reinterpret_cast<const float*>(s_ring + w * kWarpBytes<D>)[kC * (D + kPad) + 2 * c];
+        m = fmaxf(m, mw[w]);
+      }
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float* parked = reinterpret_cast<const float*>(s_ring + w * kWarpBytes<D>);
+        const float f = mw[w] == -INFINITY ? 0.0f : exp2f(mw[w] - m);
+        l += f * parked[kC * (D + kPad) + 2 * c + 1], acc += f * parked[c * (D + kPad) + dim];
       }
       if (whole) {
         const int row = r0 + (c0 + c) / p.G, hl = (c0 + c) % p.G;
@@ -496,36 +543,81 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attn_int4_kernel(co
   }
 }
 
-// Joins the pieces of segments that several CTAs worked on: a CTA per segment, in the CTAs' order.
+// Joins the pieces of segments that several CTAs worked on: a CTA per segment and column. The pieces' weights
+// exp2(m - max) are worked out side by side; then each warp adds every fourth piece, eight loads of a lane in flight,
+// and the four sums meet in shared memory. The order depends on the number of pieces alone.
 template <int D, int NT>
 __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4AttnParams p, int max_shares) {
   pdl_begin();
-  constexpr int kC = 8 * NT;
-  const int per_group = p.Hk * p.blocks, grp = blockIdx.x / per_group, sub = blockIdx.x % per_group;
+  constexpr int kC = 8 * NT, kPer = D / 32;
+  __shared__ float s_w[kMaxShares];
+  __shared__ float s_red[2][kWarps];
+  __shared__ float s_acc[kWarps][D];
+  const int per_group = p.Hk * p.blocks, grp = blockIdx.x / per_group, sub = blockIdx.x % per_group, c = blockIdx.y;
   const int hkv = sub / p.blocks, c0 = (sub % p.blocks) * kC, r0 = grp * p.per, nrows = min(p.per, p.rows - r0);
-  const int columns = min(kC, nrows * p.G - c0);
+  if (c >= min(kC, nrows * p.G - c0)) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int before = __ldcg(p.prefix + grp), n_tiles = __ldcg(p.prefix + grp + 1) - before;
   const long long all = static_cast<long long>(__ldcg(p.prefix + p.groups)) * per_group;
   const long long x0 = static_cast<long long>(before) * per_group + static_cast<long long>(sub) * n_tiles;
-  int i0 = 0, i1 = -1;  // the CTAs whose shares hold the segment's first and last tile
+  int i0 = 0, n = 0;  // the first of the CTAs whose shares hold the segment's tiles, and how many there are
   if (n_tiles > 0) {
     const long long shares = shares_of(all, max_shares);
-    i0 = static_cast<int>(((x0 + 1) * shares - 1) / all), i1 = static_cast<int>(((x0 + n_tiles) * shares - 1) / all);
-    if (i0 == i1) return;  // written by that CTA
+    i0 = static_cast<int>(((x0 + 1) * shares - 1) / all), n = static_cast<int>(((x0 + n_tiles) * shares - 1) / all) - i0 + 1;
+    if (n == 1) return;  // written by that CTA
   }
-  for (int i = threadIdx.x; i < columns * D; i += kThreads) {
-    const int c = i / D, dim = i % D;
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
-    for (int s = i0; s <= i1; ++s) {
-      const size_t at = (static_cast<size_t>(s) + blockIdx.x) * kC + c;
-      const float ms = __ldcg(p.part_ml + at * 2), ls = __ldcg(p.part_ml + at * 2 + 1);
-      if (ms == -INFINITY) continue;
-      const float mn = fmaxf(m, ms), f = m == -INFINITY ? 0.0f : exp2f(m - mn), fs = exp2f(ms - mn);
-      acc = acc * f + fs * __ldcg(p.part_o + at * D + dim), l = l * f + fs * ls, m = mn;
+  const size_t first = (static_cast<size_t>(i0) + blockIdx.x) * kC + c;  // (slot, column) of the first piece
+  float m = -INFINITY, l = 0.0f;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    s_w[i] = __ldcg(p.part_ml + (first + static_cast<size_t>(i) * kC) * 2);
+    m = fmaxf(m, s_w[i]);
+  }
+  m = warp_max(m);
+  if (lane == 0) s_red[0][warp] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const float f = s_w[i] == -INFINITY ? 0.0f : exp2f(s_w[i] - m);
+    s_w[i] = f;
+    l += f * __ldcg(p.part_ml + (first + static_cast<size_t>(i) * kC) * 2 + 1);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (lane == 0) s_red[1][warp] = l;
+  __syncthreads();
+  float acc[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
+  constexpr int kFly = 8;
+  for (int i = warp; i < n; i += kFly * kWarps) {
+    float v[kFly][kPer];
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      const int s = i + u * kWarps;
+      const float* src = p.part_o + (first + static_cast<size_t>(s) * kC) * D + lane * kPer;
+#pragma unroll
+      for (int e = 0; e < kPer; e += 2) {
+        const float2 w = s < n ? __ldcg(reinterpret_cast<const float2*>(src + e)) : make_float2(0.0f, 0.0f);
+        v[u][e] = w.x, v[u][e + 1] = w.y;
+      }
     }
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      const float f = i + u * kWarps < n ? s_w[i + u * kWarps] : 0.0f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] += f * v[u][e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) s_acc[warp][lane * kPer + e] = acc[e];
+  __syncthreads();
+  l = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+  const int dim = threadIdx.x;
+  if (dim < D) {
+    const float sum = (s_acc[0][dim] + s_acc[1][dim]) + (s_acc[2][dim] + s_acc[3][dim]);
     const int row = r0 + (c0 + c) / p.G, hl = (c0 + c) % p.G;
     p.out[(static_cast<size_t>(row) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + dim] =
-        static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? acc / l : 0.0f));
+        static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? sum / l : 0.0f));
   }
 }
 
@@ -542,7 +634,7 @@ Int4Plan plan_int4(int rows, int per, int Hq, int Hk, int d, int max_len) {
   s.blocks = (columns + 8 * s.nt - 1) / (8 * s.nt);
   s.groups = (rows + per - 1) / per;
   s.segments = static_cast<long long>(s.groups) * Hk * s.blocks;
-  const long long resident = static_cast<long long>(s.nt == 1 ? 3 : 2) * sm_count();
+  const long long resident = std::min(static_cast<long long>(s.nt == 1 ? 4 : 3) * sm_count(), static_cast<long long>(kMaxShares));
   const long long tiles = s.segments * ((max_len + kTile - 1) / kTile);
   // short caches: a segment is one tile per warp. Many segments: the CTAs balance one another, and each saves its
   // neighbours the joining of a piece.
@@ -563,9 +655,20 @@ int launch_int4(const char* fn, const Int4AttnParams& p, const Int4Plan& s) {
   const cudaStream_t st = current_stream();
   if (s.segments > INT_MAX) return fail(fn, "too many rows");
   const unsigned ctas = static_cast<unsigned>(p.split ? s.shares : s.segments);
-  G4_LAUNCH_PDL(fn, (attn_int4_kernel<D, NT>), dim3(ctas), dim3(kThreads), 0, st, p);
+  constexpr int smem = kWarps * kWarpBytes<D>;
+  if (smem > 48 * 1024) {
+    static std::atomic<bool> attr_set[64];  // per device; relaxed: setting the attribute twice is harmless
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) return fail(fn, "cannot identify the current device");
+    if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_relaxed)) {
+      G4_CUDA_TRY(fn, cudaFuncSetAttribute(attn_int4_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_relaxed);
+    }
+  }
+  G4_LAUNCH_PDL(fn, (attn_int4_kernel<D, NT>), dim3(ctas), dim3(kThreads), smem, st, p);
   if (p.split)
-    G4_LAUNCH_PDL(fn, (attn_int4_join_kernel<D, NT>), dim3(static_cast<unsigned>(s.segments)), dim3(kThreads), 0, st, p, s.shares);
+    G4_LAUNCH_PDL(fn, (attn_int4_join_kernel<D, NT>), dim3(static_cast<unsigned>(s.segments), static_cast<unsigned>(std::min(8 * NT, p.per * p.G))),
+                  dim3(kThreads), 0, st, p, s.shares);
   return 0;
 }
 
