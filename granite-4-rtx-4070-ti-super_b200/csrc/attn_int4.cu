@@ -7,18 +7,24 @@
 //
 // A position costs d + 8 bytes a kv head and 4 d multiply-adds a query head: memory bounds it as long as the
 // conversion of the codes stays cheap, so nothing is converted that need not be:
-//  * A nibble u = c + 8 masked out of a word IS an fp16 number: bits 0-3 of a half are the subnormal u 2^-24,
-//    bits 4-7 the value u 2^-20. One AND gives two mma operand elements. The 2^-24 (and the factor 16 of the odd
-//    dims: folded into q for the logits, taken out of the output rows for V) are powers of two, hence exact.
-//  * The 8 of u = c + 8 is one number per column: sum_d q_d (u_d - 8) = sum q u - 8 sum q, and
-//    sum_t p_t (u_t - 8) = sum p u - 8 sum p, with sum p from one more mma against ones.
+//  * A nibble u = c + 8 masked out of a word IS a number of the mma's operand type. K: in the low half of a byte it is the
+//    e4m3 value u 2^-9 (0 - 7 are subnormal, 8 - 15 carry on with the same step); two ANDs and a shift give the eight
+//    operand elements of a word. V: in bits 0-3 of a half it is the fp16 subnormal u 2^-24, in bits 4-7 u 2^-20.
+//    Powers of two come out of the logits' scale and of the output rows, exactly.
+//  * The 8 of u = c + 8 is one number per column: sum_d q_d (u_d - 8) = sum q u - 8 sum q, which starts the logits'
+//    accumulator, and sum_t p_t (u_t - 8) = sum p u - 8 sum p, with sum p from one more mma against ones.
 //  * The row scales multiply a logit (K) and a probability (V), never an element.
-//  * Both contractions have the cache positions on the 16-row side (S^T = K Q^T) or the 16-deep side (O^T = V^T P^T)
-//    of mma.sync m16n8k16 and the (query row, head) pairs on the 8-column side. Which dims a lane's fragment
-//    elements stand for is free as long as q's match, so a lane's K elements are 16 consecutive bytes of a row and
-//    its V elements 8: both are loaded straight into the registers the masks are applied to.
-// P is rounded to fp16 (11 bits; everything else is f32) after the multiplication with v_scale and a power of two
-// that puts the largest v_scale seen at 2^12, so values of any magnitude keep the format's precision.
+//  * Both contractions have the cache positions on the 16-row side (S^T = K Q^T, m16n8k32 e4m3) or the 16-deep side
+//    (O^T = V^T P^T, m16n8k16 fp16) and the (query row, head) pairs on the 8-column side. Which dims a lane's fragment
+//    elements stand for is free as long as q's match, so a lane's K elements are 16 consecutive bytes of a row, and
+//    V's come out of ldmatrix.trans on 16-bit units: four dims of two positions in a register, ready for the masks.
+//  * q (bf16, 8 significant bits) is two e4m3 columns, hi = e4m3(q) and lo = q - hi (4 bits each, exact): the pair's logit
+//    is the sum of two accumulator elements of one lane. Scaled by a power of two that puts the head's largest |q| into
+//    [128, 256), values below 2^-9 of it lose what is under 2^-10, 2^-17 of the largest.
+// Products are exact in the f32 accumulators. P is rounded to fp16 (11 bits; everything else is f32) after the
+// multiplication with v_scale and a power of two that puts the largest v_scale seen at 2^8, so that values of any
+// magnitude keep the format's precision. The running maximum moves only when it is passed by 4 (in powers of two):
+// P is at most 16, v_scale 2^11, fp16 ends at 2^16, and most tiles leave the accumulators as they are.
 //
 // Work split: the (group, kv head, column block) segments' tiles of 32 positions form one line, cut into equal
 // shares, one CTA each, whatever the sequences' lengths (read on the device). A CTA's four warps take every fourth
@@ -77,6 +83,30 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void load_8x8_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+// Two floats as e4m3 in the low 16 bits, and back.
+__device__ __forceinline__ uint32_t to_e4m3(float a, float b) {
+  uint16_t h;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(b), "f"(a));
+  return h;
+}
+__device__ __forceinline__ float2 from_e4m3(uint32_t h) {
+  uint32_t w;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(w) : "h"(static_cast<uint16_t>(h)));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
@@ -153,9 +183,11 @@ __device__ __forceinline__ void copies_wait() {
 }
 
 // A warp's ring of raw tiles: 32 K rows, 32 V rows, their scales, as they are in the pool (what no row sees: zeros).
-// Row r of a block of eight, as the mma operands count them, is position r (r < 4) or r ^ 1 of the block: with that
-// order, and the 16-byte pieces of V rows 2, 3, 6 and 7 of a block exchanged in pairs, the lanes' reads of either
-// operand meet no bank twice.
+// The 16-byte pieces of a V row lie exchanged, so that the eight rows of an ldmatrix piece meet no bank twice.
+template <int D>
+__device__ __forceinline__ int v_piece(int row, int piece) {
+  return D == 128 ? piece ^ ((row >> 1) & 3) : piece ^ ((row >> 2) & 1);
+}
 constexpr int kStages = 3;
 template <int D>
 constexpr int kRowBytes = D / 2;
@@ -165,13 +197,17 @@ template <int D>
 constexpr int kWarpBytes = kStages * kStageBytes<D>;
 constexpr int kPad = 4;  // floats after a parked row of O
 
-// NT column tiles of 8: column 8 nt + i of column block cb is (query row c / G, query head c % G), c = 8 NT cb + 8 nt + i.
-template <int D, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) attn_int4_kernel(const Int4AttnParams p) {
+// NS logit tiles of four columns each: column 4 i + t of column block cb is pair c = 4 NS cb + 4 i + t, query row c / G,
+// query head c % G. P and O have a tile of eight columns for two of them: column 2 t + e of tile n is pair 4 (2 n + e) + t
+// (NS = 1: odd columns are zero).
+constexpr int ctas_per_sm(int ns) { return ns == 4 ? 3 : 4; }
+template <int D, int NS>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(const Int4AttnParams p) {
   // a launch that splits the line is one resident wave: what comes next may be staged beside it
   if (p.split) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   pdl_begin();
-  constexpr int kC = 8 * NT, kW = D / 32 /* K words of a row per lane */, kM = D / 16 /* 16-dim tiles of O^T */;
+  constexpr int kC = 4 * NS, kNP = (NS + 1) / 2, kE = NS == 1 ? 1 : 2;
+  constexpr int kW = D / 32 /* K words of a row per lane */, kM = D / 16 /* 16-dim tiles of O^T */;
   constexpr int kRB = kRowBytes<D>, kVAt = kTile * kRB, kSAt = 2 * kTile * kRB;
   static_assert(kWarpBytes<D> >= kC * (D + kPad) * 4 + kC * 8, "a warp parks its state in its ring");
   __shared__ int s_prefix[kMaxGroups + 1];
@@ -179,8 +215,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) attn_int4_kernel(co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   unsigned char* const ring = s_ring + warp * kWarpBytes<D>;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-  const int pg = g < 4 ? g : g ^ 1;                                // position of row g
-  const int v_even = 2 * t + (t >> 1), v_odd = 2 * t + 1 - (t >> 1);  // positions of rows 2t, 2t + 1
   const int per_group = p.Hk * p.blocks;
   long long x = 0, x_end = 0;  // this CTA's share of the line of tiles
   int grp = 0, sub = 0;
@@ -240,15 +274,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) attn_int4_kernel(co
       constexpr int kPieces = kRB / 16, kRowsAtOnce = 32 / kPieces;
       const uint32_t at = ring_at + stage * kStageBytes<D>;
       const int piece = lane % kPieces, r_in = lane / kPieces;
-      // rows 2, 3, 6, 7 of a block (rows of kRowsAtOnce are whole blocks)
-      const int v_piece = D == 128 ? piece ^ (((r_in >> 1) & 1) << 1) : piece;
+      const int piece_v = v_piece<D>(r_in, piece);  // (kRowsAtOnce rows are whole blocks of eight)
 #pragma unroll
       for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
         const int r = i * kRowsAtOnce + r_in;
         const int pr = __shfl_sync(0xffffffffu, row, r);
         const size_t off = static_cast<size_t>(max(pr, 0)) * kRB + piece * 16;
         copy16_async(at + r * kRB + piece * 16, ck + off, pr >= 0);
-        copy16_async(at + kVAt + r * kRB + v_piece * 16, cv + off, pr >= 0);
+        copy16_async(at + kVAt + r * kRB + piece_v * 16, cv + off, pr >= 0);
       }
       copy4_async(at + kSAt + lane * 4, ks + max(row, 0), row >= 0);
       copy4_async(at + kSAt + kTile * 4 + lane * 4, vs + max(row, 0), row >= 0);
@@ -266,17 +299,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) attn_int4_kernel(co
       copies_commit();
     }
 
-    // q as the B operand, scaled by a power of two per column; the operand's elements follow the nibbles of K's
-    // words: dims 8w + {0, 4} | {1, 5} and {2, 6} | {3, 7} of the lane's quarter, the odd ones over 16
-    uint32_t qb[NT][2 * kW][2];
-    float l_scale[NT][2], l_off[NT][2];  // of the accumulator's columns 8 nt + 2 t + e
-    int pos_col[NT][2], lo_col[NT][2];
+    // q as the B operand: the lane's column g of tile i is pair 4 i + g / 2, hi (g even) or lo; its elements follow the
+    // nibbles of K's words, dims 8 w + {0, 2, 4, 6} and {1, 3, 5, 7} of the lane's quarter
+    uint32_t qb[NS][kW][2];
+    float l_scale[NS], l_off[NS];  // of the lane's accumulator pairs 4 i + t
+    int pos_col[NS], lo_col[NS];
     int all_lo = 0, all_hi = INT_MAX;  // positions that every column sees
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int c = c0 + 8 * nt + g;
-      const bool live = 8 * nt + g < columns;
-      const int j = live ? c / p.G : 0, hl = live ? c % p.G : 0;
+    for (int i = 0; i < NS; ++i) {
+      const int cq = 4 * i + (g >> 1);
+      const bool live = cq < columns;
+      const int j = live ? (c0 + cq) / p.G : 0, hl = live ? (c0 + cq) % p.G : 0;
       const uint16_t* qrow = p.q + (static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + t * (D / 4);
       float f[kW][8];
       float top = 0.0f;
@@ -289,39 +322,36 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) attn_int4_kernel(co
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       int ex = 0;
-      if (top > 0.0f && top < INFINITY) ex = min(max(((__float_as_int(top) >> 23) & 0xff) - 127 - 12, -100), 100);
-      const float down = __int_as_float((127 - ex) << 23), down16 = down * 0.0625f;
+      if (top > 0.0f && top < INFINITY) ex = min(max(((__float_as_int(top) >> 23) & 0xff) - 127 - 7, -100), 100);
+      const float down = __int_as_float((127 - ex) << 23);
       float sum = 0.0f;
 #pragma unroll
       for (int w = 0; w < kW; ++w) {
-        qb[nt][2 * w][0] = halves(f[w][0] * down, f[w][4] * down);
-        qb[nt][2 * w][1] = halves(f[w][1] * down16, f[w][5] * down16);
-        qb[nt][2 * w + 1][0] = halves(f[w][2] * down, f[w][6] * down);
-        qb[nt][2 * w + 1][1] = halves(f[w][3] * down16, f[w][7] * down16);
+        uint32_t part[4];  // dims {0, 2}, {4, 6}, {1, 3}, {5, 7}
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&qb[nt][2 * w + i][0]));
-          const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&qb[nt][2 * w + i][1]));
-          sum += (a.x + a.y) + 16.0f * (b.x + b.y);
+        for (int u = 0; u < 4; ++u) {
+          const float a = f[w][4 * (u & 1) + (u >> 1)] * down, b = f[w][4 * (u & 1) + (u >> 1) + 2] * down;
+          part[u] = to_e4m3(a, b);
+          float2 back = from_e4m3(part[u]);
+          if (g & 1) part[u] = to_e4m3(a - back.x, b - back.y), back = from_e4m3(part[u]);
+          sum += back.x + back.y;
         }
+        qb[i][w][0] = part[0] | part[1] << 16, qb[i][w][1] = part[2] | part[3] << 16;
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const float up = p.scale_log2 * __int_as_float((127 + ex) << 23) * 16777216.0f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int cc = 8 * nt + 2 * t + e;
-        l_scale[nt][e] = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4);
-        l_off[nt][e] = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4) * (8.0f / 16777216.0f);
-        pos_col[nt][e] = INT_MAX, lo_col[nt][e] = 0;  // a column that is not there sees everything and is dropped
-        if (cc < columns) {
-          const int row = r0 + (c0 + cc) / p.G;
-          const int raw = p.row_pos != nullptr ? __ldg(p.row_pos + row) : p.base_pos + row;
-          const int pos = raw < 0 ? -1 : min(raw, p.max_len - 1);
-          pos_col[nt][e] = pos, lo_col[nt][e] = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
-        }
-        all_hi = min(all_hi, pos_col[nt][e]), all_lo = max(all_lo, lo_col[nt][e]);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);  // hi + lo
+      l_scale[i] = __shfl_sync(0xffffffffu, p.scale_log2 * __int_as_float((127 + ex) << 23) * 512.0f, 8 * t);
+      l_off[i] = __shfl_sync(0xffffffffu, sum, 8 * t) * (8.0f / 512.0f);
+      const int cc = 4 * i + t;
+      pos_col[i] = INT_MAX, lo_col[i] = 0;  // a column that is not there sees everything and is dropped
+      if (cc < columns) {
+        const int row = r0 + (c0 + cc) / p.G;
+        const int raw = p.row_pos != nullptr ? __ldg(p.row_pos + row) : p.base_pos + row;
+        const int pos = raw < 0 ? -1 : min(raw, p.max_len - 1);
+        pos_col[i] = pos, lo_col[i] = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
       }
+      all_hi = min(all_hi, pos_col[i]), all_lo = max(all_lo, lo_col[i]);
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
@@ -329,14 +359,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) attn_int4_kernel(co
       all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, o));
     }
 
-    float o[NT][kM][4], osum[NT][4], m_run[NT][2], l_run[NT][2];
+    float o[kNP][kM][4], osum[kNP][4], m_run[NS], l_run[NS];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int n = 0; n < kNP; ++n) {
 #pragma unroll
-      for (int b = 0; b < kM; ++b) o[nt][b][0] = o[nt][b][1] = o[nt][b][2] = o[nt][b][3] = 0.0f;
-      osum[nt][0] = osum[nt][1] = osum[nt][2] = osum[nt][3] = 0.0f;
-      m_run[nt][0] = m_run[nt][1] = -INFINITY, l_run[nt][0] = l_run[nt][1] = 0.0f;
+      for (int b = 0; b < kM; ++b) o[n][b][0] = o[n][b][1] = o[n][b][2] = o[n][b][3] = 0.0f;
+      osum[n][0] = osum[n][1] = osum[n][2] = osum[n][3] = 0.0f;
     }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) m_run[i] = -INFINITY, l_run[i] = 0.0f;
     float v_mult = 1.0f, v_cap = -1.0f;  // power of two on v_scale, and the largest v_scale it is good for
 
     for (int stage = 0; tile < tile_end; tile += kWarps, stage = stage == kStages - 1 ? 0 : stage + 1) {
@@ -350,18 +381,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) attn_int4_kernel(co
       const float* const raw_vs = raw_ks + kTile;
       const int t0 = tile * kTile;
 
-      // S^T = K Q^T for the tile's two halves
-      float s[NT][2][4];
+      // S^T = K Q^T for the tile's two halves, less 8 sum q
+      float s[NS][2][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) s[nt][h][0] = s[nt][h][1] = s[nt][h][2] = s[nt][h][3] = 0.0f;
+        for (int h = 0; h < 2; ++h) s[i][h][0] = s[i][h][2] = -l_off[i], s[i][h][1] = s[i][h][3] = 0.0f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t k[2][kW];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const unsigned char* src = raw + (pg + 8 * i + 16 * h) * kRB + t * (D / 8);
+          const unsigned char* src = raw + (g + 8 * i + 16 * h) * kRB + t * (D / 8);
           if (D == 128) {
             const uint4 w = *reinterpret_cast<const uint4*>(src);
             k[i][0] = w.x, k[i][1] = w.y, k[i][kW - 2] = w.z, k[i][kW - 1] = w.w;
@@ -372,121 +403,119 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) attn_int4_kernel(co
         }
 #pragma unroll
         for (int w = 0; w < kW; ++w) {
-          const uint32_t a = k[0][w], c = k[1][w], a8 = a >> 8, c8 = c >> 8;
+          const uint32_t a0 = k[0][w] & 0x0f0f0f0fu, a1 = k[1][w] & 0x0f0f0f0fu;
+          const uint32_t a2 = (k[0][w] >> 4) & 0x0f0f0f0fu, a3 = (k[1][w] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816(s[nt][h], a & 0x000f000fu, c & 0x000f000fu, a & 0x00f000f0u, c & 0x00f000f0u, qb[nt][2 * w][0],
-                     qb[nt][2 * w][1]);
-            mma16816(s[nt][h], a8 & 0x000f000fu, c8 & 0x000f000fu, a8 & 0x00f000f0u, c8 & 0x00f000f0u,
-                     qb[nt][2 * w + 1][0], qb[nt][2 * w + 1][1]);
-          }
+          for (int i = 0; i < NS; ++i) mma16832(s[i][h], a0, a1, a2, a3, qb[i][w][0], qb[i][w][1]);
         }
       }
       const bool unmasked = t0 >= all_lo && t0 + kTile - 1 <= all_hi;
-      const float sv_lane = raw_vs[lane];
-      if (__any_sync(0xffffffffu, sv_lane > v_cap)) {
-        const float top = warp_max(sv_lane);
+      float fk[4], fv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fk[i] = raw_ks[g + 8 * i], fv[i] = raw_vs[g + 8 * i];
+      if (__any_sync(0xffffffffu, fmaxf(fmaxf(fv[0], fv[1]), fmaxf(fv[2], fv[3])) > v_cap)) {
+        const float top = warp_max(fmaxf(fmaxf(fv[0], fv[1]), fmaxf(fv[2], fv[3])));
         float mult = 1.0f;
         v_cap = 0.0f;
         if (top > 0.0f && top < INFINITY) {
           const int ex = min(max(((__float_as_int(top) >> 23) & 0xff) - 127, -100), 100);
-          mult = __int_as_float((127 + 12 - ex) << 23);
-          v_cap = __int_as_float((127 + 3 + ex) << 23);  // 2^15 once multiplied
+          mult = __int_as_float((127 + 8 - ex) << 23);
+          v_cap = __int_as_float((127 + 3 + ex) << 23);  // 2^11 once multiplied
         }
         const float f = mult / v_mult;
         v_mult = mult;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int n = 0; n < kNP; ++n) {
 #pragma unroll
           for (int m = 0; m < kM; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[nt][m][i] *= f;
+            for (int i = 0; i < 4; ++i) o[n][m][i] *= f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) osum[nt][i] *= f;
+          for (int i = 0; i < 4; ++i) osum[n][i] *= f;
         }
       }
-      float fk[4], fv[4];
+      float l[NS][4];  // logits in powers of two of pair 4 i + t at positions g + 8 u
+      float passed = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) fk[i] = raw_ks[pg + 8 * i], fv[i] = raw_vs[pg + 8 * i] * v_mult;
-      uint32_t pb[NT][2][2];
-      bool moved = false;
-      float corr[NT][2];
+      for (int i = 0; i < NS; ++i) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float pr[2][4];  // [column e][position pg + 8 i]
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float l[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            l[i] = (s[nt][i >> 1][2 * (i & 1) + e] - l_off[nt][e]) * (fk[i] * l_scale[nt][e]);
-            if (!unmasked) {
-              const int pos = t0 + pg + 8 * i;
-              if (pos > pos_col[nt][e] || pos < lo_col[nt][e]) l[i] = -INFINITY;
-            }
+        for (int u = 0; u < 4; ++u) {
+          l[i][u] = (s[i][u >> 1][2 * (u & 1)] + s[i][u >> 1][2 * (u & 1) + 1]) * (fk[u] * l_scale[i]);
+          if (!unmasked) {
+            const int pos = t0 + g + 8 * u;
+            if (pos > pos_col[i] || pos < lo_col[i]) l[i][u] = -INFINITY;
           }
-          float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
+        }
+        // (-inf against a maximum of -inf is no move; nor is anything against NaN)
+        const float top = fmaxf(fmaxf(l[i][0], l[i][1]), fmaxf(l[i][2], l[i][3]));
+        passed = fmaxf(passed, top > m_run[i] ? top - m_run[i] : -INFINITY);
+      }
+      if (__any_sync(0xffffffffu, passed > 4.0f)) {
+        float corr[2 * kNP];
+        corr[2 * kNP - 1] = 1.0f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          float top = fmaxf(fmaxf(l[i][0], l[i][1]), fmaxf(l[i][2], l[i][3]));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const float m_new = fmaxf(m_run[nt][e], top), base = m_new == -INFINITY ? 0.0f : m_new;
-          corr[nt][e] = exp2_fast(m_run[nt][e] - base);
-          moved |= m_new != m_run[nt][e];
-          m_run[nt][e] = m_new;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) pr[e][i] = exp2_fast(l[i] - base);
-          l_run[nt][e] = l_run[nt][e] * corr[nt][e] + ((pr[e][0] + pr[e][1]) + (pr[e][2] + pr[e][3]));
+          const float m_new = fmaxf(m_run[i], top);
+          corr[i] = m_new == -INFINITY ? 1.0f : exp2_fast(m_run[i] - m_new);
+          l_run[i] *= corr[i], m_run[i] = m_new;
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            pb[nt][h][u] = transpose8x8(halves(pr[0][2 * h + u] * fv[2 * h + u], pr[1][2 * h + u] * fv[2 * h + u]));
-      }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int n = 0; n < kNP; ++n) {
 #pragma unroll
           for (int m = 0; m < kM; ++m) {
-            o[nt][m][0] *= corr[nt][0], o[nt][m][1] *= corr[nt][1];
-            o[nt][m][2] *= corr[nt][0], o[nt][m][3] *= corr[nt][1];
+            o[n][m][0] *= corr[2 * n], o[n][m][2] *= corr[2 * n];
+            if (kE == 2) o[n][m][1] *= corr[2 * n + 1], o[n][m][3] *= corr[2 * n + 1];
           }
-          osum[nt][0] *= corr[nt][0], osum[nt][1] *= corr[nt][1];
-          osum[nt][2] *= corr[nt][0], osum[nt][3] *= corr[nt][1];
+          osum[n][0] *= corr[2 * n];
+          if (kE == 2) osum[n][1] *= corr[2 * n + 1];
         }
       }
-      // O^T += V^T P^T: the halves of two positions' words side by side are four dims of both
+#pragma unroll
+      for (int u = 0; u < 4; ++u) fv[u] *= v_mult;
+      uint32_t pb[kNP][2][2];
+#pragma unroll
+      for (int n = 0; n < kNP; ++n) {
+        float pv[2][4];
+#pragma unroll
+        for (int e = 0; e < kE; ++e) {
+          const int i = 2 * n + e;
+          const float base = m_run[i] == -INFINITY ? 0.0f : m_run[i];
+          float pr[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) pr[u] = exp2_fast(l[i][u] - base), pv[e][u] = pr[u] * fv[u];
+          l_run[i] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) pb[n][u >> 1][u & 1] = transpose8x8(halves(pv[0][u], kE == 2 ? pv[1][u] : 0.0f));
+      }
+      // O^T += V^T P^T
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t v[4][D / 64];
+        const int r = 16 * h + (lane & 15);
+        const uint32_t at = ring_at + stage * kStageBytes<D> + kVAt + r * kRB;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = (i & 1 ? v_odd : v_even) + 8 * (i >> 1) + 16 * h;
-          if (D == 128) {
-            const uint2 w = *reinterpret_cast<const uint2*>(raw + kVAt + r * kRB + ((g * 8) ^ ((r & 2) << 4)));
-            v[i][0] = w.x, v[i][D / 64 - 1] = w.y;
-          } else {
-            v[i][0] = *reinterpret_cast<const uint32_t*>(raw + kVAt + r * kRB + g * 4);
+        for (int c = 0; c < D / 32; c += 2) {
+          uint32_t v[4];  // positions 0-7 and 8-15 of the half, dims 32 c ..; the same, dims 32 (c + 1) ..
+          load_8x8_trans(v, at + v_piece<D>(r, c + (lane >> 4)) * 16);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t a = v[2 * u], b = v[2 * u + 1], a8 = a >> 8, b8 = b >> 8;
+#pragma unroll
+            for (int n = 0; n < kNP; ++n) {
+              mma16816(o[n][2 * (c + u)], a & 0x000f000fu, a & 0x00f000f0u, b & 0x000f000fu, b & 0x00f000f0u, pb[n][h][0],
+                       pb[n][h][1]);
+              mma16816(o[n][2 * (c + u) + 1], a8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x000f000fu, b8 & 0x00f000f0u,
+                       pb[n][h][0], pb[n][h][1]);
+            }
           }
         }
 #pragma unroll
-        for (int w = 0; w < D / 64; ++w)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t sel = u ? 0x7632u : 0x5410u;
-            const uint32_t a = __byte_perm(v[0][w], v[1][w], sel), a8 = a >> 8;
-            const uint32_t c = __byte_perm(v[2][w], v[3][w], sel), c8 = c >> 8;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816(o[nt][4 * w + 2 * u], a & 0x000f000fu, a & 0x00f000f0u, c & 0x000f000fu, c & 0x00f000f0u,
-                       pb[nt][h][0], pb[nt][h][1]);
-              mma16816(o[nt][4 * w + 2 * u + 1], a8 & 0x000f000fu, a8 & 0x00f000f0u, c8 & 0x000f000fu, c8 & 0x00f000f0u,
-                       pb[nt][h][0], pb[nt][h][1]);
-            }
-          }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          mma16816(osum[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[nt][h][0], pb[nt][h][1]);
+        for (int n = 0; n < kNP; ++n)
+          mma16816(osum[n], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[n][h][0], pb[n][h][1]);
       }
     }
 
@@ -496,21 +525,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) attn_int4_kernel(co
     float* const park = reinterpret_cast<float*>(ring);  // [kC][D + kPad], then [kC][2] (max, sum)
     const float back = 16777216.0f / v_mult;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int i = 0; i < NS; ++i) {
+      const int n = i >> 1, e = i & 1, c = 4 * i + t;
+      float l = l_run[i];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      if (g == 0) park[kC * (D + kPad) + 2 * c] = m_run[i], park[kC * (D + kPad) + 2 * c + 1] = l;
+      const float off = osum[n][e] * (8.0f / 16777216.0f);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float l = l_run[nt][e];
-        l += __shfl_xor_sync(0xffffffffu, l, 4);
-        l += __shfl_xor_sync(0xffffffffu, l, 8);
-        l += __shfl_xor_sync(0xffffffffu, l, 16);
-        const int c = 8 * nt + 2 * t + e;
-        if (g == 0) park[kC * (D + kPad) + 2 * c] = m_run[nt][e], park[kC * (D + kPad) + 2 * c + 1] = l;
-        const float off = osum[nt][e] * (8.0f / 16777216.0f);
-#pragma unroll
-        for (int m = 0; m < kM; ++m)
-          *reinterpret_cast<float2*>(park + c * (D + kPad) + g * (D / 8) + 2 * m) =
-              make_float2((o[nt][m][e] - off) * back, (o[nt][m][2 + e] * 0.0625f - off) * back);
-      }
+      for (int m = 0; m < kM; ++m)  // rows g, g + 8: dims 32 (m / 2) + 4 g + 2 (m % 2), + 1
+        *reinterpret_cast<float2*>(park + c * (D + kPad) + 32 * (m >> 1) + 4 * g + 2 * (m & 1)) =
+            make_float2((o[n][m][e] - off) * back, (o[n][m][2 + e] * 0.0625f - off) * back);
     }
     __syncthreads();
     const bool whole = piece_begin == 0 && piece_end == n_tiles;
@@ -546,10 +572,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) attn_int4_kernel(co
 // Joins the pieces of segments that several CTAs worked on: a CTA per segment and column. The pieces' weights
 // exp2(m - max) are worked out side by side; then each warp adds every fourth piece, eight loads of a lane in flight,
 // and the four sums meet in shared memory. The order depends on the number of pieces alone.
-template <int D, int NT>
+template <int D, int NS>
 __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4AttnParams p, int max_shares) {
   pdl_begin();
-  constexpr int kC = 8 * NT, kPer = D / 32;
+  constexpr int kC = 4 * NS, kPer = D / 32;
   __shared__ float s_w[kMaxShares];
   __shared__ float s_red[2][kWarps];
   __shared__ float s_acc[kWarps][D];
@@ -623,25 +649,25 @@ __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4Attn
 
 // How a launch is cut: `shares` CTAs over the line of tiles, or a CTA per segment (shares 0).
 struct Int4Plan {
-  int nt, blocks, groups, shares;
+  int ns, blocks, groups, shares;
   long long segments, bytes;
 };
 
 Int4Plan plan_int4(int rows, int per, int Hq, int Hk, int d, int max_len) {
   Int4Plan s{};
   const int columns = per * (Hq / Hk);
-  s.nt = columns <= 8 ? 1 : 2;
-  s.blocks = (columns + 8 * s.nt - 1) / (8 * s.nt);
+  s.ns = columns <= 4 ? 1 : columns <= 8 ? 2 : 4;
+  s.blocks = (columns + 4 * s.ns - 1) / (4 * s.ns);
   s.groups = (rows + per - 1) / per;
   s.segments = static_cast<long long>(s.groups) * Hk * s.blocks;
-  const long long resident = std::min(static_cast<long long>(s.nt == 1 ? 4 : 3) * sm_count(), static_cast<long long>(kMaxShares));
+  const long long resident = std::min(static_cast<long long>(ctas_per_sm(s.ns)) * sm_count(), static_cast<long long>(kMaxShares));
   const long long tiles = s.segments * ((max_len + kTile - 1) / kTile);
   // short caches: a segment is one tile per warp. Many segments: the CTAs balance one another, and each saves its
   // neighbours the joining of a piece.
   if (max_len <= kTile * kWarps || s.groups > kMaxGroups || s.segments >= 4 * resident) return s;
   s.shares = static_cast<int>(std::min(resident, std::max(1ll, tiles / kWarps)));
   const long long slots = s.shares + s.segments;
-  s.bytes = slots * 8 * s.nt * (d + 2) * 4 + (s.groups + 1 + 3) / 4 * 16;
+  s.bytes = slots * 4 * s.ns * (d + 2) * 4 + (s.groups + 1 + 3) / 4 * 16;
   return s;
 }
 
@@ -650,7 +676,7 @@ bool int4_shape_ok(int Hq, int Hk, int d, int per) {
          static_cast<long long>(per) * (Hq / Hk) <= kMaxColumns;
 }
 
-template <int D, int NT>
+template <int D, int NS>
 int launch_int4(const char* fn, const Int4AttnParams& p, const Int4Plan& s) {
   const cudaStream_t st = current_stream();
   if (s.segments > INT_MAX) return fail(fn, "too many rows");
@@ -661,13 +687,13 @@ int launch_int4(const char* fn, const Int4AttnParams& p, const Int4Plan& s) {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) return fail(fn, "cannot identify the current device");
     if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_relaxed)) {
-      G4_CUDA_TRY(fn, cudaFuncSetAttribute(attn_int4_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      G4_CUDA_TRY(fn, cudaFuncSetAttribute(attn_int4_kernel<D, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
       if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_relaxed);
     }
   }
-  G4_LAUNCH_PDL(fn, (attn_int4_kernel<D, NT>), dim3(ctas), dim3(kThreads), smem, st, p);
+  G4_LAUNCH_PDL(fn, (attn_int4_kernel<D, NS>), dim3(ctas), dim3(kThreads), smem, st, p);
   if (p.split)
-    G4_LAUNCH_PDL(fn, (attn_int4_join_kernel<D, NT>), dim3(static_cast<unsigned>(s.segments), static_cast<unsigned>(std::min(8 * NT, p.per * p.G))),
+    G4_LAUNCH_PDL(fn, (attn_int4_join_kernel<D, NS>), dim3(static_cast<unsigned>(s.segments), static_cast<unsigned>(std::min(4 * NS, p.per * p.G))),
                   dim3(kThreads), 0, st, p, s.shares);
   return 0;
 }
@@ -686,11 +712,12 @@ int attn_int4(const char* fn, Int4AttnParams p, int d, void* scratch, long long 
   if (p.split) {
     p.part_o = static_cast<float*>(scratch);
     const long long slots = s.shares + s.segments;
-    p.part_ml = p.part_o + slots * 8 * s.nt * d;
-    p.prefix = reinterpret_cast<int*>(p.part_ml + slots * 8 * s.nt * 2);
+    p.part_ml = p.part_o + slots * 4 * s.ns * d;
+    p.prefix = reinterpret_cast<int*>(p.part_ml + slots * 4 * s.ns * 2);
   }
-  if (d == 128) return s.nt == 1 ? launch_int4<128, 1>(fn, p, s) : launch_int4<128, 2>(fn, p, s);
-  return s.nt == 1 ? launch_int4<64, 1>(fn, p, s) : launch_int4<64, 2>(fn, p, s);
+  if (d == 128)
+    return s.ns == 1 ? launch_int4<128, 1>(fn, p, s) : s.ns == 2 ? launch_int4<128, 2>(fn, p, s) : launch_int4<128, 4>(fn, p, s);
+  return s.ns == 1 ? launch_int4<64, 1>(fn, p, s) : s.ns == 2 ? launch_int4<64, 2>(fn, p, s) : launch_int4<64, 4>(fn, p, s);
 }
 
 // Chunks from this many rows on go through the tensor-core prefill kernels, which read an 8-bit pool.
