@@ -7,24 +7,25 @@
 //
 // A position costs d + 8 bytes a kv head and 4 d multiply-adds a query head: memory bounds it as long as the
 // conversion of the codes stays cheap, so nothing is converted that need not be:
-//  * A nibble u = c + 8 masked out of a word IS a number of the mma's operand type. K: in the low half of a byte it is the
-//    e4m3 value u 2^-9 (0 - 7 are subnormal, 8 - 15 carry on with the same step); two ANDs and a shift give the eight
-//    operand elements of a word. V: in bits 0-3 of a half it is the fp16 subnormal u 2^-24, in bits 4-7 u 2^-20.
-//    Powers of two come out of the logits' scale and of the output rows, exactly.
-//  * The 8 of u = c + 8 is one number per column: sum_d q_d (u_d - 8) = sum q u - 8 sum q, which starts the logits'
-//    accumulator, and sum_t p_t (u_t - 8) = sum p u - 8 sum p, with sum p from one more mma against ones.
+//  * A nibble u = c + 8 masked out of a word IS a number of the mma's operand type. K: in the low half of a byte it is a
+//    u8; two ANDs and a shift give the eight operand elements of a word. V: in bits 0-3 of a half it is the fp16
+//    subnormal u 2^-24, in bits 4-7 u 2^-20; the powers of two come out of the output rows, exactly.
+//  * The 8 of u = c + 8 is one number per column: sum_d q_d (u_d - 8) = sum q u - 8 sum q, and
+//    sum_t p_t (u_t - 8) = sum p u - 8 sum p, with sum p from one more mma against ones.
 //  * The row scales multiply a logit (K) and a probability (V), never an element.
-//  * Both contractions have the cache positions on the 16-row side (S^T = K Q^T, m16n8k32 e4m3) or the 16-deep side
+//  * Both contractions have the cache positions on the 16-row side (S^T = K Q^T, m16n8k32 u8 x s8) or the 16-deep side
 //    (O^T = V^T P^T, m16n8k16 fp16) and the (query row, head) pairs on the 8-column side. Which dims a lane's fragment
 //    elements stand for is free as long as q's match, so a lane's K elements are 16 consecutive bytes of a row, and
 //    V's come out of ldmatrix.trans on 16-bit units: four dims of two positions in a register, ready for the masks.
-//  * q (bf16, 8 significant bits) is two e4m3 columns, hi = e4m3(q) and lo = q - hi (4 bits each, exact): the pair's logit
-//    is the sum of two accumulator elements of one lane. Scaled by a power of two that puts the head's largest |q| into
-//    [128, 256), values below 2^-9 of it lose what is under 2^-10, 2^-17 of the largest.
-// Products are exact in the f32 accumulators. P is rounded to fp16 (11 bits; everything else is f32) after the
-// multiplication with v_scale and a power of two that puts the largest v_scale seen at 2^8, so that values of any
-// magnitude keep the format's precision. The running maximum moves only when it is passed by 4 (in powers of two):
-// P is at most 16, v_scale 2^11, fp16 ends at 2^16, and most tiles leave the accumulators as they are.
+//  * q is two s8 columns, the digits of a 16-bit integer round(q 32639 / max |q| of the head) = 256 hi + lo: the pair's
+//    logit is 256 times one accumulator element of a lane plus its neighbour, in exact integers. What q loses is 2^-16 of
+//    the head's largest value, a step finer than the fp16 that P is rounded to for logits up to 2^4.
+//    (The same in e4m3 takes twice the instructions: sm_100 widens e4m3 to fp16 before the product. fp16 itself takes
+//    five instructions instead of three per eight codes and twice the mma.)
+// P is rounded to fp16 (11 bits; everything else is f32) after the multiplication with v_scale and a power of two that
+// puts the largest v_scale seen at 2^8, so that values of any magnitude keep the format's precision. The running maximum
+// moves only when it is passed by 4 (in powers of two): P is at most 16, v_scale 2^11, fp16 ends at 2^16, and most tiles
+// leave the accumulators as they are.
 //
 // Work split: the (group, kv head, column block) segments' tiles of 32 positions form one line, cut into equal
 // shares, one CTA each, whatever the sequences' lengths (read on the device). A CTA's four warps take every fourth
@@ -84,11 +85,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+__device__ __forceinline__ void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void load_8x8_trans(uint32_t (&r)[4], uint32_t at) {
@@ -96,17 +97,6 @@ __device__ __forceinline__ void load_8x8_trans(uint32_t (&r)[4], uint32_t at) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(at)
                : "memory");
-}
-// Two floats as e4m3 in the low 16 bits, and back.
-__device__ __forceinline__ uint32_t to_e4m3(float a, float b) {
-  uint16_t h;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(b), "f"(a));
-  return h;
-}
-__device__ __forceinline__ float2 from_e4m3(uint32_t h) {
-  uint32_t w;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(w) : "h"(static_cast<uint16_t>(h)));
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
@@ -170,11 +160,11 @@ __device__ __forceinline__ long long shares_of(long long all, int shares) {
   return min(static_cast<long long>(shares), (all + kWarps - 1) / kWarps);
 }
 
-__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, bool have) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void copy4_async(uint32_t dst, const void* src, bool have) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have ? 4 : 0) : "memory");
+__device__ __forceinline__ void copy4_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -182,10 +172,11 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// A warp's ring of raw tiles: 32 K rows, 32 V rows, their scales, as they are in the pool (what no row sees: zeros).
-// The 16-byte pieces of a V row lie exchanged, so that the eight rows of an ldmatrix piece meet no bank twice.
+// A warp's ring of raw tiles: 32 K rows, 32 V rows, their scales, as they are in the pool (for positions that no
+// row sees, the nearest that one sees). The 16-byte pieces of a row lie exchanged, so that neither the copies (two lanes a row),
+// nor the eight rows of an ldmatrix piece, nor the lanes' reads of K meet a bank more often than their width asks for.
 template <int D>
-__device__ __forceinline__ int v_piece(int row, int piece) {
+__device__ __forceinline__ int piece_at(int row, int piece) {
   return D == 128 ? piece ^ ((row >> 1) & 3) : piece ^ ((row >> 2) & 1);
 }
 constexpr int kStages = 3;
@@ -211,6 +202,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
   constexpr int kRB = kRowBytes<D>, kVAt = kTile * kRB, kSAt = 2 * kTile * kRB;
   static_assert(kWarpBytes<D> >= kC * (D + kPad) * 4 + kC * 8, "a warp parks its state in its ring");
   __shared__ int s_prefix[kMaxGroups + 1];
+  __shared__ __align__(16) unsigned char s_q[8 * NS][D + 16];  // a row per column of the logit tiles
+  __shared__ float2 s_pair[4 * NS];                            // logit scale, 8 sum q (an integer)
   extern __shared__ __align__(128) unsigned char s_ring[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   unsigned char* const ring = s_ring + warp * kWarpBytes<D>;
@@ -263,35 +256,36 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     const float* vs = p.vs + head_row0;
     const int* pt = p.row_pt != nullptr ? p.row_pt[r0] : p.pt;
 
-    // pool row of the lane's position of a tile, -1 where no row of the group sees it
+    // pool row of the lane's position of a tile (past the end of what the group sees: the end's)
     auto table_row = [&](int tile) -> int {
-      const int pos = tile * kTile + lane;
-      if (pos < span_lo || pos > span_hi) return -1;
+      const int pos = min(max(tile * kTile + lane, span_lo), span_hi);
       const int row = pt != nullptr ? __ldg(pt + pos) : pos;
       return min(max(row, 0), static_cast<int>(p.stride) - 1);
     };
+    // A row takes 16 bytes of two lanes (32: a sector) at a time.
     auto fetch = [&](int stage, int row) {
-      constexpr int kPieces = kRB / 16, kRowsAtOnce = 32 / kPieces;
       const uint32_t at = ring_at + stage * kStageBytes<D>;
-      const int piece = lane % kPieces, r_in = lane / kPieces;
-      const int piece_v = v_piece<D>(r_in, piece);  // (kRowsAtOnce rows are whole blocks of eight)
 #pragma unroll
-      for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
-        const int r = i * kRowsAtOnce + r_in;
-        const int pr = __shfl_sync(0xffffffffu, row, r);
-        const size_t off = static_cast<size_t>(max(pr, 0)) * kRB + piece * 16;
-        copy16_async(at + r * kRB + piece * 16, ck + off, pr >= 0);
-        copy16_async(at + kVAt + r * kRB + piece_v * 16, cv + off, pr >= 0);
+      for (int i = 0; i < 2; ++i) {
+        const int r = 16 * i + (lane >> 1);
+        const size_t off = static_cast<size_t>(static_cast<unsigned>(__shfl_sync(0xffffffffu, row, r))) * kRB + (lane & 1) * 16;
+        const uint8_t *src_k = ck + off, *src_v = cv + off;
+#pragma unroll
+        for (int c = 0; c < kRB / 32; ++c) {
+          const uint32_t dst = at + r * kRB + piece_at<D>(r, 2 * c + (lane & 1)) * 16;
+          copy16_async(dst, src_k + 32 * c);
+          copy16_async(dst + kVAt, src_v + 32 * c);
+        }
       }
-      copy4_async(at + kSAt + lane * 4, ks + max(row, 0), row >= 0);
-      copy4_async(at + kSAt + kTile * 4 + lane * 4, vs + max(row, 0), row >= 0);
+      copy4_async(at + kSAt + lane * 4, ks + row);
+      copy4_async(at + kSAt + kTile * 4 + lane * 4, vs + row);
     };
     const int tile_end = first_tile + piece_end;
     int tile = first_tile + piece_begin + warp;
-    int row_next = -1;
+    int row_next = 0;
     {
-      const int row0 = tile < tile_end ? table_row(tile) : -1;
-      const int row1 = tile + kWarps < tile_end ? table_row(tile + kWarps) : -1;
+      const int row0 = tile < tile_end ? table_row(tile) : 0;
+      const int row1 = tile + kWarps < tile_end ? table_row(tile + kWarps) : 0;
       if (tile + 2 * kWarps < tile_end) row_next = table_row(tile + 2 * kWarps);
       if (tile < tile_end) fetch(0, row0);
       copies_commit();
@@ -299,54 +293,69 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       copies_commit();
     }
 
-    // q as the B operand: the lane's column g of tile i is pair 4 i + g / 2, hi (g even) or lo; its elements follow the
-    // nibbles of K's words, dims 8 w + {0, 2, 4, 6} and {1, 3, 5, 7} of the lane's quarter
-    uint32_t qb[NS][kW][2];
-    float l_scale[NS], l_off[NS];  // of the lane's accumulator pairs 4 i + t
-    int pos_col[NS], lo_col[NS];
+    // q's digits into shared memory: a warp per pair, D / 32 dims a lane. Bytes follow the nibbles of K's words: of
+    // eight dims first 0, 2, 4, 6, then 1, 3, 5, 7.
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int c = i * kWarps + warp;
+      constexpr int kPer = D / 32;
+      float f[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) f[e] = 0.0f;
+      if (c < columns) {
+        const int j = (c0 + c) / p.G, hl = (c0 + c) % p.G;
+        const uint16_t* qrow = p.q + (static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + lane * kPer;
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) {
+          const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(qrow + e));
+          f[e] = bf16_lo(w), f[e + 1] = bf16_hi(w);
+        }
+      }
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) top = fmaxf(top, fabsf(f[e]));
+      top = warp_max(top);
+      const bool sound = top > 0.0f && top < INFINITY;
+      const float to_int = sound ? 32639.0f / fmaxf(top, 1e-30f) : 0.0f;
+      int sum = 0;
+      uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};  // even dims, odd dims
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int v = __float2int_rn(f[e] * to_int), h = (v + 128) >> 8;
+        sum += v;
+        hi[e & 1] |= static_cast<uint32_t>(h & 0xff) << (8 * (e >> 1)), lo[e & 1] |= static_cast<uint32_t>((v - 256 * h) & 0xff) << (8 * (e >> 1));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      unsigned char* dst = s_q[2 * c] + (lane * kPer / 8) * 8 + lane * kPer % 8 / 2;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (kPer == 4) {
+          *reinterpret_cast<uint16_t*>(dst + 4 * u) = static_cast<uint16_t>(hi[u]);
+          *reinterpret_cast<uint16_t*>(dst + 4 * u + sizeof(s_q[0])) = static_cast<uint16_t>(lo[u]);
+        } else {
+          dst[4 * u] = static_cast<unsigned char>(hi[u]), dst[4 * u + sizeof(s_q[0])] = static_cast<unsigned char>(lo[u]);
+        }
+      }
+      if (lane == 0) s_pair[c] = make_float2(sound ? p.scale_log2 * fmaxf(top, 1e-30f) / 32639.0f : 0.0f, __int_as_float(8 * sum));
+    }
+    __syncthreads();
+    uint32_t qb[NS][kW][2];  // the lane's column g of tile i: pair 4 i + g / 2, hi (g even) or lo
+    float l_scale[NS];       // of the lane's accumulator pairs 4 i + t
+    int l_off[NS], pos_col[NS], lo_col[NS];
     int all_lo = 0, all_hi = INT_MAX;  // positions that every column sees
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      const int cq = 4 * i + (g >> 1);
-      const bool live = cq < columns;
-      const int j = live ? (c0 + cq) / p.G : 0, hl = live ? (c0 + cq) % p.G : 0;
-      const uint16_t* qrow = p.q + (static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + t * (D / 4);
-      float f[kW][8];
-      float top = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kW; ++w) {
-        unpack8(live ? __ldg(reinterpret_cast<const uint4*>(qrow) + w) : make_uint4(0u, 0u, 0u, 0u), f[w]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[w][e]));
+      for (int w = 0; w < kW; w += 2) {
+        const uint4 v = *reinterpret_cast<const uint4*>(s_q[8 * i + g] + t * (D / 4) + 8 * w);
+        qb[i][w][0] = v.x, qb[i][w][1] = v.y, qb[i][w + 1][0] = v.z, qb[i][w + 1][1] = v.w;
       }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      int ex = 0;
-      if (top > 0.0f && top < INFINITY) ex = min(max(((__float_as_int(top) >> 23) & 0xff) - 127 - 7, -100), 100);
-      const float down = __int_as_float((127 - ex) << 23);
-      float sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kW; ++w) {
-        uint32_t part[4];  // dims {0, 2}, {4, 6}, {1, 3}, {5, 7}
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const float a = f[w][4 * (u & 1) + (u >> 1)] * down, b = f[w][4 * (u & 1) + (u >> 1) + 2] * down;
-          part[u] = to_e4m3(a, b);
-          float2 back = from_e4m3(part[u]);
-          if (g & 1) part[u] = to_e4m3(a - back.x, b - back.y), back = from_e4m3(part[u]);
-          sum += back.x + back.y;
-        }
-        qb[i][w][0] = part[0] | part[1] << 16, qb[i][w][1] = part[2] | part[3] << 16;
-      }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 4);  // hi + lo
-      l_scale[i] = __shfl_sync(0xffffffffu, p.scale_log2 * __int_as_float((127 + ex) << 23) * 512.0f, 8 * t);
-      l_off[i] = __shfl_sync(0xffffffffu, sum, 8 * t) * (8.0f / 512.0f);
-      const int cc = 4 * i + t;
+      const int c = 4 * i + t;
+      l_scale[i] = s_pair[c].x, l_off[i] = __float_as_int(s_pair[c].y);
       pos_col[i] = INT_MAX, lo_col[i] = 0;  // a column that is not there sees everything and is dropped
-      if (cc < columns) {
-        const int row = r0 + (c0 + cc) / p.G;
+      if (c < columns) {
+        const int row = r0 + (c0 + c) / p.G;
         const int raw = p.row_pos != nullptr ? __ldg(p.row_pos + row) : p.base_pos + row;
         const int pos = raw < 0 ? -1 : min(raw, p.max_len - 1);
         pos_col[i] = pos, lo_col[i] = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
@@ -359,7 +368,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, o));
     }
 
-    float o[kNP][kM][4], osum[kNP][4], m_run[NS], l_run[NS];
+    float o[kNP][kM][4], osum[kNP][4], m_run[NS], l_run[NS];  // l_run times v_mult
+    float m_pass[NS], e_base[NS];  // m_run + 4; what is taken off a logit: m_run - log2(v_mult)
 #pragma unroll
     for (int n = 0; n < kNP; ++n) {
 #pragma unroll
@@ -367,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       osum[n][0] = osum[n][1] = osum[n][2] = osum[n][3] = 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < NS; ++i) m_run[i] = -INFINITY, l_run[i] = 0.0f;
+    for (int i = 0; i < NS; ++i) m_run[i] = m_pass[i] = -INFINITY, e_base[i] = l_run[i] = 0.0f;
     float v_mult = 1.0f, v_cap = -1.0f;  // power of two on v_scale, and the largest v_scale it is good for
 
     for (int stage = 0; tile < tile_end; tile += kWarps, stage = stage == kStages - 1 ? 0 : stage + 1) {
@@ -381,18 +391,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       const float* const raw_vs = raw_ks + kTile;
       const int t0 = tile * kTile;
 
-      // S^T = K Q^T for the tile's two halves, less 8 sum q
-      float s[NS][2][4];
+      // S^T = K Q^T for the tile's two halves
+      int s[NS][2][4];
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) s[i][h][0] = s[i][h][2] = -l_off[i], s[i][h][1] = s[i][h][3] = 0.0f;
+        for (int h = 0; h < 2; ++h) s[i][h][0] = s[i][h][1] = s[i][h][2] = s[i][h][3] = 0;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t k[2][kW];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const unsigned char* src = raw + (g + 8 * i + 16 * h) * kRB + t * (D / 8);
+          const int r = g + 8 * i + 16 * h;
+          const unsigned char* src = raw + r * kRB + (D == 128 ? piece_at<D>(r, t) * 16 : piece_at<D>(r, t >> 1) * 16 + (t & 1) * 8);
           if (D == 128) {
             const uint4 w = *reinterpret_cast<const uint4*>(src);
             k[i][0] = w.x, k[i][1] = w.y, k[i][kW - 2] = w.z, k[i][kW - 1] = w.w;
@@ -406,62 +417,62 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
           const uint32_t a0 = k[0][w] & 0x0f0f0f0fu, a1 = k[1][w] & 0x0f0f0f0fu;
           const uint32_t a2 = (k[0][w] >> 4) & 0x0f0f0f0fu, a3 = (k[1][w] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
-          for (int i = 0; i < NS; ++i) mma16832(s[i][h], a0, a1, a2, a3, qb[i][w][0], qb[i][w][1]);
+          for (int i = 0; i < NS; ++i) mma_u8s8(s[i][h], a0, a1, a2, a3, qb[i][w][0], qb[i][w][1]);
         }
       }
-      const bool unmasked = t0 >= all_lo && t0 + kTile - 1 <= all_hi;
       float fk[4], fv[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) fk[i] = raw_ks[g + 8 * i], fv[i] = raw_vs[g + 8 * i];
-      if (__any_sync(0xffffffffu, fmaxf(fmaxf(fv[0], fv[1]), fmaxf(fv[2], fv[3])) > v_cap)) {
-        const float top = warp_max(fmaxf(fmaxf(fv[0], fv[1]), fmaxf(fv[2], fv[3])));
-        float mult = 1.0f;
-        v_cap = 0.0f;
-        if (top > 0.0f && top < INFINITY) {
-          const int ex = min(max(((__float_as_int(top) >> 23) & 0xff) - 127, -100), 100);
-          mult = __int_as_float((127 + 8 - ex) << 23);
-          v_cap = __int_as_float((127 + 3 + ex) << 23);  // 2^11 once multiplied
-        }
-        const float f = mult / v_mult;
-        v_mult = mult;
+      float l[NS][4], l_top[NS];  // logits in powers of two of pair 4 i + t at positions g + 8 u
 #pragma unroll
-        for (int n = 0; n < kNP; ++n) {
+      for (int i = 0; i < NS; ++i)
 #pragma unroll
-          for (int m = 0; m < kM; ++m)
+        for (int u = 0; u < 4; ++u)
+          l[i][u] = static_cast<float>(s[i][u >> 1][2 * (u & 1)] * 256 + s[i][u >> 1][2 * (u & 1) + 1] - l_off[i]) * (fk[u] * l_scale[i]);
+      if (!(t0 >= all_lo && t0 + kTile - 1 <= all_hi)) {  // the same for the whole warp
+        asm volatile("" ::: "memory");  // (a branch, not selects)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[n][m][i] *= f;
+        for (int i = 0; i < NS; ++i)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) osum[n][i] *= f;
-        }
-      }
-      float l[NS][4];  // logits in powers of two of pair 4 i + t at positions g + 8 u
-      float passed = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          l[i][u] = (s[i][u >> 1][2 * (u & 1)] + s[i][u >> 1][2 * (u & 1) + 1]) * (fk[u] * l_scale[i]);
-          if (!unmasked) {
+          for (int u = 0; u < 4; ++u) {
             const int pos = t0 + g + 8 * u;
             if (pos > pos_col[i] || pos < lo_col[i]) l[i][u] = -INFINITY;
           }
-        }
-        // (-inf against a maximum of -inf is no move; nor is anything against NaN)
-        const float top = fmaxf(fmaxf(l[i][0], l[i][1]), fmaxf(l[i][2], l[i][3]));
-        passed = fmaxf(passed, top > m_run[i] ? top - m_run[i] : -INFINITY);
       }
-      if (__any_sync(0xffffffffu, passed > 4.0f)) {
+      const float v_top = fmaxf(fmaxf(fv[0], fv[1]), fmaxf(fv[2], fv[3]));
+      bool moves = v_top > v_cap;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        l_top[i] = fmaxf(fmaxf(l[i][0], l[i][1]), fmaxf(l[i][2], l[i][3]));
+        moves |= l_top[i] > m_pass[i];
+      }
+      if (__any_sync(0xffffffffu, moves)) {
+        float f = 1.0f;
+        if (__any_sync(0xffffffffu, v_top > v_cap)) {
+          const float top = warp_max(v_top);
+          float mult = 1.0f;
+          v_cap = 0.0f;
+          if (top > 0.0f && top < INFINITY) {
+            const int ex = min(max(((__float_as_int(top) >> 23) & 0xff) - 127, -100), 100);
+            mult = __int_as_float((127 + 8 - ex) << 23);
+            v_cap = __int_as_float((127 + 3 + ex) << 23);  // 2^11 once multiplied
+          }
+          f = mult / v_mult;
+          v_mult = mult;
+        }
+        const float log_mult = static_cast<float>(((__float_as_int(v_mult) >> 23) & 0xff) - 127);
         float corr[2 * kNP];
         corr[2 * kNP - 1] = 1.0f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-          float top = fmaxf(fmaxf(l[i][0], l[i][1]), fmaxf(l[i][2], l[i][3]));
+          float top = l_top[i];
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
           const float m_new = fmaxf(m_run[i], top);
-          corr[i] = m_new == -INFINITY ? 1.0f : exp2_fast(m_run[i] - m_new);
-          l_run[i] *= corr[i], m_run[i] = m_new;
+          corr[i] = m_new == -INFINITY ? 1.0f : exp2_fast(m_run[i] - m_new) * f;
+          l_run[i] *= corr[i], m_run[i] = m_new, m_pass[i] = m_new + 4.0f;
+          e_base[i] = (m_new == -INFINITY ? 0.0f : m_new) - log_mult;
         }
 #pragma unroll
         for (int n = 0; n < kNP; ++n) {
@@ -474,8 +485,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
           if (kE == 2) osum[n][1] *= corr[2 * n + 1];
         }
       }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) fv[u] *= v_mult;
       uint32_t pb[kNP][2][2];
 #pragma unroll
       for (int n = 0; n < kNP; ++n) {
@@ -483,10 +492,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
           const int i = 2 * n + e;
-          const float base = m_run[i] == -INFINITY ? 0.0f : m_run[i];
           float pr[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) pr[u] = exp2_fast(l[i][u] - base), pv[e][u] = pr[u] * fv[u];
+          for (int u = 0; u < 4; ++u) pr[u] = exp2_fast(l[i][u] - e_base[i]), pv[e][u] = pr[u] * fv[u];
           l_run[i] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
         }
 #pragma unroll
@@ -500,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 #pragma unroll
         for (int c = 0; c < D / 32; c += 2) {
           uint32_t v[4];  // positions 0-7 and 8-15 of the half, dims 32 c ..; the same, dims 32 (c + 1) ..
-          load_8x8_trans(v, at + v_piece<D>(r, c + (lane >> 4)) * 16);
+          load_8x8_trans(v, at + piece_at<D>(r, c + (lane >> 4)) * 16);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const uint32_t a = v[2 * u], b = v[2 * u + 1], a8 = a >> 8, b8 = b >> 8;
@@ -531,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       l += __shfl_xor_sync(0xffffffffu, l, 4);
       l += __shfl_xor_sync(0xffffffffu, l, 8);
       l += __shfl_xor_sync(0xffffffffu, l, 16);
-      if (g == 0) park[kC * (D + kPad) + 2 * c] = m_run[i], park[kC * (D + kPad) + 2 * c + 1] = l;
+      if (g == 0) park[kC * (D + kPad) + 2 * c] = m_run[i], park[kC * (D + kPad) + 2 * c + 1] = l / v_mult;
       const float off = osum[n][e] * (8.0f / 16777216.0f);
 #pragma unroll
       for (int m = 0; m < kM; ++m)  // rows g, g + 8: dims 32 (m / 2) + 4 g + 2 (m % 2), + 1

@@ -5,15 +5,14 @@ Tolerances (a rounding is off by at most half a step, eps / 2 of its type: bf16 
   codes, scales, read-back   equal (codes are those of exact arithmetic, the scale is one rounding)
   q_rot                      2^-8 |exact| for the store, and 12 f32 roundings (square sum, root, weight, rotation) of the
                              pair's larger value: 12 * 2^-24 * 2 max(|a|, |b|)
-  attention                  2^-8 |exact| for the store; P is fp16: 2^-11 sum p |v|; a logit is off by the f32 sum of d
-                             products of up to 15 |q| and by what q loses as two e4m3 numbers, 2^-17 of the head's largest
-                             (scaled into [128, 256), their step is 2^-9, so it is off by at most 2^-10), times |c| <= 7: p
-                             by twice that, 2 dl sum p |v|, dl = scale max(s_k) (15 sum|q| (d + 8) 2^-23 + 7 d 2^-17 max|q|),
-                             and by 2^-20 for exp2; the sums over u = c + 8 instead of c add at most
-                             16 sum p s_v (steps + 16) 2^-23, steps = 16-position steps of a warp; and what lies below the
-                             range of fp16: p s_v is kept times mult >= 2^8 / max(s_v) in steps of 2^-24, so each of the
-                             n positions is off by at most 2^-25 / mult <= 2^-33 max(s_v), times |c| <= 7, over a sum of p
-                             of at least 1: 7 n 2^-33 max(s_v)
+  attention                  2^-8 |exact| for the store; P is fp16: 2^-11 sum p |v|; q is a 16-bit integer round(q 32639 /
+                             max |q|), off by at most max |q| / 65278 < 1.01 2^-17 2 max |q|, times |c| <= 7, and a logit is
+                             three f32 roundings of an exact integer: p is off by twice dl, 2 dl sum p |v|, dl = scale
+                             max(s_k) (7 d 1.01 2^-16 max |q| + 4 * 2^-24 * 7 sum |q|), and by 2^-20 for exp2; the sums over
+                             u = c + 8 instead of c add at most 16 sum p s_v (steps + 16) 2^-23, steps = 16-position steps of
+                             a warp; and what lies below the range of fp16: p s_v is kept times mult >= 2^8 / max(s_v) in
+                             steps of 2^-24, so each of the n positions is off by at most 2^-25 / mult <= 2^-33 max(s_v),
+                             times |c| <= 7, over a sum of p of at least 1: 7 n 2^-33 max(s_v)
   prefill through the 8-bit kernels (32 rows and more): that form's own bar, 0.01 + 2^-8 |exact|, tests/test_gpu_attn_prefill_tc.py
 """
 import numpy as np
@@ -222,8 +221,8 @@ def attention64(q, p, codes, tables_, row_pos, per, Hq, Hk, d, scale, window, st
             v = codes[1][h, at].double() * p.vs[h, at].double()[:, None]
             x = qd[r, h * G:(h + 1) * G]
             w = torch.softmax(scale * x @ k.t(), -1)
-            dl = abs(scale) * p.ks[h, at].max().double() * (15 * x.abs().sum(-1) * (d + 8) * 2.0**-23 +
-                                                            7 * d * 2.0**-17 * x.abs().amax(-1))
+            dl = abs(scale) * p.ks[h, at].max().double() * (7 * d * 1.01 * 2.0**-16 * x.abs().amax(-1) +
+                                                            28 * 2.0**-24 * x.abs().sum(-1))
             e = w @ v
             off = 2.0**-8 * e.abs() + (2.0**-11 + 2.0**-20 + 2 * dl)[:, None] * (w @ v.abs())
             off += 16 * (steps + 16) * 2.0**-23 * (w @ p.vs[h, at].double())[:, None]
