@@ -53,8 +53,9 @@ namespace {
 constexpr int kTile = 32;     // positions a warp works on at a time
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxGroups = 512;   // of a launch that splits the line of tiles
-constexpr int kMaxShares = 1024;  // it is cut into
+constexpr int kMaxGroups = 2 * kThreads;  // of a launch that splits the line of tiles
+constexpr int kMaxShares = 640;   // it is cut into
+constexpr int kKept = 64;         // groups whose span and table are kept in shared memory
 constexpr int kMaxColumns = 64;   // rows of a group x query heads of a kv head
 
 struct Int4AttnParams {
@@ -70,8 +71,9 @@ struct Int4AttnParams {
   uint16_t* out;
   float* part_o;   // [slots][columns][D]
   float* part_ml;  // [slots][columns][2]
-  int* prefix;     // [groups + 1] tiles before each group
+  int* prefix;     // [groups + 1] tiles or chunks before each group, then the shares of a straight cut (0: chunks)
   int rows, per, groups, Hq, Hk, G, blocks;  // blocks: column blocks of a segment
+  unsigned g_inv;  // ceil(65536 / G): c / G = c * g_inv >> 16 for c < 256
   long long stride;
   int max_len, window;
   float scale_log2;
@@ -125,21 +127,10 @@ __device__ __forceinline__ void group_span(const Int4AttnParams& p, int grp, int
     lo = min(lo, p.window > 0 ? max(0, pos + 1 - p.window) : 0);
   }
 }
-__device__ __forceinline__ int group_tiles(const Int4AttnParams& p, int grp) {
-  int lo, hi;
-  group_span(p, grp, lo, hi);
-  return hi < 0 ? 0 : hi / kTile - lo / kTile + 1;
-}
-
-// s_prefix[g] = tiles of the groups before g, s_prefix[groups] = all.
-__device__ void scan_groups(const Int4AttnParams& p, int* s_prefix) {
-  __shared__ int s_warp[kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int each = (p.groups + kThreads - 1) / kThreads, g0 = threadIdx.x * each;
-  int sum = 0;
-  for (int i = 0; i < each; ++i)
-    if (g0 + i < p.groups) sum += group_tiles(p, g0 + i);
-  int inc = sum;
+// s_prefix[g] = sum over the groups before g, s_prefix[groups] = over all, of the values a (group 2 tid) and b (2 tid + 1).
+__device__ __forceinline__ void scan_groups(int a, int b, int groups, int* s_prefix, int* s_warp) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = 2 * threadIdx.x;
+  int inc = a + b;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -147,18 +138,39 @@ __device__ void scan_groups(const Int4AttnParams& p, int* s_prefix) {
   }
   if (lane == 31) s_warp[warp] = inc;
   __syncthreads();
-  int before = inc - sum;
+  int before = inc - a - b;
   for (int w = 0; w < warp; ++w) before += s_warp[w];
-  for (int i = 0; i < each; ++i)
-    if (g0 + i < p.groups) s_prefix[g0 + i] = before, before += group_tiles(p, g0 + i);
-  if (threadIdx.x == kThreads - 1) s_prefix[p.groups] = s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3];
+  if (g <= groups) s_prefix[g] = before;
+  if (g + 1 <= groups) s_prefix[g + 1] = before + a;
+  if (threadIdx.x == kThreads - 1 && groups == kMaxGroups) s_prefix[kMaxGroups] = before + a + b;
   __syncthreads();
 }
 
-// CTAs that a line of `all` tiles is cut for: every share has a tile at least, and one for each warp where there are so many.
-__device__ __forceinline__ long long shares_of(long long all, int shares) {
-  return min(static_cast<long long>(shares), (all + kWarps - 1) / kWarps);
+// The line of `all` tiles is cut straight, into shares that differ by a tile at most, whatever segments they cross, or,
+// where a share would be short and the segments are few, into chunks of equal parts of each segment: a CTA that crosses
+// from one segment to the next pays the start of a piece (a chain of dependent loads, 3 us) twice. `chunk` is a
+// chunk's largest length, 0 for the straight cut.
+struct Cut {
+  int shares, quot, rest, chunk;
+};
+constexpr int kShortShare = 64;  // tiles
+__device__ __forceinline__ Cut cut_line(int all, int segments, int ctas) {
+  Cut c;
+  c.shares = min(ctas, (all + kWarps - 1) / kWarps);  // a tile for each warp where there are so many
+  c.quot = c.shares > 0 ? all / c.shares : 0, c.rest = c.shares > 0 ? all % c.shares : 0;
+  c.chunk = ctas >= 2 * segments && c.quot < kShortShare ? max(kWarps, (all + ctas - segments - 1) / (ctas - segments)) : 0;
+  return c;
 }
+// The share of a straight cut that holds tile x.
+__device__ __forceinline__ int share_of(const Cut& c, int x) {
+  const int big = c.rest * (c.quot + 1);
+  return x < big ? x / (c.quot + 1) : c.rest + (x - big) / c.quot;
+}
+
+struct GroupInfo {
+  const int* pt;
+  int lo, hi;
+};
 
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -194,14 +206,14 @@ constexpr int kPad = 4;  // floats after a parked row of O
 constexpr int ctas_per_sm(int ns) { return ns == 4 ? 3 : 4; }
 template <int D, int NS>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(const Int4AttnParams p) {
-  // a launch that splits the line is one resident wave: what comes next may be staged beside it
-  if (p.split) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   pdl_begin();
   constexpr int kC = 4 * NS, kNP = (NS + 1) / 2, kE = NS == 1 ? 1 : 2;
   constexpr int kW = D / 32 /* K words of a row per lane */, kM = D / 16 /* 16-dim tiles of O^T */;
   constexpr int kRB = kRowBytes<D>, kVAt = kTile * kRB, kSAt = 2 * kTile * kRB;
   static_assert(kWarpBytes<D> >= kC * (D + kPad) * 4 + kC * 8, "a warp parks its state in its ring");
   __shared__ int s_prefix[kMaxGroups + 1];
+  __shared__ int s_warp[kWarps];
+  __shared__ GroupInfo s_kept[kKept];
   __shared__ __align__(16) unsigned char s_q[8 * NS][D + 16];  // a row per column of the logit tiles
   __shared__ float2 s_pair[4 * NS];                            // logit scale, 8 sum q (an integer)
   extern __shared__ __align__(128) unsigned char s_ring[];
@@ -209,20 +221,42 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
   unsigned char* const ring = s_ring + warp * kWarpBytes<D>;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   const int per_group = p.Hk * p.blocks;
-  long long x = 0, x_end = 0;  // this CTA's share of the line of tiles
+  int x = 0, x_end = 1, chunk = 0;  // this CTA's share of the line, or its chunk
   int grp = 0, sub = 0;
   if (p.split) {
-    scan_groups(p, s_prefix);
-    const long long all = static_cast<long long>(s_prefix[p.groups]) * per_group;
-    const long long shares = shares_of(all, gridDim.x);
-    if (blockIdx.x == 0)
+    int tiles[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int gi = 2 * threadIdx.x + i;
+      if (gi < p.groups) {
+        GroupInfo info;
+        info.pt = p.row_pt != nullptr ? p.row_pt[gi * p.per] : p.pt;
+        group_span(p, gi, info.lo, info.hi);
+        tiles[i] = info.hi < 0 ? 0 : info.hi / kTile - info.lo / kTile + 1;
+        if (gi < kKept) s_kept[gi] = info;
+      }
+    }
+    scan_groups(tiles[0], tiles[1], p.groups, s_prefix, s_warp);
+    const Cut cut = cut_line(s_prefix[p.groups] * per_group, p.groups * per_group, gridDim.x);
+    chunk = cut.chunk;
+    if (chunk > 0) {
+      __syncthreads();
+      scan_groups((tiles[0] + chunk - 1) / chunk, (tiles[1] + chunk - 1) / chunk, p.groups, s_prefix, s_warp);
+      x = blockIdx.x;
+      x_end = min(x + 1, s_prefix[p.groups] * per_group);
+    } else {
+      x = blockIdx.x * cut.quot + min(static_cast<int>(blockIdx.x), cut.rest);
+      x_end = static_cast<int>(blockIdx.x) < cut.shares ? x + cut.quot + (static_cast<int>(blockIdx.x) < cut.rest ? 1 : 0) : x;
+    }
+    if (blockIdx.x == 0) {
       for (int i = threadIdx.x; i <= p.groups; i += kThreads) p.prefix[i] = s_prefix[i];
-    if (blockIdx.x >= shares) return;
-    x = blockIdx.x * all / shares, x_end = (blockIdx.x + 1) * all / shares;
+      if (threadIdx.x == 0) p.prefix[p.groups + 1] = chunk > 0 ? 0 : cut.shares;
+    }
+    if (x >= x_end) return;
     int lo = 0, hi = p.groups - 1;  // the last group that begins at or before x
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (static_cast<long long>(s_prefix[mid]) * per_group <= x) lo = mid;
+      if (s_prefix[mid] * per_group <= x) lo = mid;
       else hi = mid - 1;
     }
     grp = lo;
@@ -230,31 +264,57 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 
   while (true) {
     int n_tiles, first_tile, piece_begin, piece_end;  // of this segment's tiles
-    int span_lo, span_hi;
     if (p.split) {
       if (x >= x_end) return;
-      while (static_cast<long long>(s_prefix[grp + 1]) * per_group <= x) ++grp;
-      n_tiles = s_prefix[grp + 1] - s_prefix[grp];
-      const long long in = x - static_cast<long long>(s_prefix[grp]) * per_group;
-      sub = static_cast<int>(in / n_tiles);
-      piece_begin = static_cast<int>(in % n_tiles);
-      piece_end = static_cast<int>(min(static_cast<long long>(n_tiles), piece_begin + (x_end - x)));
-      x += piece_end - piece_begin;
+      while (s_prefix[grp + 1] * per_group <= x) ++grp;
+      const int units = s_prefix[grp + 1] - s_prefix[grp], in = x - s_prefix[grp] * per_group;  // tiles or chunks
+      sub = in / units;
+      piece_begin = in - sub * units, piece_end = units;
     } else {
-      grp = blockIdx.x / per_group, sub = blockIdx.x % per_group;
-      piece_begin = 0;
+      grp = blockIdx.x / per_group, sub = blockIdx.x - grp * per_group;
+      piece_begin = 0, piece_end = 1;
     }
-    group_span(p, grp, span_lo, span_hi);
-    first_tile = span_hi < 0 ? 0 : span_lo / kTile;
-    if (!p.split) n_tiles = piece_end = span_hi < 0 ? 0 : span_hi / kTile - first_tile + 1;
-    const int hkv = sub / p.blocks, c0 = (sub % p.blocks) * kC;
+    const int hkv = p.blocks == 1 ? sub : sub / p.blocks, c0 = p.blocks == 1 ? 0 : (sub % p.blocks) * kC;
     const int r0 = grp * p.per, nrows = min(p.per, p.rows - r0), columns = min(kC, nrows * p.G - c0);
+    // what the piece needs first and does not depend on one another: q, positions, the table's address
+    uint32_t q_raw[NS][D / 64];
+    int pos_raw[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int cq = i * kWarps + warp, cp = 4 * i + t;
+      const int j = (c0 + cq) * p.g_inv >> 16, hl = c0 + cq - j * p.G;
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e)
+        q_raw[i][e] = cq < columns ? __ldg(reinterpret_cast<const uint32_t*>(p.q + (static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + lane * (D / 32)) + e) : 0u;
+      const int row = r0 + ((c0 + cp) * p.g_inv >> 16);
+      pos_raw[i] = cp < columns ? (p.row_pos != nullptr ? __ldg(p.row_pos + row) : p.base_pos + row) : INT_MAX;
+    }
+    GroupInfo info;
+    if (p.split && grp < kKept) {
+      info = s_kept[grp];
+    } else {
+      info.pt = p.row_pt != nullptr ? p.row_pt[r0] : p.pt;
+      group_span(p, grp, info.lo, info.hi);
+    }
+    const int span_lo = info.lo, span_hi = info.hi;
+    const int* const pt = info.pt;
+    first_tile = span_hi < 0 ? 0 : span_lo / kTile;
+    n_tiles = span_hi < 0 ? 0 : span_hi / kTile - first_tile + 1;
+    if (!p.split) {
+      piece_end = n_tiles;
+    } else if (chunk > 0) {
+      const int k = piece_begin, n = piece_end;
+      piece_begin = k * n_tiles / n, piece_end = (k + 1) * n_tiles / n;
+      x = x_end;
+    } else {
+      piece_end = min(n_tiles, piece_begin + x_end - x);
+      x += piece_end - piece_begin;
+    }
     const size_t head_row0 = static_cast<size_t>(hkv) * p.stride;
     const uint8_t* ck = p.ck + head_row0 * kRB;
     const uint8_t* cv = p.cv + head_row0 * kRB;
     const float* ks = p.ks + head_row0;
     const float* vs = p.vs + head_row0;
-    const int* pt = p.row_pt != nullptr ? p.row_pt[r0] : p.pt;
 
     // pool row of the lane's position of a tile (past the end of what the group sees: the end's)
     auto table_row = [&](int tile) -> int {
@@ -301,16 +361,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       constexpr int kPer = D / 32;
       float f[kPer];
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) f[e] = 0.0f;
-      if (c < columns) {
-        const int j = (c0 + c) / p.G, hl = (c0 + c) % p.G;
-        const uint16_t* qrow = p.q + (static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + lane * kPer;
-#pragma unroll
-        for (int e = 0; e < kPer; e += 2) {
-          const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(qrow + e));
-          f[e] = bf16_lo(w), f[e + 1] = bf16_hi(w);
-        }
-      }
+      for (int e = 0; e < kPer; e += 2) f[e] = bf16_lo(q_raw[i][e >> 1]), f[e + 1] = bf16_hi(q_raw[i][e >> 1]);
       float top = 0.0f;
 #pragma unroll
       for (int e = 0; e < kPer; ++e) top = fmaxf(top, fabsf(f[e]));
@@ -353,13 +404,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       }
       const int c = 4 * i + t;
       l_scale[i] = s_pair[c].x, l_off[i] = __float_as_int(s_pair[c].y);
-      pos_col[i] = INT_MAX, lo_col[i] = 0;  // a column that is not there sees everything and is dropped
-      if (c < columns) {
-        const int row = r0 + (c0 + c) / p.G;
-        const int raw = p.row_pos != nullptr ? __ldg(p.row_pos + row) : p.base_pos + row;
-        const int pos = raw < 0 ? -1 : min(raw, p.max_len - 1);
-        pos_col[i] = pos, lo_col[i] = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
-      }
+      // a column that is not there sees everything and is dropped
+      pos_col[i] = pos_raw[i] < 0 ? -1 : c < columns ? min(pos_raw[i], p.max_len - 1) : INT_MAX;
+      lo_col[i] = c < columns && p.window > 0 ? max(0, pos_col[i] + 1 - p.window) : 0;
       all_hi = min(all_hi, pos_col[i]), all_lo = max(all_lo, lo_col[i]);
     }
 #pragma unroll
@@ -528,6 +575,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     }
 
     // the four warps' states meet in shared memory, each parked in the warp's own ring
+    if (p.split) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     copies_wait<0>();
     __syncwarp();
     float* const park = reinterpret_cast<float*>(ring);  // [kC][D + kPad], then [kC][2] (max, sum)
@@ -548,9 +596,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     }
     __syncthreads();
     const bool whole = piece_begin == 0 && piece_end == n_tiles;
-    const size_t slot = static_cast<size_t>(blockIdx.x) + static_cast<size_t>(grp) * per_group + sub;
-    for (int i = threadIdx.x; i < columns * D; i += kThreads) {
-      const int c = i / D, dim = i % D;
+    const size_t slot = blockIdx.x + (chunk > 0 ? 0 : static_cast<size_t>(grp) * per_group + sub);
+    const int dim = threadIdx.x % D;
+    for (int c = threadIdx.x / D; c < columns; c += kThreads / D) {
       float mw[kWarps], m = -INFINITY, l = 0.0f, acc = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
@@ -560,13 +608,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float* parked = reinterpret_cast<const float*>(s_ring + w * kWarpBytes<D>);
-        const float f = mw[w] == -INFINITY ? 0.0f : exp2f(mw[w] - m);
+        const float f = mw[w] == -INFINITY ? 0.0f : exp2_fast(mw[w] - m);
         l += f * parked[kC * (D + kPad) + 2 * c + 1], acc += f * parked[c * (D + kPad) + dim];
       }
       if (whole) {
-        const int row = r0 + (c0 + c) / p.G, hl = (c0 + c) % p.G;
-        p.out[(static_cast<size_t>(row) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + dim] =
-            static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? acc / l : 0.0f));
+        const int j = (c0 + c) * p.g_inv >> 16, hl = c0 + c - j * p.G;
+        p.out[(static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + dim] =
+            static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? __fdividef(acc, l) : 0.0f));
       } else {
         p.part_o[(slot * kC + c) * D + dim] = acc;
         if (dim == 0) p.part_ml[(slot * kC + c) * 2] = m, p.part_ml[(slot * kC + c) * 2 + 1] = l;
@@ -578,42 +626,64 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 }
 
 // Joins the pieces of segments that several CTAs worked on: a CTA per segment and column. The pieces' weights
-// exp2(m - max) are worked out side by side; then each warp adds every fourth piece, eight loads of a lane in flight,
-// and the four sums meet in shared memory. The order depends on the number of pieces alone.
+// exp2(m - max) are worked out side by side while the first pieces are on their way; each warp adds every fourth piece,
+// eight loads of a lane in flight, and the four sums meet in shared memory. The order depends on the number of pieces
+// alone.
 template <int D, int NS>
-__global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4AttnParams p, int max_shares) {
+__global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4AttnParams p, int ctas) {
   pdl_begin();
-  constexpr int kC = 4 * NS, kPer = D / 32;
+  constexpr int kC = 4 * NS, kPer = D / 32, kFly = 8;
   __shared__ float s_w[kMaxShares];
   __shared__ float s_red[2][kWarps];
   __shared__ float s_acc[kWarps][D];
-  const int per_group = p.Hk * p.blocks, grp = blockIdx.x / per_group, sub = blockIdx.x % per_group, c = blockIdx.y;
-  const int hkv = sub / p.blocks, c0 = (sub % p.blocks) * kC, r0 = grp * p.per, nrows = min(p.per, p.rows - r0);
+  const int per_group = p.Hk * p.blocks, grp = blockIdx.x / per_group, sub = blockIdx.x - grp * per_group, c = blockIdx.y;
+  const int hkv = p.blocks == 1 ? sub : sub / p.blocks, c0 = p.blocks == 1 ? 0 : (sub % p.blocks) * kC;
+  const int r0 = grp * p.per, nrows = min(p.per, p.rows - r0);
   if (c >= min(kC, nrows * p.G - c0)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int before = __ldcg(p.prefix + grp), n_tiles = __ldcg(p.prefix + grp + 1) - before;
-  const long long all = static_cast<long long>(__ldcg(p.prefix + p.groups)) * per_group;
-  const long long x0 = static_cast<long long>(before) * per_group + static_cast<long long>(sub) * n_tiles;
-  int i0 = 0, n = 0;  // the first of the CTAs whose shares hold the segment's tiles, and how many there are
-  if (n_tiles > 0) {
-    const long long shares = shares_of(all, max_shares);
-    i0 = static_cast<int>(((x0 + 1) * shares - 1) / all), n = static_cast<int>(((x0 + n_tiles) * shares - 1) / all) - i0 + 1;
-    if (n == 1) return;  // written by that CTA
+  const int before = __ldcg(p.prefix + grp), units = __ldcg(p.prefix + grp + 1) - before;
+  const int all = __ldcg(p.prefix + p.groups) * per_group, shares = __ldcg(p.prefix + p.groups + 1);
+  int n = units, slot = before * per_group + sub * units;  // pieces of the segment, and where the first one lies
+  if (n > 0 && shares > 0) {
+    const Cut cut = cut_line(all, p.groups * per_group, ctas);
+    const int i0 = share_of(cut, slot);
+    n = share_of(cut, slot + units - 1) - i0 + 1, slot = i0 + blockIdx.x;
   }
-  const size_t first = (static_cast<size_t>(i0) + blockIdx.x) * kC + c;  // (slot, column) of the first piece
+  if (n == 1) return;  // written by the one CTA
+  const float* const part_ml = p.part_ml + (static_cast<size_t>(slot) * kC + c) * 2;
+  const float* const part_o = p.part_o + (static_cast<size_t>(slot) * kC + c) * D + lane * kPer;
+  float v[kFly][kPer];
+  auto load = [&](int i) {
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      const int s = i + u * kWarps;
+#pragma unroll
+      for (int e = 0; e < kPer; e += 2) {
+        const float2 w = s < n ? __ldcg(reinterpret_cast<const float2*>(part_o + static_cast<size_t>(s) * (kC * D) + e)) : make_float2(0.0f, 0.0f);
+        v[u][e] = w.x, v[u][e + 1] = w.y;
+      }
+    }
+  };
+  load(warp);
   float m = -INFINITY, l = 0.0f;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    s_w[i] = __ldcg(p.part_ml + (first + static_cast<size_t>(i) * kC) * 2);
-    m = fmaxf(m, s_w[i]);
+  constexpr int kEach = (kMaxShares + kThreads - 1) / kThreads;
+  float2 ml[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = threadIdx.x + k * kThreads;
+    ml[k] = i < n ? __ldcg(reinterpret_cast<const float2*>(part_ml + static_cast<size_t>(i) * (kC * 2))) : make_float2(-INFINITY, 0.0f);
+    m = fmaxf(m, ml[k].x);
   }
   m = warp_max(m);
   if (lane == 0) s_red[0][warp] = m;
   __syncthreads();
   m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const float f = s_w[i] == -INFINITY ? 0.0f : exp2f(s_w[i] - m);
-    s_w[i] = f;
-    l += f * __ldcg(p.part_ml + (first + static_cast<size_t>(i) * kC) * 2 + 1);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = threadIdx.x + k * kThreads;
+    const float f = ml[k].x == -INFINITY ? 0.0f : exp2_fast(ml[k].x - m);
+    if (i < n) s_w[i] = f;
+    l += f * ml[k].y;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
@@ -622,19 +692,8 @@ __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4Attn
   float acc[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
-  constexpr int kFly = 8;
   for (int i = warp; i < n; i += kFly * kWarps) {
-    float v[kFly][kPer];
-#pragma unroll
-    for (int u = 0; u < kFly; ++u) {
-      const int s = i + u * kWarps;
-      const float* src = p.part_o + (first + static_cast<size_t>(s) * kC) * D + lane * kPer;
-#pragma unroll
-      for (int e = 0; e < kPer; e += 2) {
-        const float2 w = s < n ? __ldcg(reinterpret_cast<const float2*>(src + e)) : make_float2(0.0f, 0.0f);
-        v[u][e] = w.x, v[u][e + 1] = w.y;
-      }
-    }
+    if (i != warp) load(i);
 #pragma unroll
     for (int u = 0; u < kFly; ++u) {
       const float f = i + u * kWarps < n ? s_w[i + u * kWarps] : 0.0f;
@@ -649,9 +708,9 @@ __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4Attn
   const int dim = threadIdx.x;
   if (dim < D) {
     const float sum = (s_acc[0][dim] + s_acc[1][dim]) + (s_acc[2][dim] + s_acc[3][dim]);
-    const int row = r0 + (c0 + c) / p.G, hl = (c0 + c) % p.G;
-    p.out[(static_cast<size_t>(row) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + dim] =
-        static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? sum / l : 0.0f));
+    const int j = (c0 + c) * p.g_inv >> 16, hl = c0 + c - j * p.G;
+    p.out[(static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + dim] =
+        static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? __fdividef(sum, l) : 0.0f));
   }
 }
 
@@ -672,10 +731,10 @@ Int4Plan plan_int4(int rows, int per, int Hq, int Hk, int d, int max_len) {
   const long long tiles = s.segments * ((max_len + kTile - 1) / kTile);
   // short caches: a segment is one tile per warp. Many segments: the CTAs balance one another, and each saves its
   // neighbours the joining of a piece.
-  if (max_len <= kTile * kWarps || s.groups > kMaxGroups || s.segments >= 4 * resident) return s;
+  if (max_len <= kTile * kWarps || s.groups > kMaxGroups || s.segments >= 4 * resident || tiles > INT_MAX / 2) return s;
   s.shares = static_cast<int>(std::min(resident, std::max(1ll, tiles / kWarps)));
   const long long slots = s.shares + s.segments;
-  s.bytes = slots * 4 * s.ns * (d + 2) * 4 + (s.groups + 1 + 3) / 4 * 16;
+  s.bytes = slots * 4 * s.ns * (d + 2) * 4 + (s.groups + 2 + 3) / 4 * 16;
   return s;
 }
 
@@ -711,6 +770,7 @@ int attn_int4(const char* fn, Int4AttnParams p, int d, void* scratch, long long 
   p.G = p.Hq / p.Hk;
   Int4Plan s = plan_int4(p.rows, p.per, p.Hq, p.Hk, d, p.max_len);
   p.blocks = s.blocks, p.groups = s.groups;
+  p.g_inv = (65536u + p.G - 1) / p.G;
   const bool have = scratch != nullptr && scratch_bytes >= s.bytes && aligned16(scratch);
   if (s.shares > 0 && !have) {
     if (scratch_needed) return fail(fn, "scratch missing, misaligned or smaller than the size the scratch query returns");
