@@ -53,9 +53,8 @@ namespace {
 constexpr int kTile = 32;     // positions a warp works on at a time
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxGroups = 2 * kThreads;  // of a launch that splits the line of tiles
+constexpr int kMaxGroups = 256;   // of a launch that cuts the line of tiles
 constexpr int kMaxShares = 640;   // it is cut into
-constexpr int kKept = 64;         // groups whose span and table are kept in shared memory
 constexpr int kMaxColumns = 64;   // rows of a group x query heads of a kv head
 
 struct Int4AttnParams {
@@ -127,28 +126,31 @@ __device__ __forceinline__ void group_span(const Int4AttnParams& p, int grp, int
     lo = min(lo, p.window > 0 ? max(0, pos + 1 - p.window) : 0);
   }
 }
-// s_prefix[g] = sum over the groups before g, s_prefix[groups] = over all, of the values a (group 2 tid) and b (2 tid + 1).
-__device__ __forceinline__ void scan_groups(int a, int b, int groups, int* s_prefix, int* s_warp) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = 2 * threadIdx.x;
-  int inc = a + b;
+// Sum over the lanes before this one; `all` gets the sum over all lanes.
+__device__ __forceinline__ int sum_before(int v, int& all) {
+  const int lane = threadIdx.x & 31;
+  int inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += v;
+    const int u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
   }
-  if (lane == 31) s_warp[warp] = inc;
-  __syncthreads();
-  int before = inc - a - b;
-  for (int w = 0; w < warp; ++w) before += s_warp[w];
-  if (g <= groups) s_prefix[g] = before;
-  if (g + 1 <= groups) s_prefix[g + 1] = before + a;
-  if (threadIdx.x == kThreads - 1 && groups == kMaxGroups) s_prefix[kMaxGroups] = before + a + b;
-  __syncthreads();
+  all = __shfl_sync(0xffffffffu, inc, 31);
+  return inc - v;
 }
+
+// a / d for quotients below 2^21: a float quotient is then off by less than one.
+__device__ __forceinline__ int quotient(int a, int d) {
+  int q = static_cast<int>(__fdividef(static_cast<float>(a), static_cast<float>(d)));
+  const int r = a - q * d;
+  q += (r >= d ? 1 : 0) - (r < 0 ? 1 : 0);
+  return q;
+}
+constexpr int kMaxQuotient = 1 << 21;
 
 // The line of `all` tiles is cut straight, into shares that differ by a tile at most, whatever segments they cross, or,
 // where a share would be short and the segments are few, into chunks of equal parts of each segment: a CTA that crosses
-// from one segment to the next pays the start of a piece (a chain of dependent loads, 3 us) twice. `chunk` is a
+// from one segment to the next pays the start of a piece (a chain of dependent loads, 2 us) twice. `chunk` is a
 // chunk's largest length, 0 for the straight cut.
 struct Cut {
   int shares, quot, rest, chunk;
@@ -156,21 +158,16 @@ struct Cut {
 constexpr int kShortShare = 64;  // tiles
 __device__ __forceinline__ Cut cut_line(int all, int segments, int ctas) {
   Cut c;
-  c.shares = min(ctas, (all + kWarps - 1) / kWarps);  // a tile for each warp where there are so many
-  c.quot = c.shares > 0 ? all / c.shares : 0, c.rest = c.shares > 0 ? all % c.shares : 0;
-  c.chunk = ctas >= 2 * segments && c.quot < kShortShare ? max(kWarps, (all + ctas - segments - 1) / (ctas - segments)) : 0;
+  c.shares = all >= ctas * kWarps ? ctas : max(1, all / kWarps);  // a tile for each warp
+  c.quot = quotient(all, c.shares), c.rest = all - c.quot * c.shares;
+  c.chunk = ctas >= 2 * segments && c.quot < kShortShare ? max(kWarps, quotient(all + ctas - segments - 1, ctas - segments)) : 0;
   return c;
 }
 // The share of a straight cut that holds tile x.
 __device__ __forceinline__ int share_of(const Cut& c, int x) {
   const int big = c.rest * (c.quot + 1);
-  return x < big ? x / (c.quot + 1) : c.rest + (x - big) / c.quot;
+  return x < big ? quotient(x, c.quot + 1) : c.rest + quotient(x - big, c.quot);
 }
-
-struct GroupInfo {
-  const int* pt;
-  int lo, hi;
-};
 
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -202,77 +199,97 @@ constexpr int kPad = 4;  // floats after a parked row of O
 
 // NS logit tiles of four columns each: column 4 i + t of column block cb is pair c = 4 NS cb + 4 i + t, query row c / G,
 // query head c % G. P and O have a tile of eight columns for two of them: column 2 t + e of tile n is pair 4 (2 n + e) + t
-// (NS = 1: odd columns are zero).
-constexpr int ctas_per_sm(int ns) { return ns == 4 ? 3 : 4; }
+// (an odd NS: the odd columns of the last tile are zero).
+constexpr int ctas_per_sm(int ns) { return ns >= 3 ? 3 : 4; }
 template <int D, int NS>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(const Int4AttnParams p) {
   pdl_begin();
-  constexpr int kC = 4 * NS, kNP = (NS + 1) / 2, kE = NS == 1 ? 1 : 2;
+  constexpr int kC = 4 * NS, kNP = (NS + 1) / 2;
   constexpr int kW = D / 32 /* K words of a row per lane */, kM = D / 16 /* 16-dim tiles of O^T */;
   constexpr int kRB = kRowBytes<D>, kVAt = kTile * kRB, kSAt = 2 * kTile * kRB;
   static_assert(kWarpBytes<D> >= kC * (D + kPad) * 4 + kC * 8, "a warp parks its state in its ring");
-  __shared__ int s_prefix[kMaxGroups + 1];
-  __shared__ int s_warp[kWarps];
-  __shared__ GroupInfo s_kept[kKept];
   __shared__ __align__(16) unsigned char s_q[8 * NS][D + 16];  // a row per column of the logit tiles
-  __shared__ float2 s_pair[4 * NS];                            // logit scale, 8 sum q (an integer)
+  __shared__ float s_scale[4 * NS];                            // of a pair's logits
   extern __shared__ __align__(128) unsigned char s_ring[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   unsigned char* const ring = s_ring + warp * kWarpBytes<D>;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   const int per_group = p.Hk * p.blocks;
+  // Every warp lays out the line for itself: lane L has groups [L n, L n + n), their tiles (or chunks) and those before.
   int x = 0, x_end = 1, chunk = 0;  // this CTA's share of the line, or its chunk
-  int grp = 0, sub = 0;
+  const int lane_groups = (p.groups + 31) >> 5, lane_first = lane * lane_groups;
+  int lane_units = 0, lane_before = 0, lane_lo = 0, lane_hi = -1;
+  const int* lane_pt = nullptr;  // span and table of a lane's only group
+  auto units_of = [&](int grp) -> int {
+    int lo = lane_lo, hi = lane_hi;
+    if (lane_groups > 1) group_span(p, grp, lo, hi);
+    const int n = hi < 0 ? 0 : hi / kTile - lo / kTile + 1;
+    return chunk > 0 ? quotient(n + chunk - 1, chunk) : n;
+  };
   if (p.split) {
-    int tiles[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int gi = 2 * threadIdx.x + i;
-      if (gi < p.groups) {
-        GroupInfo info;
-        info.pt = p.row_pt != nullptr ? p.row_pt[gi * p.per] : p.pt;
-        group_span(p, gi, info.lo, info.hi);
-        tiles[i] = info.hi < 0 ? 0 : info.hi / kTile - info.lo / kTile + 1;
-        if (gi < kKept) s_kept[gi] = info;
-      }
+    const int lane_end = min(lane_first + lane_groups, p.groups);
+    if (lane_groups == 1 && lane_first < lane_end) {
+      lane_pt = p.row_pt != nullptr ? p.row_pt[lane_first * p.per] : p.pt;
+      group_span(p, lane_first, lane_lo, lane_hi);
     }
-    scan_groups(tiles[0], tiles[1], p.groups, s_prefix, s_warp);
-    const Cut cut = cut_line(s_prefix[p.groups] * per_group, p.groups * per_group, gridDim.x);
+    int all;
+#pragma unroll 1
+    for (int gi = lane_first; gi < lane_end; ++gi) lane_units += units_of(gi);
+    lane_before = sum_before(lane_units, all);
+    const Cut cut = cut_line(all * per_group, p.groups * per_group, gridDim.x);
     chunk = cut.chunk;
     if (chunk > 0) {
-      __syncthreads();
-      scan_groups((tiles[0] + chunk - 1) / chunk, (tiles[1] + chunk - 1) / chunk, p.groups, s_prefix, s_warp);
+      lane_units = 0;
+#pragma unroll 1
+      for (int gi = lane_first; gi < lane_end; ++gi) lane_units += units_of(gi);
+      lane_before = sum_before(lane_units, all);
       x = blockIdx.x;
-      x_end = min(x + 1, s_prefix[p.groups] * per_group);
+      x_end = min(x + 1, all * per_group);
     } else {
       x = blockIdx.x * cut.quot + min(static_cast<int>(blockIdx.x), cut.rest);
       x_end = static_cast<int>(blockIdx.x) < cut.shares ? x + cut.quot + (static_cast<int>(blockIdx.x) < cut.rest ? 1 : 0) : x;
     }
-    if (blockIdx.x == 0) {
-      for (int i = threadIdx.x; i <= p.groups; i += kThreads) p.prefix[i] = s_prefix[i];
-      if (threadIdx.x == 0) p.prefix[p.groups + 1] = chunk > 0 ? 0 : cut.shares;
+    if (blockIdx.x == 0 && warp == 0) {
+      int before = lane_before;
+#pragma unroll 1
+      for (int gi = lane_first; gi < lane_end; ++gi) p.prefix[gi] = before, before += units_of(gi);
+      if (lane == 0) p.prefix[p.groups] = all, p.prefix[p.groups + 1] = chunk > 0 ? 0 : cut.shares;
     }
-    if (x >= x_end) return;
-    int lo = 0, hi = p.groups - 1;  // the last group that begins at or before x
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_prefix[mid] * per_group <= x) lo = mid;
-      else hi = mid - 1;
-    }
-    grp = lo;
   }
 
   while (true) {
-    int n_tiles, first_tile, piece_begin, piece_end;  // of this segment's tiles
+    int grp, sub, n_tiles, first_tile, piece_begin, piece_end;  // of this segment's tiles
+    int span_lo, span_hi;
+    const int* pt;
     if (p.split) {
       if (x >= x_end) return;
-      while (s_prefix[grp + 1] * per_group <= x) ++grp;
-      const int units = s_prefix[grp + 1] - s_prefix[grp], in = x - s_prefix[grp] * per_group;  // tiles or chunks
-      sub = in / units;
+      const int at = quotient(x, per_group);  // the group that holds the line's unit x
+      const int owner = 31 - __clz(__ballot_sync(0xffffffffu, lane_units > 0 && lane_before <= at));
+      int found = lane_first, before = lane_before, units = lane_units;
+      if (lane_groups > 1 && lane == owner) {
+#pragma unroll 1
+        for (int gi = lane_first, next = lane_before; gi < min(lane_first + lane_groups, p.groups) && next <= at; ++gi) {
+          const int n = units_of(gi);
+          if (n > 0) found = gi, before = next, units = n;
+          next += n;
+        }
+      }
+      grp = __shfl_sync(0xffffffffu, found, owner);
+      before = __shfl_sync(0xffffffffu, before, owner), units = __shfl_sync(0xffffffffu, units, owner);
+      const int in = x - before * per_group;
+      sub = quotient(in, units);
       piece_begin = in - sub * units, piece_end = units;
+      if (lane_groups == 1) {
+        span_lo = __shfl_sync(0xffffffffu, lane_lo, owner), span_hi = __shfl_sync(0xffffffffu, lane_hi, owner);
+        pt = reinterpret_cast<const int*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(lane_pt), owner));
+      }
     } else {
       grp = blockIdx.x / per_group, sub = blockIdx.x - grp * per_group;
       piece_begin = 0, piece_end = 1;
+    }
+    if (!p.split || lane_groups > 1) {
+      pt = p.row_pt != nullptr ? p.row_pt[grp * p.per] : p.pt;
+      group_span(p, grp, span_lo, span_hi);
     }
     const int hkv = p.blocks == 1 ? sub : sub / p.blocks, c0 = p.blocks == 1 ? 0 : (sub % p.blocks) * kC;
     const int r0 = grp * p.per, nrows = min(p.per, p.rows - r0), columns = min(kC, nrows * p.G - c0);
@@ -289,22 +306,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       const int row = r0 + ((c0 + cp) * p.g_inv >> 16);
       pos_raw[i] = cp < columns ? (p.row_pos != nullptr ? __ldg(p.row_pos + row) : p.base_pos + row) : INT_MAX;
     }
-    GroupInfo info;
-    if (p.split && grp < kKept) {
-      info = s_kept[grp];
-    } else {
-      info.pt = p.row_pt != nullptr ? p.row_pt[r0] : p.pt;
-      group_span(p, grp, info.lo, info.hi);
-    }
-    const int span_lo = info.lo, span_hi = info.hi;
-    const int* const pt = info.pt;
     first_tile = span_hi < 0 ? 0 : span_lo / kTile;
     n_tiles = span_hi < 0 ? 0 : span_hi / kTile - first_tile + 1;
     if (!p.split) {
       piece_end = n_tiles;
     } else if (chunk > 0) {
       const int k = piece_begin, n = piece_end;
-      piece_begin = k * n_tiles / n, piece_end = (k + 1) * n_tiles / n;
+      piece_begin = quotient(k * n_tiles, n), piece_end = quotient((k + 1) * n_tiles, n);
       x = x_end;
     } else {
       piece_end = min(n_tiles, piece_begin + x_end - x);
@@ -362,22 +370,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       float f[kPer];
 #pragma unroll
       for (int e = 0; e < kPer; e += 2) f[e] = bf16_lo(q_raw[i][e >> 1]), f[e + 1] = bf16_hi(q_raw[i][e >> 1]);
-      float top = 0.0f;
+      unsigned top_bits = 0;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) top = fmaxf(top, fabsf(f[e]));
-      top = warp_max(top);
-      const bool sound = top > 0.0f && top < INFINITY;
-      const float to_int = sound ? 32639.0f / fmaxf(top, 1e-30f) : 0.0f;
-      int sum = 0;
+      for (int e = 0; e < kPer; ++e) top_bits = max(top_bits, __float_as_uint(f[e]) & 0x7fffffffu);
+      const float top = fmaxf(__uint_as_float(__reduce_max_sync(0xffffffffu, top_bits)), 1e-30f);
+      const float to_int = top < INFINITY ? 32639.0f / top : 0.0f;
       uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};  // even dims, odd dims
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
         const int v = __float2int_rn(f[e] * to_int), h = (v + 128) >> 8;
-        sum += v;
         hi[e & 1] |= static_cast<uint32_t>(h & 0xff) << (8 * (e >> 1)), lo[e & 1] |= static_cast<uint32_t>((v - 256 * h) & 0xff) << (8 * (e >> 1));
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       unsigned char* dst = s_q[2 * c] + (lane * kPer / 8) * 8 + lane * kPer % 8 / 2;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -388,12 +391,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
           dst[4 * u] = static_cast<unsigned char>(hi[u]), dst[4 * u + sizeof(s_q[0])] = static_cast<unsigned char>(lo[u]);
         }
       }
-      if (lane == 0) s_pair[c] = make_float2(sound ? p.scale_log2 * fmaxf(top, 1e-30f) / 32639.0f : 0.0f, __int_as_float(8 * sum));
+      if (lane == 0) s_scale[c] = top < INFINITY ? p.scale_log2 * top / 32639.0f : 0.0f;
     }
     __syncthreads();
     uint32_t qb[NS][kW][2];  // the lane's column g of tile i: pair 4 i + g / 2, hi (g even) or lo
     float l_scale[NS];       // of the lane's accumulator pairs 4 i + t
-    int l_off[NS], pos_col[NS], lo_col[NS];
+    int l_off[NS], pos_col[NS];
     int all_lo = 0, all_hi = INT_MAX;  // positions that every column sees
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
@@ -403,11 +406,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
         qb[i][w][0] = v.x, qb[i][w][1] = v.y, qb[i][w + 1][0] = v.z, qb[i][w + 1][1] = v.w;
       }
       const int c = 4 * i + t;
-      l_scale[i] = s_pair[c].x, l_off[i] = __float_as_int(s_pair[c].y);
+      l_scale[i] = s_scale[c];
+      int sums[4] = {0, 0, 0, 0};  // a K of codes 0 (u = 8) gives what the 8 of every u adds
+#pragma unroll
+      for (int w = 0; w < kW; ++w) mma_u8s8(sums, 0x08080808u, 0x08080808u, 0x08080808u, 0x08080808u, qb[i][w][0], qb[i][w][1]);
+      l_off[i] = sums[0] * 256 + sums[1];
       // a column that is not there sees everything and is dropped
       pos_col[i] = pos_raw[i] < 0 ? -1 : c < columns ? min(pos_raw[i], p.max_len - 1) : INT_MAX;
-      lo_col[i] = c < columns && p.window > 0 ? max(0, pos_col[i] + 1 - p.window) : 0;
-      all_hi = min(all_hi, pos_col[i]), all_lo = max(all_lo, lo_col[i]);
+      all_hi = min(all_hi, pos_col[i]);
+      if (c < columns && p.window > 0) all_lo = max(all_lo, pos_col[i] + 1 - p.window);
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
@@ -416,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     }
 
     float o[kNP][kM][4], osum[kNP][4], m_run[NS], l_run[NS];  // l_run times v_mult
-    float m_pass[NS], e_base[NS];  // m_run + 4; what is taken off a logit: m_run - log2(v_mult)
+    float e_base[NS];  // what is taken off a logit: m_run - log2(v_mult)
 #pragma unroll
     for (int n = 0; n < kNP; ++n) {
 #pragma unroll
@@ -424,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       osum[n][0] = osum[n][1] = osum[n][2] = osum[n][3] = 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < NS; ++i) m_run[i] = m_pass[i] = -INFINITY, e_base[i] = l_run[i] = 0.0f;
+    for (int i = 0; i < NS; ++i) m_run[i] = -INFINITY, e_base[i] = l_run[i] = 0.0f;
     float v_mult = 1.0f, v_cap = -1.0f;  // power of two on v_scale, and the largest v_scale it is good for
 
     for (int stage = 0; tile < tile_end; tile += kWarps, stage = stage == kStages - 1 ? 0 : stage + 1) {
@@ -483,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int pos = t0 + g + 8 * u;
-            if (pos > pos_col[i] || pos < lo_col[i]) l[i][u] = -INFINITY;
+            if (pos > pos_col[i] || (p.window > 0 && pos_col[i] != INT_MAX && pos <= pos_col[i] - p.window)) l[i][u] = -INFINITY;
           }
       }
       const float v_top = fmaxf(fmaxf(fv[0], fv[1]), fmaxf(fv[2], fv[3]));
@@ -491,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         l_top[i] = fmaxf(fmaxf(l[i][0], l[i][1]), fmaxf(l[i][2], l[i][3]));
-        moves |= l_top[i] > m_pass[i];
+        moves |= l_top[i] > m_run[i] + 4.0f;
       }
       if (__any_sync(0xffffffffu, moves)) {
         float f = 1.0f;
@@ -518,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
           const float m_new = fmaxf(m_run[i], top);
           corr[i] = m_new == -INFINITY ? 1.0f : exp2_fast(m_run[i] - m_new) * f;
-          l_run[i] *= corr[i], m_run[i] = m_new, m_pass[i] = m_new + 4.0f;
+          l_run[i] *= corr[i], m_run[i] = m_new;
           e_base[i] = (m_new == -INFINITY ? 0.0f : m_new) - log_mult;
         }
 #pragma unroll
@@ -526,10 +533,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 #pragma unroll
           for (int m = 0; m < kM; ++m) {
             o[n][m][0] *= corr[2 * n], o[n][m][2] *= corr[2 * n];
-            if (kE == 2) o[n][m][1] *= corr[2 * n + 1], o[n][m][3] *= corr[2 * n + 1];
+            if (2 * n + 1 < NS) o[n][m][1] *= corr[2 * n + 1], o[n][m][3] *= corr[2 * n + 1];
           }
           osum[n][0] *= corr[2 * n];
-          if (kE == 2) osum[n][1] *= corr[2 * n + 1];
+          if (2 * n + 1 < NS) osum[n][1] *= corr[2 * n + 1];
         }
       }
       uint32_t pb[kNP][2][2];
@@ -537,15 +544,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       for (int n = 0; n < kNP; ++n) {
         float pv[2][4];
 #pragma unroll
-        for (int e = 0; e < kE; ++e) {
+        for (int e = 0; e < 2; ++e) {
           const int i = 2 * n + e;
+          if (i >= NS) break;
           float pr[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) pr[u] = exp2_fast(l[i][u] - e_base[i]), pv[e][u] = pr[u] * fv[u];
           l_run[i] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) pb[n][u >> 1][u & 1] = transpose8x8(halves(pv[0][u], kE == 2 ? pv[1][u] : 0.0f));
+        for (int u = 0; u < 4; ++u) pb[n][u >> 1][u & 1] = transpose8x8(halves(pv[0][u], 2 * n + 1 < NS ? pv[1][u] : 0.0f));
       }
       // O^T += V^T P^T
 #pragma unroll
@@ -631,6 +639,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 // alone.
 template <int D, int NS>
 __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4AttnParams p, int ctas) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   pdl_begin();
   constexpr int kC = 4 * NS, kPer = D / 32, kFly = 8;
   __shared__ float s_w[kMaxShares];
@@ -723,7 +732,7 @@ struct Int4Plan {
 Int4Plan plan_int4(int rows, int per, int Hq, int Hk, int d, int max_len) {
   Int4Plan s{};
   const int columns = per * (Hq / Hk);
-  s.ns = columns <= 4 ? 1 : columns <= 8 ? 2 : 4;
+  s.ns = columns <= 4 ? 1 : columns <= 8 ? 2 : columns <= 12 ? 3 : 4;
   s.blocks = (columns + 4 * s.ns - 1) / (4 * s.ns);
   s.groups = (rows + per - 1) / per;
   s.segments = static_cast<long long>(s.groups) * Hk * s.blocks;
@@ -731,7 +740,9 @@ Int4Plan plan_int4(int rows, int per, int Hq, int Hk, int d, int max_len) {
   const long long tiles = s.segments * ((max_len + kTile - 1) / kTile);
   // short caches: a segment is one tile per warp. Many segments: the CTAs balance one another, and each saves its
   // neighbours the joining of a piece.
-  if (max_len <= kTile * kWarps || s.groups > kMaxGroups || s.segments >= 4 * resident || tiles > INT_MAX / 2) return s;
+  if (max_len <= kTile * kWarps || s.groups > kMaxGroups || s.segments >= 4 * resident ||
+      tiles > INT_MAX / 2 || tiles / (static_cast<long long>(Hk) * s.blocks) >= kMaxQuotient || tiles / resident >= kMaxQuotient)
+    return s;
   s.shares = static_cast<int>(std::min(resident, std::max(1ll, tiles / kWarps)));
   const long long slots = s.shares + s.segments;
   s.bytes = slots * 4 * s.ns * (d + 2) * 4 + (s.groups + 2 + 3) / 4 * 16;
@@ -783,9 +794,16 @@ int attn_int4(const char* fn, Int4AttnParams p, int d, void* scratch, long long 
     p.part_ml = p.part_o + slots * 4 * s.ns * d;
     p.prefix = reinterpret_cast<int*>(p.part_ml + slots * 4 * s.ns * 2);
   }
-  if (d == 128)
-    return s.ns == 1 ? launch_int4<128, 1>(fn, p, s) : s.ns == 2 ? launch_int4<128, 2>(fn, p, s) : launch_int4<128, 4>(fn, p, s);
-  return s.ns == 1 ? launch_int4<64, 1>(fn, p, s) : s.ns == 2 ? launch_int4<64, 2>(fn, p, s) : launch_int4<64, 4>(fn, p, s);
+  switch (s.ns + (d == 128 ? 4 : 0)) {
+    case 1: return launch_int4<64, 1>(fn, p, s);
+    case 2: return launch_int4<64, 2>(fn, p, s);
+    case 3: return launch_int4<64, 3>(fn, p, s);
+    case 4: return launch_int4<64, 4>(fn, p, s);
+    case 5: return launch_int4<128, 1>(fn, p, s);
+    case 6: return launch_int4<128, 2>(fn, p, s);
+    case 7: return launch_int4<128, 3>(fn, p, s);
+    default: return launch_int4<128, 4>(fn, p, s);
+  }
 }
 
 // Chunks from this many rows on go through the tensor-core prefill kernels, which read an 8-bit pool.
