@@ -175,11 +175,8 @@ __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
 __device__ __forceinline__ void copy4_async(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+// All of this thread's copies have landed.
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // A warp's ring of raw tiles: 32 K rows, 32 V rows, their scales, as they are in the pool (for positions that no
 // row sees, the nearest that one sees). The 16-byte pieces of a row lie exchanged, so that neither the copies (two lanes a row),
@@ -188,7 +185,7 @@ template <int D>
 __device__ __forceinline__ int piece_at(int row, int piece) {
   return D == 128 ? piece ^ ((row >> 1) & 3) : piece ^ ((row >> 2) & 1);
 }
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 template <int D>
 constexpr int kRowBytes = D / 2;
 template <int D>
@@ -351,14 +348,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     const int tile_end = first_tile + piece_end;
     int tile = first_tile + piece_begin + warp;
     int row_next = 0;
-    {
-      const int row0 = tile < tile_end ? table_row(tile) : 0;
-      const int row1 = tile + kWarps < tile_end ? table_row(tile + kWarps) : 0;
-      if (tile + 2 * kWarps < tile_end) row_next = table_row(tile + 2 * kWarps);
-      if (tile < tile_end) fetch(0, row0);
-      copies_commit();
-      if (tile + kWarps < tile_end) fetch(1, row1);
-      copies_commit();
+    if (tile < tile_end) {
+      const int row = table_row(tile);
+      if (tile + kWarps < tile_end) row_next = table_row(tile + kWarps);
+      fetch(0, row);
     }
 
     // q's digits into shared memory: a warp per pair, D / 32 dims a lane. Bytes follow the nibbles of K's words: of
@@ -434,12 +427,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     for (int i = 0; i < NS; ++i) m_run[i] = -INFINITY, e_base[i] = l_run[i] = 0.0f;
     float v_mult = 1.0f, v_cap = -1.0f;  // power of two on v_scale, and the largest v_scale it is good for
 
-    for (int stage = 0; tile < tile_end; tile += kWarps, stage = stage == kStages - 1 ? 0 : stage + 1) {
-      copies_wait<kStages - 2>();
+    for (int stage = 0; tile < tile_end; tile += kWarps, stage ^= 1) {
+      copies_wait();
       __syncwarp();
-      if (tile + 2 * kWarps < tile_end) fetch(stage == 0 ? 2 : stage - 1, row_next);
-      copies_commit();
-      if (tile + 3 * kWarps < tile_end) row_next = table_row(tile + 3 * kWarps);
+      if (tile + kWarps < tile_end) fetch(stage ^ 1, row_next);
+      if (tile + 2 * kWarps < tile_end) row_next = table_row(tile + 2 * kWarps);
       const unsigned char* const raw = ring + stage * kStageBytes<D>;
       const float* const raw_ks = reinterpret_cast<const float*>(raw + kSAt);
       const float* const raw_vs = raw_ks + kTile;
@@ -584,7 +576,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 
     // the four warps' states meet in shared memory, each parked in the warp's own ring
     if (p.split) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    copies_wait<0>();
     __syncwarp();
     float* const park = reinterpret_cast<float*>(ring);  // [kC][D + kPad], then [kC][2] (max, sum)
     const float back = 16777216.0f / v_mult;
@@ -639,7 +630,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 // alone.
 template <int D, int NS>
 __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4AttnParams p, int ctas) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   pdl_begin();
   constexpr int kC = 4 * NS, kPer = D / 32, kFly = 8;
   __shared__ float s_w[kMaxShares];

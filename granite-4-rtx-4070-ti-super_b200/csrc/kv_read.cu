@@ -38,30 +38,56 @@ struct ReadParams {
   long long stride, n;
 };
 
-// A thread reads eight codes and writes 16 bytes; consecutive threads follow the output.
-template <int D, int BITS>
+// A thread reads eight codes of K and V and writes 16 bytes of each, N times; consecutive threads follow the output.
+// The N rows' indices, then their codes and scales, are all on their way before the first is used.
+template <int D, int BITS, int N>
 __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const ReadParams p) {
   pdl_begin();
   constexpr int kParts = D / 8;
-  const long long items = p.n * p.Hk * kParts;
-  const long long i = static_cast<long long>(blockIdx.x) * kReadThreads + threadIdx.x;
-  if (i >= items) return;
-  const int part = static_cast<int>(i % kParts);
-  const long long rh = i / kParts;
-  const int h = static_cast<int>(rh % p.Hk);
-  const int row = __ldg(p.kv_rows + rh / p.Hk);
-  const bool have = row >= 0 && row < p.stride;
-  const size_t srow = static_cast<size_t>(h) * p.stride + (have ? row : 0);
+  const long long items = p.n * p.Hk * kParts, first = static_cast<long long>(blockIdx.x) * (kReadThreads * N) + threadIdx.x;
+  int row[N];
+  size_t srow[N];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    const uint8_t* cache = (kv ? p.cv : p.ck) + srow * (D * BITS / 8);
-    const float s = have ? __ldg((kv ? p.vs : p.ks) + srow) : 0.0f;
-    uint2 w = make_uint2(0u, 0u);
-    if (have) w = BITS == 4 ? nibbles_to_bytes(__ldg(reinterpret_cast<const uint32_t*>(cache) + part)) : __ldg(reinterpret_cast<const uint2*>(cache) + part);
-    float v[8];
+  for (int u = 0; u < N; ++u) {
+    const long long i = first + u * kReadThreads;
+    row[u] = -1;
+    if (i < items) {
+      // (row, head) pairs of a call fit 32 bits: checked by the launcher
+      const unsigned rh = static_cast<unsigned>(i / kParts), r = rh / static_cast<unsigned>(p.Hk);
+      row[u] = __ldg(p.kv_rows + r);
+      srow[u] = static_cast<size_t>(rh - r * static_cast<unsigned>(p.Hk)) * p.stride;
+    }
+  }
+  uint2 w[N][2];
+  float s[N][2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = byte_value(e < 4 ? w.x : w.y, e & 3) * s;
-    st_stream(reinterpret_cast<uint4*>(kv ? p.v_out : p.k_out) + i, pack8(v));
+  for (int u = 0; u < N; ++u) {
+    const int part = static_cast<int>((first + u * kReadThreads) % kParts);
+    const bool have = row[u] >= 0 && row[u] < p.stride;
+    if (have) srow[u] += row[u];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      w[u][kv] = make_uint2(0u, 0u), s[u][kv] = 0.0f;
+      if (have) {
+        const uint8_t* cache = (kv ? p.cv : p.ck) + srow[u] * (D * BITS / 8);
+        if (BITS == 4) w[u][kv].x = __ldg(reinterpret_cast<const uint32_t*>(cache) + part);
+        else w[u][kv] = __ldg(reinterpret_cast<const uint2*>(cache) + part);
+        s[u][kv] = __ldg((kv ? p.vs : p.ks) + srow[u]);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const long long i = first + u * kReadThreads;
+    if (i >= items) break;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const uint2 b = BITS == 4 ? nibbles_to_bytes(w[u][kv].x) : w[u][kv];
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = byte_value(e < 4 ? b.x : b.y, e & 3) * s[u][kv];
+      st_stream(reinterpret_cast<uint4*>(kv ? p.v_out : p.k_out) + i, pack8(v));
+    }
   }
 }
 
@@ -102,9 +128,13 @@ __global__ void __launch_bounds__(kReadThreads) kv_widen_kernel(const WidenParam
 
 template <int D, int BITS>
 int launch_read(const char* fn, const ReadParams& p) {
-  const long long blocks = (p.n * p.Hk * (D / 8) + kReadThreads - 1) / kReadThreads;
-  if (blocks > INT_MAX) return fail(fn, "too many rows");
-  G4_LAUNCH_PDL(fn, (kv_read_kernel<D, BITS>), dim3(static_cast<unsigned>(blocks)), dim3(kReadThreads), 0, current_stream(), p);
+  if (p.n * p.Hk > INT_MAX) return fail(fn, "too many rows");
+  const long long items = p.n * p.Hk * (D / 8);
+  // one item a thread while that does not fill the card twice over: latency is what counts
+  const bool few = items <= 2ll * 2048 * sm_count();
+  const long long per = kReadThreads * (few ? 1 : 4), blocks = (items + per - 1) / per;
+  if (few) G4_LAUNCH_PDL(fn, (kv_read_kernel<D, BITS, 1>), dim3(static_cast<unsigned>(blocks)), dim3(kReadThreads), 0, current_stream(), p);
+  else G4_LAUNCH_PDL(fn, (kv_read_kernel<D, BITS, 4>), dim3(static_cast<unsigned>(blocks)), dim3(kReadThreads), 0, current_stream(), p);
   return 0;
 }
 

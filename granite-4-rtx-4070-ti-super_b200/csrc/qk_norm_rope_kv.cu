@@ -12,10 +12,16 @@
 // The one rounding of a code is its own: K is normed and rotated in double from its bf16 values and the f32
 // tables, so that a code does not depend on the order in which a kernel rounds its way there. What is left
 // of a double between the value and the border of two codes is 1e-15 of the scale.
+// Doubles are short: 80 of them a key element's lane and head, no division. The code itself is found in f32 (value
+// times the scale's reciprocal, off by 2^-22 of it at most) wherever that is further from a border than 2^-14;
+// where it is not, the sign of fma(-(code +- 1/2), scale, |x|) decides, which an fma gives exactly.
+//
 #include "g4_host.h"
 #include "g4_math.cuh"
 
 #include "../../include/granite4_b200.h"
+
+#include <algorithm>
 
 namespace g4 {
 namespace {
@@ -39,130 +45,229 @@ struct QkNormParams {
 };
 
 constexpr int kQkThreads = 128;
+constexpr float kNearBorder = 0.5f - 1.0f / 16384.0f;
 
-// sign * floor(|x| / s + 1/2) of a value whose quotient by the scale is at most top (but for a rounding)
-template <int TOP>
-__device__ __forceinline__ int code_of(double x, double s) {
-  const double t = floor(fabs(x) / s + 0.5);
-  const int m = static_cast<int>(fmin(t, static_cast<double>(TOP)));
-  return x < 0.0 ? -m : m;
+// |x| against the borders of code c: the code itself.
+__device__ __forceinline__ float settle(float c, float x, float s) {
+  if (fmaf(-(c + 0.5f), s, x) >= 0.0f) return c + 1.0f;
+  return c > 0.0f && fmaf(-(c - 0.5f), s, x) < 0.0f ? c - 1.0f : c;
+}
+__device__ __forceinline__ float settle(float c, double x, float s) {
+  if (fma(-static_cast<double>(c + 0.5f), static_cast<double>(s), x) >= 0.0) return c + 1.0f;
+  return c > 0.0f && fma(-static_cast<double>(c - 0.5f), static_cast<double>(s), x) < 0.0 ? c - 1.0f : c;
+}
+
+// Codes of a lane's values x (xf: the same in f32) under scale s, as the words of the pool: 4 bits, code + 8, or 8.
+template <int BITS, typename T>
+__device__ __forceinline__ uint2 encode8(const T (&x)[8], const float (&xf)[8], float s, bool plain, float inv) {
+  // adding 1.5 2^23 (and the 8) leaves the integer in the low bits of the sum
+  constexpr float kMagic = 12582912.0f + (BITS == 4 ? 8.0f : 0.0f);
+  float z[8], far = plain ? 0.0f : 1.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = xf[e] * inv;
+    z[e] = t + kMagic;
+    far = fmaxf(far, fabsf(t - (z[e] - kMagic)));
+  }
+  if (!(far < kNearBorder)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const T ax = x[e] < T(0) ? -x[e] : x[e];
+      float c = 0.0f;
+      if (s > 0.0f) {
+        if (plain) {
+          c = settle(fabsf(z[e] - kMagic), ax, s);
+        } else {  // a scale whose reciprocal, or the fma's difference, may lie outside of f32
+          c = fminf(rintf(static_cast<float>(static_cast<double>(ax) / static_cast<double>(s))), BITS == 4 ? 7.0f : 127.0f);
+          c = settle(c, static_cast<double>(ax), s);
+        }
+      }
+      z[e] = (x[e] < T(0) ? -c : c) + kMagic;
+    }
+  }
+  // sum of (z - magic's bits) 2^(BITS e): the magic's bits are taken out of the sum
+  uint2 w = make_uint2(0u, 0u);
+  if (BITS == 4) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w.x += __float_as_uint(z[e]) << (4 * e);
+    w.x -= 0x4b400000u * 0x11111111u;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w.x |= (__float_as_uint(z[e]) & 0xffu) << (8 * e);
+      w.y |= (__float_as_uint(z[4 + e]) & 0xffu) << (8 * e);
+    }
+  }
+  return w;
 }
 
 // d / 16 lanes own a head: lane j has columns [8j, 8j + 8) of both halves, i.e. both sides of its eight
-// rotation pairs, so the rotation needs no exchange and the head's sums are log2(d / 16) shuffles.
-template <int D, int BITS>
-__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kv_kernel(const QkNormParams p) {
+// rotation pairs, so the rotation needs no exchange and the head's sums are log2(d / 16) shuffles. A CTA takes
+// 128 / (d / 16) heads of a row at once, KH times (48 heads of 128: three times, a whole row), and goes on to its next
+// row with that row's values and index already on their way: what bounds the kernel is memory, 22 KB a row in and out.
+template <int D, int BITS, int KH>
+__global__ void __launch_bounds__(kQkThreads, KH == 1 ? 4 : 4) qk_norm_rope_kv_kernel(const QkNormParams p, int parts, int items) {
   pdl_begin();
   constexpr int kLanes = D / 16, kHeads = kQkThreads / kLanes, kTop = BITS == 4 ? 7 : 127;
-  const int g = threadIdx.x / kLanes + blockIdx.y * kHeads, step = gridDim.y * kHeads, j = threadIdx.x % kLanes;
+  const int g = threadIdx.x / kLanes, j = threadIdx.x % kLanes;
   const unsigned mask = ((1u << kLanes) - 1u) << (threadIdx.x & 31 & ~(kLanes - 1));
-  const int heads = p.Hq + 2 * p.Hk, r = blockIdx.x;
-  const int pos = __ldg(p.pos_rows + r), kv_row = __ldg(p.kv_rows + r);
-  // a bad index skips the row instead of touching memory outside the tables or the pool
-  if (pos < 0 || pos >= p.max_pos || kv_row < 0 || kv_row >= p.stride) return;
-  float c[8], s[8];
+  const int heads = p.Hq + 2 * p.Hk;
+  struct Raw {
+    uint4 lo[KH], hi[KH];
+    int r, first, pos, kv_row;
+  };
+  auto load = [&](Raw& w, int item) {
+    w.r = parts == 1 ? item : item / parts;
+    w.first = parts == 1 ? g : (item - w.r * parts) * (kHeads * KH) + g;
+    w.pos = __ldg(p.pos_rows + w.r), w.kv_row = __ldg(p.kv_rows + w.r);
 #pragma unroll
-  for (int e = 0; e < 8; e += 4) {
-    const float4 cv = __ldg(reinterpret_cast<const float4*>(p.cos_tbl + static_cast<size_t>(pos) * (D / 2) + 8 * j + e));
-    const float4 sv = __ldg(reinterpret_cast<const float4*>(p.sin_tbl + static_cast<size_t>(pos) * (D / 2) + 8 * j + e));
-    c[e] = cv.x, c[e + 1] = cv.y, c[e + 2] = cv.z, c[e + 3] = cv.w;
-    s[e] = sv.x, s[e + 1] = sv.y, s[e + 2] = sv.z, s[e + 3] = sv.w;
-  }
-  for (int head = g; head < heads; head += step) {
-    const uint4* src = reinterpret_cast<const uint4*>(p.qkv + (static_cast<size_t>(r) * heads + head) * D);
-    float lo[8], hi[8], wl[8], wh[8];
-    unpack8(ld_stream(src + j), lo);
-    unpack8(ld_stream(src + kLanes + j), hi);
-    const bool is_q = head < p.Hq, is_k = !is_q && head < p.Hq + p.Hk;
-    const uint16_t* w = is_q ? p.wq : p.wk;
-    if (w != nullptr) {
-      unpack8(__ldg(reinterpret_cast<const uint4*>(w) + j), wl);
-      unpack8(__ldg(reinterpret_cast<const uint4*>(w) + kLanes + j), wh);
-    }
-    if (is_q) {
-      if (w != nullptr) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += lo[e] * lo[e] + hi[e] * hi[e];
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float rn = 1.0f / sqrtf(ss / D + p.eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) lo[e] *= rn * wl[e], hi[e] *= rn * wh[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = lo[e], b = hi[e];
-        lo[e] = a * c[e] - b * s[e], hi[e] = b * c[e] + a * s[e];
-      }
-      uint4* dst = reinterpret_cast<uint4*>(p.q_rot + (static_cast<size_t>(r) * p.Hq + head) * D);
-      st_stream(dst + j, pack8(lo));
-      st_stream(dst + kLanes + j, pack8(hi));
-      continue;
-    }
-    double dl[8], dh[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) dl[e] = lo[e], dh[e] = hi[e];
-    if (is_k) {
-      if (w != nullptr) {
-        double ss = 0.0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += dl[e] * dl[e] + dh[e] * dh[e];
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const double rn = 1.0 / sqrt(ss / D + static_cast<double>(p.eps));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dl[e] = dl[e] * rn * wl[e], dh[e] = dh[e] * rn * wh[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double a = dl[e], b = dh[e];
-        dl[e] = a * c[e] - b * s[e], dh[e] = b * c[e] + a * s[e];
+    for (int k = 0; k < KH; ++k) {
+      const int head = w.first + k * kHeads;
+      if (head < heads) {
+        const uint4* src = reinterpret_cast<const uint4*>(p.qkv + (static_cast<size_t>(w.r) * heads + head) * D);
+        w.lo[k] = ld_stream(src + j), w.hi[k] = ld_stream(src + kLanes + j);
       }
     }
-    double amax = 0.0;
+  };
+  auto work = [&](const Raw& w) {
+    const int pos = w.pos, kv_row = w.kv_row;
+    // a bad index skips the row instead of touching memory outside the tables or the pool
+    if (pos < 0 || pos >= p.max_pos || kv_row < 0 || kv_row >= p.stride) return;
+    float c[8], s[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = fmax(amax, fmax(fabs(dl[e]), fabs(dh[e])));
-#pragma unroll
-    for (int o = 1; o < kLanes; o <<= 1) amax = fmax(amax, __shfl_xor_sync(mask, amax, o));
-    const float sc = static_cast<float>(amax / kTop);
-    const int hkv = is_k ? head - p.Hq : head - p.Hq - p.Hk;
-    const size_t srow = static_cast<size_t>(hkv) * p.stride + kv_row;
-    if (j == 0) (is_k ? p.k_scale : p.v_scale)[srow] = sc;
-    uint8_t* cache = (is_k ? p.cache_k : p.cache_v) + srow * (D * BITS / 8);
-    int cl[8], ch[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      cl[e] = sc > 0.0f ? code_of<kTop>(dl[e], sc) : 0;
-      ch[e] = sc > 0.0f ? code_of<kTop>(dh[e], sc) : 0;
+    for (int e = 0; e < 8; e += 4) {
+      const float4 cv = __ldg(reinterpret_cast<const float4*>(p.cos_tbl + static_cast<size_t>(pos) * (D / 2) + 8 * j + e));
+      const float4 sv = __ldg(reinterpret_cast<const float4*>(p.sin_tbl + static_cast<size_t>(pos) * (D / 2) + 8 * j + e));
+      c[e] = cv.x, c[e + 1] = cv.y, c[e + 2] = cv.z, c[e + 3] = cv.w;
+      s[e] = sv.x, s[e + 1] = sv.y, s[e + 2] = sv.z, s[e + 3] = sv.w;
     }
-    if (BITS == 4) {
-      uint32_t a = 0, b = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a |= static_cast<uint32_t>(cl[e] + 8) << (4 * e), b |= static_cast<uint32_t>(ch[e] + 8) << (4 * e);
-      reinterpret_cast<uint32_t*>(cache)[j] = a;
-      reinterpret_cast<uint32_t*>(cache)[kLanes + j] = b;
-    } else {
-      uint32_t a[2] = {0, 0}, b[2] = {0, 0};
+    for (int k = 0; k < KH; ++k) {
+      const int head = w.first + k * kHeads;
+      if (head >= heads) break;
+      float lo[8], hi[8];
+      unpack8(w.lo[k], lo);
+      unpack8(w.hi[k], hi);
+      const bool is_q = head < p.Hq, is_k = !is_q && head < p.Hq + p.Hk;
+      const uint16_t* wt = is_q ? p.wq : p.wk;
+      if (is_q) {
+        if (wt != nullptr) {
+          float wl[8], wh[8];
+          unpack8(__ldg(reinterpret_cast<const uint4*>(wt) + j), wl);
+          unpack8(__ldg(reinterpret_cast<const uint4*>(wt) + kLanes + j), wh);
+          float ss = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        a[e >> 2] |= static_cast<uint32_t>(cl[e] & 0xff) << (8 * (e & 3));
-        b[e >> 2] |= static_cast<uint32_t>(ch[e] & 0xff) << (8 * (e & 3));
+          for (int e = 0; e < 8; ++e) ss += lo[e] * lo[e] + hi[e] * hi[e];
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+          const float rn = 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) lo[e] *= rn * wl[e], hi[e] *= rn * wh[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float a = lo[e], b = hi[e];
+          lo[e] = a * c[e] - b * s[e], hi[e] = b * c[e] + a * s[e];
+        }
+        uint4* dst = reinterpret_cast<uint4*>(p.q_rot + (static_cast<size_t>(w.r) * p.Hq + head) * D);
+        st_stream(dst + j, pack8(lo));
+        st_stream(dst + kLanes + j, pack8(hi));
+        continue;
       }
-      reinterpret_cast<uint2*>(cache)[j] = make_uint2(a[0], a[1]);
-      reinterpret_cast<uint2*>(cache)[kLanes + j] = make_uint2(b[0], b[1]);
+      const int hkv = is_k ? head - p.Hq : head - p.Hq - p.Hk;
+      const size_t srow = static_cast<size_t>(hkv) * p.stride + kv_row;
+      float sc;
+      uint2 cl, ch;
+      if (is_k) {
+        double dl[8], dh[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dl[e] = lo[e], dh[e] = hi[e];
+        if (wt != nullptr) {
+          double ss = 0.0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss += dl[e] * dl[e] + dh[e] * dh[e];
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+          const double rn = 1.0 / sqrt(ss * (1.0 / D) + static_cast<double>(p.eps));
+          float wl[8], wh[8];
+          unpack8(__ldg(reinterpret_cast<const uint4*>(wt) + j), wl);
+          unpack8(__ldg(reinterpret_cast<const uint4*>(wt) + kLanes + j), wh);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dl[e] *= rn * wl[e], dh[e] *= rn * wh[e];
+        }
+        double amax = 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const double a = dl[e], b = dh[e];
+          dl[e] = a * c[e] - b * s[e], dh[e] = b * c[e] + a * s[e];
+          const double x = fabs(dl[e]), y = fabs(dh[e]);
+          amax = x > amax ? x : amax;
+          amax = y > amax ? y : amax;
+          lo[e] = static_cast<float>(dl[e]), hi[e] = static_cast<float>(dh[e]);
+        }
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) {
+          const double x = __shfl_xor_sync(mask, amax, o);
+          amax = x > amax ? x : amax;
+        }
+        sc = static_cast<float>(amax / kTop);
+        const bool plain = sc > 1e-30f;
+        const float inv = plain ? 1.0f / sc : 0.0f;
+        cl = encode8<BITS>(dl, lo, sc, plain, inv), ch = encode8<BITS>(dh, hi, sc, plain, inv);
+      } else {
+        float amax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
+        sc = __fdiv_rn(amax, static_cast<float>(kTop));  // eight significant bits over 7 or 127: never half way between floats
+        const bool plain = sc > 1e-30f;
+        const float inv = plain ? 1.0f / sc : 0.0f;
+        cl = encode8<BITS>(lo, lo, sc, plain, inv), ch = encode8<BITS>(hi, hi, sc, plain, inv);
+      }
+      if (j == 0) (is_k ? p.k_scale : p.v_scale)[srow] = sc;
+      uint8_t* cache = (is_k ? p.cache_k : p.cache_v) + srow * (D * BITS / 8);
+      if (BITS == 4) {
+        reinterpret_cast<uint32_t*>(cache)[j] = cl.x;
+        reinterpret_cast<uint32_t*>(cache)[kLanes + j] = ch.x;
+      } else {
+        reinterpret_cast<uint2*>(cache)[j] = cl;
+        reinterpret_cast<uint2*>(cache)[kLanes + j] = ch;
+      }
+    }
+  };
+  Raw w[2];
+  int item = blockIdx.x;
+  load(w[0], item);
+  while (true) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int next = item + gridDim.x;
+      if (next < items) load(w[i ^ 1], next);
+      work(w[i]);
+      if (next >= items) return;
+      item = next;
     }
   }
 }
 
+template <int D, int BITS, int KH>
+int launch_qk_norm(const char* fn, const QkNormParams& p) {
+  constexpr int heads_per_cta = kQkThreads / (D / 16) * KH;
+  const int heads = p.Hq + 2 * p.Hk, parts = (heads + heads_per_cta - 1) / heads_per_cta;
+  const long long items = static_cast<long long>(p.rows) * parts;
+  if (items > INT_MAX / 2) return fail(fn, "too many rows");
+  const long long grid = std::min(items, 4ll * sm_count());
+  G4_LAUNCH_PDL(fn, (qk_norm_rope_kv_kernel<D, BITS, KH>), dim3(static_cast<unsigned>(grid)), dim3(kQkThreads), 0, current_stream(), p,
+                parts, static_cast<int>(items));
+  return 0;
+}
+
+// Few rows: a head a lane group, over as many CTAs as that takes.
 template <int D, int BITS>
 int launch_qk_norm(const char* fn, const QkNormParams& p) {
-  constexpr int heads_per_cta = kQkThreads / (D / 16);
-  const int heads = p.Hq + 2 * p.Hk;
-  const unsigned parts = p.rows <= 16 ? static_cast<unsigned>((heads + heads_per_cta - 1) / heads_per_cta) : 1u;
-  G4_LAUNCH_PDL(fn, (qk_norm_rope_kv_kernel<D, BITS>), dim3(static_cast<unsigned>(p.rows), parts), dim3(kQkThreads), 0,
-                current_stream(), p);
-  return 0;
+  const long long ctas = static_cast<long long>(p.rows) * ((p.Hq + 2 * p.Hk + kQkThreads / (D / 16) - 1) / (kQkThreads / (D / 16)));
+  return ctas <= 4ll * sm_count() ? launch_qk_norm<D, BITS, 1>(fn, p) : launch_qk_norm<D, BITS, 3>(fn, p);
 }
 
 }  // namespace
