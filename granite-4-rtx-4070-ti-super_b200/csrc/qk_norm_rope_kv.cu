@@ -12,7 +12,7 @@
 // The one rounding of a code is its own: K is normed and rotated in double from its bf16 values and the f32
 // tables, so that a code does not depend on the order in which a kernel rounds its way there. What is left
 // of a double between the value and the border of two codes is 1e-15 of the scale.
-// Doubles are short: 80 of them a key element's lane and head, no division. The code itself is found in f32 (value
+// The code itself is found in f32 (value
 // times the scale's reciprocal, off by 2^-22 of it at most) wherever that is further from a border than 2^-14;
 // where it is not, the sign of fma(-(code +- 1/2), scale, |x|) decides, which an fma gives exactly.
 //
@@ -65,28 +65,33 @@ __device__ __noinline__ float code_by_division(double x, float s, float top) {
   return x < 0.0 ? -c : c;
 }
 
-// Codes of a lane's values x (xf: the same in f32) under scale s, as the words of the pool: 4 bits, code + 8, or 8.
+// Codes of a lane's values r x (xf: x in f32; inv: r / s) under scale s, as the words of the pool: 4 bits, code + 8, or 8.
 template <int BITS, typename T>
-__device__ __forceinline__ uint2 encode8(const T (&x)[8], const float (&xf)[8], float s, bool plain, float inv) {
+__device__ __forceinline__ uint2 encode8(const T (&x)[8], const float (&xf)[8], float s, T r, bool plain, float inv) {
   // adding 1.5 2^23 (and the 8) leaves the integer in the low bits of the sum
   constexpr float kMagic = 12582912.0f + (BITS == 4 ? 8.0f : 0.0f);
+  const F32x2 inv2 = f32x2(inv, inv), magic2 = f32x2(kMagic, kMagic), one2 = f32x2(1.0f, 1.0f), minus2 = f32x2(-1.0f, -1.0f);
+  const F32x2 less2 = f32x2(-kMagic, -kMagic);
   float z[8], far = plain ? 0.0f : 1.0f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float t = xf[e] * inv;
-    z[e] = t + kMagic;
-    far = fmaxf(far, fabsf(t - (z[e] - kMagic)));
+  for (int e = 0; e < 8; e += 2) {
+    const F32x2 t = mul2(f32x2(xf[e], xf[e + 1]), inv2), zz = fma2(t, one2, magic2);
+    const F32x2 off = fma2(fma2(zz, one2, less2), minus2, t);  // t - code
+    float u, v;
+    f32x2_split(off, u, v);
+    f32x2_split(zz, z[e], z[e + 1]);
+    far = fmaxf(far, fmaxf(fabsf(u), fabsf(v)));
   }
   if (!(far < kNearBorder)) {
     if (plain) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float code = settle(fabsf(z[e] - kMagic), x[e] < T(0) ? -x[e] : x[e], s);
+        const float code = settle(fabsf(z[e] - kMagic), (x[e] < T(0) ? -x[e] : x[e]) * r, s);
         z[e] = (x[e] < T(0) ? -code : code) + kMagic;
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = code_by_division(x[e], s, BITS == 4 ? 7.0f : 127.0f) + kMagic;
+      for (int e = 0; e < 8; ++e) z[e] = code_by_division(static_cast<double>(x[e]) * r, s, BITS == 4 ? 7.0f : 127.0f) + kMagic;
     }
   }
   // sum of (z - magic's bits) 2^(BITS e): the magic's bits are taken out of the sum
@@ -117,13 +122,17 @@ __device__ __forceinline__ void copies_wait() {
 
 // d / 16 lanes own a head: lane j has columns [8j, 8j + 8) of both halves, i.e. both sides of its eight
 // rotation pairs, so the rotation needs no exchange and the head's sums are log2(d / 16) shuffles. An item is the heads
-// that a warp takes at once (four of 128); the items of all rows are one line, of which every warp has an equal run:
-// query, key and value heads cost 1 : 3 : 1.5, so runs, not strides, keep the warps even, and a row's tables are
-// loaded once. A lane's 32 bytes of the next three items are on their way by asynchronous copies into slots of
-// its own, so nothing is synchronised. What bounds the kernel is memory, 22 KB a row of 48 heads in and out.
-constexpr int kQkDepth = 4, kQkCtas = 6;
+// that a warp takes at once (four of 128), of q or of k and v; the items of all rows are one line, of which every warp has
+// an equal run: the kinds cost 1 : 5 : 2, so runs, not strides, keep the warps even, and what depends on the row alone
+// (the products of norm weights and tables for q) is worked out once. A lane's 32 bytes of the next three items are on
+// their way by asynchronous copies into slots of its own, so nothing is synchronised. Arithmetic is on pairs of f32 where
+// it can be. What bounds the kernel is memory, 22 KB a row of 48 heads in and out, and close behind it the issue slots
+// (2000 warp instructions a row).
+// K: with y = rot(x w), in double from exact products, rot(n) = r y: the scale is f32(r max |y| / top) and the
+// quotients are y (r / scale), so r multiplies a head's largest value only.
+constexpr int kQkDepth = 4, kQkCtas = 5;
 template <int D, int BITS>
-__global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(const QkNormParams p, int per_row, int items) {
+__global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(const QkNormParams p, int q_parts, int per_row, int items) {
   pdl_begin();
   constexpr int kLanes = D / 16, kHeads = 32 / kLanes, kTop = BITS == 4 ? 7 : 127;
   __shared__ uint4 s_raw[kQkDepth][2][kQkThreads];
@@ -134,136 +143,166 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
   const int begin = static_cast<int>(static_cast<unsigned long long>(warp) * items / warps);
   const int end = static_cast<int>(static_cast<unsigned long long>(warp + 1) * items / warps);
   if (begin >= end) return;
-  // (row, part) of the item to work on and of the item to fetch
-  int row = begin / per_row, part = begin - row * per_row, f_row = row, f_part = part;
-  auto fetch = [&](int item) {
-    if (item < end) {
-      const int head = f_part * kHeads + g;
-      if (head < heads) {
-        const uint4* src = reinterpret_cast<const uint4*>(p.qkv + (static_cast<size_t>(f_row) * heads + head) * D) + j;
-        copy16_async(&s_raw[item % kQkDepth][0][threadIdx.x], src);
-        copy16_async(&s_raw[item % kQkDepth][1][threadIdx.x], src + kLanes);
+  int row = begin / per_row, f_row = row, part = begin - row * per_row, f_part = part, f_item = begin;
+  auto fetch = [&]() {  // the next item that is not on its way yet
+    if (f_item < end) {
+      const bool q = f_part < q_parts;
+      const int in = (q ? f_part : f_part - q_parts) * kHeads + g;
+      if (in < (q ? p.Hq : 2 * p.Hk)) {
+        const uint4* src = reinterpret_cast<const uint4*>(p.qkv + (static_cast<size_t>(f_row) * heads + (q ? in : p.Hq + in)) * D) + j;
+        copy16_async(&s_raw[f_item % kQkDepth][0][threadIdx.x], src);
+        copy16_async(&s_raw[f_item % kQkDepth][1][threadIdx.x], src + kLanes);
       }
       if (++f_part == per_row) f_part = 0, ++f_row;
     }
+    ++f_item;
     copies_commit();
   };
 #pragma unroll
-  for (int i = 0; i < kQkDepth - 1; ++i) fetch(begin + i);
-  int next_pos = __ldg(p.pos_rows + row), next_kv = __ldg(p.kv_rows + row), pos = 0, kv_row = 0;
-  float c[8], s[8];
-  bool fresh = true, sound = false;
-#pragma unroll 1
-  for (int item = begin; item < end; ++item) {
-    if (fresh) {
-      pos = next_pos, kv_row = next_kv;
-      if (row + 1 < p.rows) next_pos = __ldg(p.pos_rows + row + 1), next_kv = __ldg(p.kv_rows + row + 1);
-      // a bad index skips the row instead of touching memory outside the tables or the pool
-      sound = pos >= 0 && pos < p.max_pos && kv_row >= 0 && kv_row < p.stride;
-      if (sound) {
+  for (int i = 0; i < kQkDepth - 1; ++i) fetch();
+  int next_pos = __ldg(p.pos_rows + row), next_kv = __ldg(p.kv_rows + row);
+  for (int item = begin; item < end; ++row, part = 0) {
+    const int pos = next_pos, kv_row = next_kv, stop = min(end, item + per_row - part);  // this row's items of the run
+    if (row + 1 < p.rows) next_pos = __ldg(p.pos_rows + row + 1), next_kv = __ldg(p.kv_rows + row + 1);
+    // a bad index skips the row instead of touching memory outside the tables or the pool
+    const bool sound = pos >= 0 && pos < p.max_pos && kv_row >= 0 && kv_row < p.stride;
+    const float4* cp = reinterpret_cast<const float4*>(p.cos_tbl + static_cast<size_t>(sound ? pos : 0) * (D / 2) + 8 * j);
+    const float4* sp = reinterpret_cast<const float4*>(p.sin_tbl + static_cast<size_t>(sound ? pos : 0) * (D / 2) + 8 * j);
+
+    if (part < q_parts) {
+      F32x2 ac[4], as[4], bc[4], bs[4];  // rot = (a ac - b bs, b bc + a as), bs kept negative
+      {
+        const float4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
+        ac[0] = f32x2(c0.x, c0.y), ac[1] = f32x2(c0.z, c0.w), ac[2] = f32x2(c1.x, c1.y), ac[3] = f32x2(c1.z, c1.w);
+        as[0] = f32x2(s0.x, s0.y), as[1] = f32x2(s0.z, s0.w), as[2] = f32x2(s1.x, s1.y), as[3] = f32x2(s1.z, s1.w);
+        const uint4 one = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+        const uint4 a4 = p.wq != nullptr ? __ldg(reinterpret_cast<const uint4*>(p.wq) + j) : one;
+        const uint4 b4 = p.wq != nullptr ? __ldg(reinterpret_cast<const uint4*>(p.wq) + kLanes + j) : one;
+        const uint32_t aw[4] = {a4.x, a4.y, a4.z, a4.w}, bw[4] = {b4.x, b4.y, b4.z, b4.w};
+        const F32x2 minus = f32x2(-1.0f, -1.0f);
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          const float4 cv = __ldg(reinterpret_cast<const float4*>(p.cos_tbl + static_cast<size_t>(pos) * (D / 2) + 8 * j + e));
-          const float4 sv = __ldg(reinterpret_cast<const float4*>(p.sin_tbl + static_cast<size_t>(pos) * (D / 2) + 8 * j + e));
-          c[e] = cv.x, c[e + 1] = cv.y, c[e + 2] = cv.z, c[e + 3] = cv.w;
-          s[e] = sv.x, s[e + 1] = sv.y, s[e + 2] = sv.z, s[e + 3] = sv.w;
+        for (int e = 0; e < 4; ++e) {
+          const F32x2 a = bf16x2_f32(aw[e]), b = bf16x2_f32(bw[e]);
+          bc[e] = mul2(b, ac[e]), bs[e] = mul2(mul2(b, as[e]), minus);
+          ac[e] = mul2(a, ac[e]), as[e] = mul2(a, as[e]);
         }
       }
+#pragma unroll 1
+      for (; part < q_parts && item < stop; ++part, ++item) {
+        fetch();
+        copies_wait<kQkDepth - 1>();
+        const int head = part * kHeads + g;
+        if (!sound || head >= p.Hq) continue;
+        const uint4 a4 = s_raw[item % kQkDepth][0][threadIdx.x], b4 = s_raw[item % kQkDepth][1][threadIdx.x];
+        const F32x2 a[4] = {bf16x2_f32(a4.x), bf16x2_f32(a4.y), bf16x2_f32(a4.z), bf16x2_f32(a4.w)};
+        const F32x2 b[4] = {bf16x2_f32(b4.x), bf16x2_f32(b4.y), bf16x2_f32(b4.z), bf16x2_f32(b4.w)};
+        float rn = 1.0f;
+        if (p.wq != nullptr) {
+          F32x2 s2 = mul2(a[0], a[0]), t2 = mul2(b[0], b[0]);
+#pragma unroll
+          for (int e = 1; e < 4; ++e) s2 = fma2(a[e], a[e], s2), t2 = fma2(b[e], b[e], t2);
+          float s0, s1, t0, t1;
+          f32x2_split(s2, s0, s1);
+          f32x2_split(t2, t0, t1);
+          float ss = (s0 + s1) + (t0 + t1);
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+          rn = rsqrtf(ss * (1.0f / D) + p.eps);
+        }
+        const F32x2 rn2 = f32x2(rn, rn);
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x, y;
+          f32x2_split(mul2(fma2(b[e], bs[e], mul2(a[e], ac[e])), rn2), x, y);
+          lo[e] = pack_bf16x2(x, y);
+          f32x2_split(mul2(fma2(a[e], as[e], mul2(b[e], bc[e])), rn2), x, y);
+          hi[e] = pack_bf16x2(x, y);
+        }
+        uint4* dst = reinterpret_cast<uint4*>(p.q_rot + (static_cast<size_t>(row) * p.Hq + head) * D);
+        st_stream(dst + j, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+        st_stream(dst + kLanes + j, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+      }
     }
-    fetch(item + kQkDepth - 1);
-    copies_wait<kQkDepth - 1>();
-    const int head = part * kHeads + g, r = row;
-    fresh = ++part == per_row;
-    if (fresh) part = 0, ++row;
-    if (!sound || head >= heads) continue;
-    float lo[8], hi[8];
-    unpack8(s_raw[item % kQkDepth][0][threadIdx.x], lo);
-    unpack8(s_raw[item % kQkDepth][1][threadIdx.x], hi);
-    const bool is_q = head < p.Hq, is_k = !is_q && head < p.Hq + p.Hk;
-    const uint16_t* wt = is_q ? p.wq : p.wk;
-    if (is_q) {
-      if (wt != nullptr) {
-        float wl[8], wh[8];
-        unpack8(__ldg(reinterpret_cast<const uint4*>(wt) + j), wl);
-        unpack8(__ldg(reinterpret_cast<const uint4*>(wt) + kLanes + j), wh);
-        float ss = 0.0f;
+
+#pragma unroll 1
+    for (; item < stop; ++part, ++item) {
+      fetch();
+      copies_wait<kQkDepth - 1>();
+      const int head = (part - q_parts) * kHeads + g;  // of k, then of v
+      if (!sound || head >= 2 * p.Hk) continue;
+      const bool is_k = head < p.Hk;
+      const size_t srow = static_cast<size_t>(is_k ? head : head - p.Hk) * p.stride + kv_row;
+      float lo[8], hi[8], sc;
+      unpack8(s_raw[item % kQkDepth][0][threadIdx.x], lo);
+      unpack8(s_raw[item % kQkDepth][1][threadIdx.x], hi);
+      uint2 cl, ch;
+      if (is_k) {
+        double rn = 1.0, dl[8], dh[8];
+        if (p.wk != nullptr) {
+          double ss = 0.0, st = 0.0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += lo[e] * lo[e] + hi[e] * hi[e];
+          for (int e = 0; e < 8; ++e) {
+            const double x = lo[e], y = hi[e];
+            ss += x * x, st += y * y;
+          }
+          ss += st;
 #pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float rn = rsqrtf(ss * (1.0f / D) + p.eps);
+          for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+          rn = rsqrt(ss * (1.0 / D) + static_cast<double>(p.eps));
+          float w[8];  // products of two bf16 are exact in f32
+          unpack8(__ldg(reinterpret_cast<const uint4*>(p.wk) + j), w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) lo[e] *= rn * wl[e], hi[e] *= rn * wh[e];
+          for (int e = 0; e < 8; ++e) lo[e] *= w[e];
+          unpack8(__ldg(reinterpret_cast<const uint4*>(p.wk) + kLanes + j), w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) hi[e] *= w[e];
+        }
+        double amax = 0.0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 c4 = __ldg(cp + h), s4 = __ldg(sp + h);
+          const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int e = 4 * h + i;
+            const double a = lo[e], b = hi[e], cd = c[i], sd = s[i];
+            dl[e] = a * cd - b * sd, dh[e] = b * cd + a * sd;
+            const double x = fabs(dl[e]), y = fabs(dh[e]);
+            amax = x > amax ? x : amax;
+            amax = y > amax ? y : amax;
+            lo[e] = static_cast<float>(dl[e]), hi[e] = static_cast<float>(dh[e]);
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) {
+          const double x = __shfl_xor_sync(mask, amax, o);
+          amax = x > amax ? x : amax;
+        }
+        sc = static_cast<float>(amax * rn * (1.0 / kTop));
+        const bool plain = sc > 1e-30f;
+        const float inv = plain ? static_cast<float>(rn) / sc : 0.0f;
+        cl = encode8<BITS>(dl, lo, sc, rn, plain, inv), ch = encode8<BITS>(dh, hi, sc, rn, plain, inv);
+      } else {
+        float amax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
+        sc = __fdiv_rn(amax, static_cast<float>(kTop));  // eight significant bits over 7 or 127: never half way between floats
+        const bool plain = sc > 1e-30f;
+        const float inv = plain ? 1.0f / sc : 0.0f;
+        cl = encode8<BITS>(lo, lo, sc, 1.0f, plain, inv), ch = encode8<BITS>(hi, hi, sc, 1.0f, plain, inv);
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = lo[e], b = hi[e];
-        lo[e] = a * c[e] - b * s[e], hi[e] = b * c[e] + a * s[e];
+      if (j == 0) (is_k ? p.k_scale : p.v_scale)[srow] = sc;
+      uint8_t* cache = (is_k ? p.cache_k : p.cache_v) + srow * (D * BITS / 8);
+      if (BITS == 4) {
+        reinterpret_cast<uint32_t*>(cache)[j] = cl.x;
+        reinterpret_cast<uint32_t*>(cache)[kLanes + j] = ch.x;
+      } else {
+        reinterpret_cast<uint2*>(cache)[j] = cl;
+        reinterpret_cast<uint2*>(cache)[kLanes + j] = ch;
       }
-      uint4* dst = reinterpret_cast<uint4*>(p.q_rot + (static_cast<size_t>(r) * p.Hq + head) * D);
-      st_stream(dst + j, pack8(lo));
-      st_stream(dst + kLanes + j, pack8(hi));
-      continue;
-    }
-    const int hkv = is_k ? head - p.Hq : head - p.Hq - p.Hk;
-    const size_t srow = static_cast<size_t>(hkv) * p.stride + kv_row;
-    float sc;
-    uint2 cl, ch;
-    if (is_k) {
-      double dl[8], dh[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dl[e] = lo[e], dh[e] = hi[e];
-      if (wt != nullptr) {
-        double ss = 0.0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += dl[e] * dl[e] + dh[e] * dh[e];
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const double rn = 1.0 / sqrt(ss * (1.0 / D) + static_cast<double>(p.eps));
-        float wl[8], wh[8];
-        unpack8(__ldg(reinterpret_cast<const uint4*>(wt) + j), wl);
-        unpack8(__ldg(reinterpret_cast<const uint4*>(wt) + kLanes + j), wh);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dl[e] *= rn * wl[e], dh[e] *= rn * wh[e];
-      }
-      double amax = 0.0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double a = dl[e], b = dh[e];
-        dl[e] = a * c[e] - b * s[e], dh[e] = b * c[e] + a * s[e];
-        const double x = fabs(dl[e]), y = fabs(dh[e]);
-        amax = x > amax ? x : amax;
-        amax = y > amax ? y : amax;
-        lo[e] = static_cast<float>(dl[e]), hi[e] = static_cast<float>(dh[e]);
-      }
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) {
-        const double x = __shfl_xor_sync(mask, amax, o);
-        amax = x > amax ? x : amax;
-      }
-      sc = static_cast<float>(amax / kTop);
-      const bool plain = sc > 1e-30f;
-      const float inv = plain ? 1.0f / sc : 0.0f;
-      cl = encode8<BITS>(dl, lo, sc, plain, inv), ch = encode8<BITS>(dh, hi, sc, plain, inv);
-    } else {
-      float amax = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
-      sc = __fdiv_rn(amax, static_cast<float>(kTop));  // eight significant bits over 7 or 127: never half way between floats
-      const bool plain = sc > 1e-30f;
-      const float inv = plain ? 1.0f / sc : 0.0f;
-      cl = encode8<BITS>(lo, lo, sc, plain, inv), ch = encode8<BITS>(hi, hi, sc, plain, inv);
-    }
-    if (j == 0) (is_k ? p.k_scale : p.v_scale)[srow] = sc;
-    uint8_t* cache = (is_k ? p.cache_k : p.cache_v) + srow * (D * BITS / 8);
-    if (BITS == 4) {
-      reinterpret_cast<uint32_t*>(cache)[j] = cl.x;
-      reinterpret_cast<uint32_t*>(cache)[kLanes + j] = ch.x;
-    } else {
-      reinterpret_cast<uint2*>(cache)[j] = cl;
-      reinterpret_cast<uint2*>(cache)[kLanes + j] = ch;
     }
   }
 }
@@ -271,12 +310,13 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
 template <int D, int BITS>
 int launch_qk_norm(const char* fn, const QkNormParams& p) {
   constexpr int heads_per_item = 32 / (D / 16), warps = kQkThreads / 32;
-  const int per_row = (p.Hq + 2 * p.Hk + heads_per_item - 1) / heads_per_item;
+  const int q_parts = (p.Hq + heads_per_item - 1) / heads_per_item;
+  const int per_row = q_parts + (2 * p.Hk + heads_per_item - 1) / heads_per_item;
   const long long items = static_cast<long long>(p.rows) * per_row;
   if (items > INT_MAX - kQkDepth) return fail(fn, "too many rows");
   const long long grid = std::min((items + warps - 1) / warps, static_cast<long long>(kQkCtas) * sm_count());
   G4_LAUNCH_PDL(fn, (qk_norm_rope_kv_kernel<D, BITS>), dim3(static_cast<unsigned>(grid)), dim3(kQkThreads), 0, current_stream(), p,
-                per_row, static_cast<int>(items));
+                q_parts, per_row, static_cast<int>(items));
   return 0;
 }
 
