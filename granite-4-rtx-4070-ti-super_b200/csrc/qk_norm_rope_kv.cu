@@ -9,12 +9,16 @@
 // The 4-bit pool keeps code + 8 in a nibble, the even dim in the low half of its byte, [Hk][stride][d / 2];
 // the 8-bit pool is the one rope_kv.cu writes, [Hk][stride][d]. Both have f32 scales [Hk][stride].
 //
-// The one rounding of a code is its own: K is normed and rotated in double from its bf16 values and the f32
-// tables, so that a code does not depend on the order in which a kernel rounds its way there. What is left
-// of a double between the value and the border of two codes is 1e-15 of the scale.
-// The code itself is found in f32 (value
-// times the scale's reciprocal, off by 2^-22 of it at most) wherever that is further from a border than 2^-14;
-// where it is not, the sign of fma(-(code +- 1/2), scale, |x|) decides, which an fma gives exactly.
+// The one rounding of a code is its own: a code is the one that exact arithmetic on the bf16 inputs and the f32 tables
+// gives (in double where it matters: 1e-15 of the scale), so that it does not depend on the order in which a kernel
+// rounds its way there. Doubles are few: with y = rot(x w) (products of two bf16 are exact in f32) rot(n) = r y, the
+// scale is f32(r max |y| / top) and the quotients are y (r / scale). r is a double, y is f32, off by at most 2^-22 of the
+// head's max |y|. In double are only y of the pairs that may hold the maximum (those within 2^-19 of it: hardly ever
+// more than one a head), and y of a pair with a quotient so near to the border of two codes that f32 may be wrong, where
+// the sign of fma(-(code +- 1/2), scale, |r y|) decides, which an fma gives exactly.
+// V: value and amax have eight significant bits each, so a quotient top v / amax is a border exactly or further from it
+// than 1 / (2 top 255) >= 2^-16 of itself. Exact ones (v = amax / 2 is one in every third head) fall to the side that the
+// rounding of the scale pushes them to: the scale's reciprocal, moved by 2^-19 of itself to that side, decides all.
 //
 #include "g4_host.h"
 #include "g4_math.cuh"
@@ -45,7 +49,10 @@ struct QkNormParams {
 };
 
 constexpr int kQkThreads = 128;
-constexpr float kNearBorder = 0.5f - 1.0f / 16384.0f;
+// An f32 quotient further than this from its code may belong to the next: y and r / scale are off by 5.5 2^-24 of the
+// quotients' range, 2.3e-6 (4 bits) and 4.2e-5.
+template <int BITS>
+constexpr float kNearBorder = 0.5f - (BITS == 4 ? 1.0f / 131072.0f : 1.0f / 16384.0f);
 
 // |x| against the borders of code c: the code itself.
 __device__ __forceinline__ float settle(float c, float x, float s) {
@@ -65,38 +72,38 @@ __device__ __noinline__ float code_by_division(double x, float s, float top) {
   return x < 0.0 ? -c : c;
 }
 
-// Codes of a lane's values r x (xf: x in f32; inv: r / s) under scale s, as the words of the pool: 4 bits, code + 8, or 8.
-template <int BITS, typename T>
-__device__ __forceinline__ uint2 encode8(const T (&x)[8], const float (&xf)[8], float s, T r, bool plain, float inv) {
-  // adding 1.5 2^23 (and the 8) leaves the integer in the low bits of the sum
-  constexpr float kMagic = 12582912.0f + (BITS == 4 ? 8.0f : 0.0f);
-  const F32x2 inv2 = f32x2(inv, inv), magic2 = f32x2(kMagic, kMagic), one2 = f32x2(1.0f, 1.0f), minus2 = f32x2(-1.0f, -1.0f);
-  const F32x2 less2 = f32x2(-kMagic, -kMagic);
-  float z[8], far = plain ? 0.0f : 1.0f;
+// Eight quotients x inv rounded to the nearest integer, as z = code + magic in f32: 1.5 2^23 (and the 8 of a nibble)
+// leaves the integer in the low bits of the sum. Returns the largest distance |quotient - code|.
+template <int BITS>
+constexpr float kMagic = 12582912.0f + (BITS == 4 ? 8.0f : 0.0f);
+template <int BITS>
+__device__ __forceinline__ float round8(const float (&x)[8], float inv, float (&z)[8]) {
+  const F32x2 inv2 = f32x2(inv, inv), magic2 = f32x2(kMagic<BITS>, kMagic<BITS>), one2 = f32x2(1.0f, 1.0f);
+  const F32x2 less2 = f32x2(-kMagic<BITS>, -kMagic<BITS>), minus2 = f32x2(-1.0f, -1.0f);
+  float far = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    const F32x2 t = mul2(f32x2(xf[e], xf[e + 1]), inv2), zz = fma2(t, one2, magic2);
-    const F32x2 off = fma2(fma2(zz, one2, less2), minus2, t);  // t - code
+    const F32x2 t = mul2(f32x2(x[e], x[e + 1]), inv2), zz = fma2(t, one2, magic2);
+    const F32x2 off = fma2(fma2(zz, one2, less2), minus2, t);
     float u, v;
     f32x2_split(off, u, v);
     f32x2_split(zz, z[e], z[e + 1]);
     far = fmaxf(far, fmaxf(fabsf(u), fabsf(v)));
   }
-  if (!(far < kNearBorder)) {
-    if (plain) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float code = settle(fabsf(z[e] - kMagic), (x[e] < T(0) ? -x[e] : x[e]) * r, s);
-        z[e] = (x[e] < T(0) ? -code : code) + kMagic;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = code_by_division(static_cast<double>(x[e]) * r, s, BITS == 4 ? 7.0f : 127.0f) + kMagic;
-    }
-  }
-  // sum of (z - magic's bits) 2^(BITS e): the magic's bits are taken out of the sum
+  return far;
+}
+// z settled against the exact value x.
+template <int BITS, typename T>
+__device__ __forceinline__ float settled(float z, T x, float s, bool plain) {
+  if (!plain) return code_by_division(x, s, BITS == 4 ? 7.0f : 127.0f) + kMagic<BITS>;
+  const float c = settle(fabsf(z - kMagic<BITS>), x < T(0) ? -x : x, s);
+  return (x < T(0) ? -c : c) + kMagic<BITS>;
+}
+// The words of the pool: 4 bits, code + 8, or 8.
+template <int BITS>
+__device__ __forceinline__ uint2 pack_codes(const float (&z)[8]) {
   uint2 w = make_uint2(0u, 0u);
-  if (BITS == 4) {
+  if (BITS == 4) {  // sum of (bits of z - bits of 1.5 2^23) 16^e
 #pragma unroll
     for (int e = 0; e < 8; ++e) w.x += __float_as_uint(z[e]) << (4 * e);
     w.x -= 0x4b400000u * 0x11111111u;
@@ -108,6 +115,15 @@ __device__ __forceinline__ uint2 encode8(const T (&x)[8], const float (&xf)[8], 
     }
   }
   return w;
+}
+
+// y of pair e of a lane in double, from where its inputs lie. Out of line: the kernel's instructions have to stay in the cache.
+__device__ __noinline__ double2 key_pair(const uint16_t* a, const uint16_t* b, const uint16_t* wa, const uint16_t* wb,
+                                         const float* c, const float* s, int e) {
+  float x = bf16_to_f32(a[e]), y = bf16_to_f32(b[e]);
+  if (wa != nullptr) x *= bf16_to_f32(__ldg(wa + e)), y *= bf16_to_f32(__ldg(wb + e));
+  const double cd = __ldg(c + e), sd = __ldg(s + e);
+  return make_double2(x * cd - y * sd, y * cd + x * sd);
 }
 
 __device__ __forceinline__ void copy16_async(void* dst, const void* src) {
@@ -123,44 +139,43 @@ __device__ __forceinline__ void copies_wait() {
 // d / 16 lanes own a head: lane j has columns [8j, 8j + 8) of both halves, i.e. both sides of its eight
 // rotation pairs, so the rotation needs no exchange and the head's sums are log2(d / 16) shuffles. An item is the heads
 // that a warp takes at once (four of 128), of q or of k and v; the items of all rows are one line, of which every warp has
-// an equal run: the kinds cost 1 : 5 : 2, so runs, not strides, keep the warps even, and what depends on the row alone
+// an equal run: the kinds cost 1 : 3 : 2, so runs, not strides, keep the warps even, and what depends on the row alone
 // (the products of norm weights and tables for q) is worked out once. A lane's 32 bytes of the next three items are on
 // their way by asynchronous copies into slots of its own, so nothing is synchronised. Arithmetic is on pairs of f32 where
-// it can be. What bounds the kernel is memory, 22 KB a row of 48 heads in and out, and close behind it the issue slots
-// (2000 warp instructions a row).
-// K: with y = rot(x w), in double from exact products, rot(n) = r y: the scale is f32(r max |y| / top) and the
-// quotients are y (r / scale), so r multiplies a head's largest value only.
-constexpr int kQkDepth = 4, kQkCtas = 5;
+// it can be. What bounds the kernel is memory, 22 KB a row of 48 heads in and out, and close behind it the issue slots.
+constexpr int kQkDepth = 4, kQkCtas = 6;
 template <int D, int BITS>
-__global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(const QkNormParams p, int q_parts, int per_row, int items) {
+__global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(const QkNormParams p, int q_parts, int per_row, int run, int longer) {
   pdl_begin();
   constexpr int kLanes = D / 16, kHeads = 32 / kLanes, kTop = BITS == 4 ? 7 : 127;
   __shared__ uint4 s_raw[kQkDepth][2][kQkThreads];
   const int lane = threadIdx.x & 31, g = lane / kLanes, j = lane % kLanes;
   const unsigned mask = ((1u << kLanes) - 1u) << (lane & ~(kLanes - 1));
   const int heads = p.Hq + 2 * p.Hk;
-  const unsigned warps = gridDim.x * (kQkThreads / 32), warp = blockIdx.x * (kQkThreads / 32) + (threadIdx.x >> 5);
-  const int begin = static_cast<int>(static_cast<unsigned long long>(warp) * items / warps);
-  const int end = static_cast<int>(static_cast<unsigned long long>(warp + 1) * items / warps);
+  // the first `longer` warps have run + 1 items, the others run
+  const int warp = blockIdx.x * (kQkThreads / 32) + (threadIdx.x >> 5);
+  const int begin = warp * run + min(warp, longer), end = begin + run + (warp < longer ? 1 : 0);
   if (begin >= end) return;
-  int row = begin / per_row, f_row = row, part = begin - row * per_row, f_part = part, f_item = begin;
+  int row = begin / per_row, part = begin - row * per_row, f_left = end - begin, f_part = part;
+  int f_slot = 0, slot = 0;
+  const uint4* f_row = reinterpret_cast<const uint4*>(p.qkv) + static_cast<size_t>(row) * heads * (D / 8) + g * (D / 8) + j;
   auto fetch = [&]() {  // the next item that is not on its way yet
-    if (f_item < end) {
+    if (f_left > 0) {
       const bool q = f_part < q_parts;
-      const int in = (q ? f_part : f_part - q_parts) * kHeads + g;
-      if (in < (q ? p.Hq : 2 * p.Hk)) {
-        const uint4* src = reinterpret_cast<const uint4*>(p.qkv + (static_cast<size_t>(f_row) * heads + (q ? in : p.Hq + in)) * D) + j;
-        copy16_async(&s_raw[f_item % kQkDepth][0][threadIdx.x], src);
-        copy16_async(&s_raw[f_item % kQkDepth][1][threadIdx.x], src + kLanes);
+      const int first = (q ? f_part : f_part - q_parts) * kHeads;  // of the item's heads, counted from the first q or k head
+      if (first + g < (q ? p.Hq : 2 * p.Hk)) {
+        const uint4* src = f_row + (q ? first : p.Hq + first) * (D / 8);
+        copy16_async(&s_raw[f_slot][0][threadIdx.x], src);
+        copy16_async(&s_raw[f_slot][1][threadIdx.x], src + kLanes);
       }
-      if (++f_part == per_row) f_part = 0, ++f_row;
+      if (++f_part == per_row) f_part = 0, f_row += heads * (D / 8);
     }
-    ++f_item;
+    --f_left, f_slot = (f_slot + 1) % kQkDepth;
     copies_commit();
   };
+  int next_pos = __ldg(p.pos_rows + row), next_kv = __ldg(p.kv_rows + row);
 #pragma unroll
   for (int i = 0; i < kQkDepth - 1; ++i) fetch();
-  int next_pos = __ldg(p.pos_rows + row), next_kv = __ldg(p.kv_rows + row);
   for (int item = begin; item < end; ++row, part = 0) {
     const int pos = next_pos, kv_row = next_kv, stop = min(end, item + per_row - part);  // this row's items of the run
     if (row + 1 < p.rows) next_pos = __ldg(p.pos_rows + row + 1), next_kv = __ldg(p.kv_rows + row + 1);
@@ -192,8 +207,9 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
         fetch();
         copies_wait<kQkDepth - 1>();
         const int head = part * kHeads + g;
+        const uint4 a4 = s_raw[slot][0][threadIdx.x], b4 = s_raw[slot][1][threadIdx.x];
+        slot = (slot + 1) % kQkDepth;
         if (!sound || head >= p.Hq) continue;
-        const uint4 a4 = s_raw[item % kQkDepth][0][threadIdx.x], b4 = s_raw[item % kQkDepth][1][threadIdx.x];
         const F32x2 a[4] = {bf16x2_f32(a4.x), bf16x2_f32(a4.y), bf16x2_f32(a4.z), bf16x2_f32(a4.w)};
         const F32x2 b[4] = {bf16x2_f32(b4.x), bf16x2_f32(b4.y), bf16x2_f32(b4.z), bf16x2_f32(b4.w)};
         float rn = 1.0f;
@@ -230,16 +246,18 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
       fetch();
       copies_wait<kQkDepth - 1>();
       const int head = (part - q_parts) * kHeads + g;  // of k, then of v
+      const uint4* const raw = &s_raw[slot][0][threadIdx.x];
+      slot = (slot + 1) % kQkDepth;
       if (!sound || head >= 2 * p.Hk) continue;
       const bool is_k = head < p.Hk;
       const size_t srow = static_cast<size_t>(is_k ? head : head - p.Hk) * p.stride + kv_row;
-      float lo[8], hi[8], sc;
-      unpack8(s_raw[item % kQkDepth][0][threadIdx.x], lo);
-      unpack8(s_raw[item % kQkDepth][1][threadIdx.x], hi);
-      uint2 cl, ch;
+      float lo[8], hi[8], zl[8], zh[8], sc;
+      unpack8(raw[0], lo);
+      unpack8(raw[kQkThreads], hi);
       if (is_k) {
-        double rn = 1.0, dl[8], dh[8];
-        if (p.wk != nullptr) {
+        double rn = 1.0;
+        const uint16_t* const wa = p.wk != nullptr ? p.wk + 8 * j : nullptr;
+        if (wa != nullptr) {
           double ss = 0.0, st = 0.0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -251,14 +269,15 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
           for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
           rn = rsqrt(ss * (1.0 / D) + static_cast<double>(p.eps));
           float w[8];  // products of two bf16 are exact in f32
-          unpack8(__ldg(reinterpret_cast<const uint4*>(p.wk) + j), w);
+          unpack8(__ldg(reinterpret_cast<const uint4*>(wa)), w);
 #pragma unroll
           for (int e = 0; e < 8; ++e) lo[e] *= w[e];
-          unpack8(__ldg(reinterpret_cast<const uint4*>(p.wk) + kLanes + j), w);
+          unpack8(__ldg(reinterpret_cast<const uint4*>(wa + D / 2)), w);
 #pragma unroll
           for (int e = 0; e < 8; ++e) hi[e] *= w[e];
         }
-        double amax = 0.0;
+        // the largest |y| of a pair, its last three bits the pair's number; the lane's largest and second
+        unsigned best = 0, second = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float4 c4 = __ldg(cp + h), s4 = __ldg(sp + h);
@@ -266,14 +285,31 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int e = 4 * h + i;
-            const double a = lo[e], b = hi[e], cd = c[i], sd = s[i];
-            dl[e] = a * cd - b * sd, dh[e] = b * cd + a * sd;
-            const double x = fabs(dl[e]), y = fabs(dh[e]);
-            amax = x > amax ? x : amax;
-            amax = y > amax ? y : amax;
-            lo[e] = static_cast<float>(dl[e]), hi[e] = static_cast<float>(dh[e]);
+            const float a = lo[e], b = hi[e];
+            lo[e] = fmaf(a, c[i], -(b * s[i])), hi[e] = fmaf(b, c[i], a * s[i]);
+            const unsigned key = (__float_as_uint(fmaxf(fabsf(lo[e]), fabsf(hi[e]))) & ~7u) | e;
+            second = max(second, min(best, key)), best = max(best, key);
           }
         }
+        unsigned top = best;
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+        const unsigned floor_key = top > 32u ? top - 32u : 0u;  // what y lost, and the three bits
+        const uint16_t* const ra = reinterpret_cast<const uint16_t*>(raw);
+        const uint16_t* const rb = reinterpret_cast<const uint16_t*>(raw + kQkThreads);
+        const float* const ct = reinterpret_cast<const float*>(cp);
+        const float* const st = reinterpret_cast<const float*>(sp);
+        double amax = 0.0;
+        if (best >= floor_key) {
+          const bool several = second >= floor_key;
+          const int from = several ? 0 : best & 7, to = several ? 7 : from;
+#pragma unroll 1
+          for (int e = from; e <= to; ++e) {
+            const double2 y = key_pair(ra, rb, wa, wa + D / 2, ct, st, e);
+            amax = fmax(amax, fmax(fabs(y.x), fabs(y.y)));
+          }
+        }
+        __syncwarp(mask);
 #pragma unroll
         for (int o = 1; o < kLanes; o <<= 1) {
           const double x = __shfl_xor_sync(mask, amax, o);
@@ -282,7 +318,17 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
         sc = static_cast<float>(amax * rn * (1.0 / kTop));
         const bool plain = sc > 1e-30f;
         const float inv = plain ? static_cast<float>(rn) / sc : 0.0f;
-        cl = encode8<BITS>(dl, lo, sc, rn, plain, inv), ch = encode8<BITS>(dh, hi, sc, rn, plain, inv);
+        const float far = fmaxf(round8<BITS>(lo, inv, zl), round8<BITS>(hi, inv, zh));
+        if (!plain || !(far < kNearBorder<BITS>)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float dl = fabsf(lo[e] * inv - (zl[e] - kMagic<BITS>)), dh = fabsf(hi[e] * inv - (zh[e] - kMagic<BITS>));
+            if (!plain || !(fmaxf(dl, dh) < 2.0f * kNearBorder<BITS> - 0.5f)) {  // (these products may be rounded elsewhere)
+              const double2 y = key_pair(ra, rb, wa, wa + D / 2, ct, st, e);
+              zl[e] = settled<BITS>(zl[e], y.x * rn, sc, plain), zh[e] = settled<BITS>(zh[e], y.y * rn, sc, plain);
+            }
+          }
+        }
       } else {
         float amax = 0.0f;
 #pragma unroll
@@ -291,9 +337,16 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
         for (int o = 1; o < kLanes; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
         sc = __fdiv_rn(amax, static_cast<float>(kTop));  // eight significant bits over 7 or 127: never half way between floats
         const bool plain = sc > 1e-30f;
-        const float inv = plain ? 1.0f / sc : 0.0f;
-        cl = encode8<BITS>(lo, lo, sc, 1.0f, plain, inv), ch = encode8<BITS>(hi, hi, sc, 1.0f, plain, inv);
+        const float side = fmaf(sc, static_cast<float>(kTop), -amax) > 0.0f ? 1.0f - 1.0f / 524288.0f : 1.0f + 1.0f / 524288.0f;
+        const float inv = plain ? __fdividef(side, sc) : 0.0f;
+        round8<BITS>(lo, inv, zl);
+        round8<BITS>(hi, inv, zh);
+        if (!plain) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) zl[e] = settled<BITS>(zl[e], lo[e], sc, false), zh[e] = settled<BITS>(zh[e], hi[e], sc, false);
+        }
       }
+      const uint2 cl = pack_codes<BITS>(zl), ch = pack_codes<BITS>(zh);
       if (j == 0) (is_k ? p.k_scale : p.v_scale)[srow] = sc;
       uint8_t* cache = (is_k ? p.cache_k : p.cache_v) + srow * (D * BITS / 8);
       if (BITS == 4) {
@@ -314,9 +367,9 @@ int launch_qk_norm(const char* fn, const QkNormParams& p) {
   const int per_row = q_parts + (2 * p.Hk + heads_per_item - 1) / heads_per_item;
   const long long items = static_cast<long long>(p.rows) * per_row;
   if (items > INT_MAX - kQkDepth) return fail(fn, "too many rows");
-  const long long grid = std::min((items + warps - 1) / warps, static_cast<long long>(kQkCtas) * sm_count());
+  const int grid = static_cast<int>(std::min((items + warps - 1) / warps, static_cast<long long>(kQkCtas) * sm_count()));
   G4_LAUNCH_PDL(fn, (qk_norm_rope_kv_kernel<D, BITS>), dim3(static_cast<unsigned>(grid)), dim3(kQkThreads), 0, current_stream(), p,
-                q_parts, per_row, static_cast<int>(items));
+                q_parts, per_row, static_cast<int>(items / (grid * warps)), static_cast<int>(items % (grid * warps)));
   return 0;
 }
 
