@@ -148,14 +148,16 @@ __device__ __forceinline__ int quotient(int a, int d) {
 }
 constexpr int kMaxQuotient = 1 << 21;
 
-// The line of `all` tiles is cut straight, into shares that differ by a tile at most, whatever segments they cross, or,
+// The line of all tiles is cut straight, into shares that differ by a tile at most, whatever segments they cross, or,
 // where a share would be short and the segments are few, into chunks of equal parts of each segment: a CTA that crosses
-// from one segment to the next pays the start of a piece (a chain of dependent loads, 2 us) twice. `chunk` is a
-// chunk's largest length, 0 for the straight cut.
+// from one segment to the next pays the start of a piece (a chain of dependent loads, 2 us) and its end twice. In the
+// straight cut that start and end count as kStartTiles tiles at the head of every segment. `chunk` is a chunk's largest
+// length, 0 for the straight cut.
 struct Cut {
   int shares, quot, rest, chunk;
 };
 constexpr int kShortShare = 64;  // tiles
+constexpr int kStartTiles = 8;
 __device__ __forceinline__ Cut cut_line(int all, int segments, int ctas) {
   Cut c;
   c.shares = all >= ctas * kWarps ? ctas : max(1, all / kWarps);  // a tile for each warp
@@ -221,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     int lo = lane_lo, hi = lane_hi;
     if (lane_groups > 1) group_span(p, grp, lo, hi);
     const int n = hi < 0 ? 0 : hi / kTile - lo / kTile + 1;
-    return chunk > 0 ? quotient(n + chunk - 1, chunk) : n;
+    return chunk > 0 ? quotient(n + chunk - 1, chunk) : n > 0 ? n + kStartTiles : 0;
   };
   if (p.split) {
     const int lane_end = min(lane_first + lane_groups, p.groups);
@@ -312,8 +314,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       piece_begin = quotient(k * n_tiles, n), piece_end = quotient((k + 1) * n_tiles, n);
       x = x_end;
     } else {
-      piece_end = min(n_tiles, piece_begin + x_end - x);
-      x += piece_end - piece_begin;
+      const int past = piece_begin + x_end - x - kStartTiles;  // of the segment's tiles, the first that is not this CTA's
+      piece_begin = max(0, piece_begin - kStartTiles), piece_end = min(n_tiles, past);
+      x = past >= n_tiles ? x_end - (past - n_tiles) : x_end;
+      if (piece_end <= 0) return;  // the share ends in the head
     }
     const size_t head_row0 = static_cast<size_t>(hkv) * p.stride;
     const uint8_t* ck = p.ck + head_row0 * kRB;
@@ -624,28 +628,29 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
   }
 }
 
-// Joins the pieces of segments that several CTAs worked on: a CTA per segment and column. The pieces' weights
-// exp2(m - max) are worked out side by side while the first pieces are on their way; each warp adds every fourth piece,
-// eight loads of a lane in flight, and the four sums meet in shared memory. The order depends on the number of pieces
-// alone.
-template <int D, int NS>
+// Joins the pieces of segments that several CTAs worked on. W warps take a column of a segment: each adds every W-th
+// piece, eight loads of a lane in flight, the weights exp2(m - max) worked out beside them (W = 4: once, into shared
+// memory, where the four sums meet too). Four warps where there are few columns, which then have many pieces; one where
+// the columns alone fill the card. The order of the sum depends on the number of pieces alone.
+template <int D, int NS, int W>
 __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4AttnParams p, int ctas) {
   pdl_begin();
   constexpr int kC = 4 * NS, kPer = D / 32, kFly = 8;
-  __shared__ float s_w[kMaxShares];
+  __shared__ float s_w[W == 4 ? kMaxShares : 1];
   __shared__ float s_red[2][kWarps];
-  __shared__ float s_acc[kWarps][D];
-  const int per_group = p.Hk * p.blocks, grp = blockIdx.x / per_group, sub = blockIdx.x - grp * per_group, c = blockIdx.y;
+  __shared__ float s_acc[W == 4 ? kWarps : 1][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_group = p.Hk * p.blocks, grp = blockIdx.x / per_group, sub = blockIdx.x - grp * per_group;
+  const int c = W == 4 ? blockIdx.y : blockIdx.y * kWarps + warp, first = W == 4 ? warp : 0;
   const int hkv = p.blocks == 1 ? sub : sub / p.blocks, c0 = p.blocks == 1 ? 0 : (sub % p.blocks) * kC;
   const int r0 = grp * p.per, nrows = min(p.per, p.rows - r0);
   if (c >= min(kC, nrows * p.G - c0)) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int before = __ldcg(p.prefix + grp), units = __ldcg(p.prefix + grp + 1) - before;
   const int all = __ldcg(p.prefix + p.groups) * per_group, shares = __ldcg(p.prefix + p.groups + 1);
-  int n = units, slot = before * per_group + sub * units;  // pieces of the segment, and where the first one lies
+  int n = units, slot = before * per_group + sub * units;  // pieces of the segment, and the first one's place
   if (n > 0 && shares > 0) {
     const Cut cut = cut_line(all, p.groups * per_group, ctas);
-    const int i0 = share_of(cut, slot);
+    const int i0 = share_of(cut, slot + kStartTiles);
     n = share_of(cut, slot + units - 1) - i0 + 1, slot = i0 + blockIdx.x;
   }
   if (n == 1) return;  // written by the one CTA
@@ -655,7 +660,7 @@ __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4Attn
   auto load = [&](int i) {
 #pragma unroll
     for (int u = 0; u < kFly; ++u) {
-      const int s = i + u * kWarps;
+      const int s = i + u * W;
 #pragma unroll
       for (int e = 0; e < kPer; e += 2) {
         const float2 w = s < n ? __ldcg(reinterpret_cast<const float2*>(part_o + static_cast<size_t>(s) * (kC * D) + e)) : make_float2(0.0f, 0.0f);
@@ -663,53 +668,72 @@ __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4Attn
       }
     }
   };
-  load(warp);
+  auto ml_of = [&](int i) {
+    return i < n ? __ldcg(reinterpret_cast<const float2*>(part_ml + static_cast<size_t>(i) * (kC * 2))) : make_float2(-INFINITY, 0.0f);
+  };
+  load(first);
   float m = -INFINITY, l = 0.0f;
-  constexpr int kEach = (kMaxShares + kThreads - 1) / kThreads;
-  float2 ml[kEach];
+  if (W == 4) {
+    constexpr int kEach = (kMaxShares + kThreads - 1) / kThreads;
+    float2 ml[kEach];
 #pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    const int i = threadIdx.x + k * kThreads;
-    ml[k] = i < n ? __ldcg(reinterpret_cast<const float2*>(part_ml + static_cast<size_t>(i) * (kC * 2))) : make_float2(-INFINITY, 0.0f);
-    m = fmaxf(m, ml[k].x);
+    for (int k = 0; k < kEach; ++k) ml[k] = ml_of(threadIdx.x + k * kThreads), m = fmaxf(m, ml[k].x);
+    m = warp_max(m);
+    if (lane == 0) s_red[0][warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      const float f = ml[k].x == -INFINITY ? 0.0f : exp2_fast(ml[k].x - m);
+      if (i < n) s_w[i] = f;
+      l += f * ml[k].y;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) s_red[1][warp] = l;
+    __syncthreads();
+    l = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+  } else {
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, ml_of(i).x);
+    m = warp_max(m);
   }
-  m = warp_max(m);
-  if (lane == 0) s_red[0][warp] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    const int i = threadIdx.x + k * kThreads;
-    const float f = ml[k].x == -INFINITY ? 0.0f : exp2_fast(ml[k].x - m);
-    if (i < n) s_w[i] = f;
-    l += f * ml[k].y;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  if (lane == 0) s_red[1][warp] = l;
-  __syncthreads();
   float acc[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
-  for (int i = warp; i < n; i += kFly * kWarps) {
-    if (i != warp) load(i);
+  for (int i = first; i < n; i += kFly * W) {
+    if (i != first) load(i);
 #pragma unroll
     for (int u = 0; u < kFly; ++u) {
-      const float f = i + u * kWarps < n ? s_w[i + u * kWarps] : 0.0f;
+      float f = 0.0f;
+      if (W == 4) {
+        if (i + u * W < n) f = s_w[i + u * W];
+      } else {
+        const float2 ml = ml_of(i + u);
+        f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - m);
+        l += f * ml.y;
+      }
 #pragma unroll
       for (int e = 0; e < kPer; ++e) acc[e] += f * v[u][e];
     }
   }
+  if (W == 4) {
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) s_acc[warp][lane * kPer + e] = acc[e];
-  __syncthreads();
-  l = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
-  const int dim = threadIdx.x;
-  if (dim < D) {
-    const float sum = (s_acc[0][dim] + s_acc[1][dim]) + (s_acc[2][dim] + s_acc[3][dim]);
-    const int j = (c0 + c) * p.g_inv >> 16, hl = c0 + c - j * p.G;
-    p.out[(static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + dim] =
-        static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? __fdividef(sum, l) : 0.0f));
+    for (int e = 0; e < kPer; ++e) s_acc[warp][lane * kPer + e] = acc[e];
+    __syncthreads();
+  }
+  const int j = (c0 + c) * p.g_inv >> 16, hl = c0 + c - j * p.G;
+  uint16_t* const out = p.out + (static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D;
+  if (W == 4) {
+    const int dim = threadIdx.x;
+    if (dim < D) {
+      const float sum = (s_acc[0][dim] + s_acc[1 % W][dim]) + (s_acc[2 % W][dim] + s_acc[3 % W][dim]);
+      out[dim] = static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? __fdividef(sum, l) : 0.0f));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)  // (the output may lie on any 2-byte boundary)
+      out[lane * kPer + e] = static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? __fdividef(acc[e], l) : 0.0f));
   }
 }
 
@@ -727,12 +751,17 @@ Int4Plan plan_int4(int rows, int per, int Hq, int Hk, int d, int max_len) {
   s.groups = (rows + per - 1) / per;
   s.segments = static_cast<long long>(s.groups) * Hk * s.blocks;
   const long long resident = std::min(static_cast<long long>(ctas_per_sm(s.ns)) * sm_count(), static_cast<long long>(kMaxShares));
-  const long long tiles = s.segments * ((max_len + kTile - 1) / kTile);
-  // short caches: a segment is one tile per warp. Many segments: the CTAs balance one another, and each saves its
-  // neighbours the joining of a piece.
-  if (max_len <= kTile * kWarps || s.groups > kMaxGroups || s.segments >= 4 * resident ||
-      tiles > INT_MAX / 2 || tiles / (static_cast<long long>(Hk) * s.blocks) >= kMaxQuotient || tiles / resident >= kMaxQuotient)
+  if (s.groups > kMaxGroups || s.segments > kMaxQuotient) return s;
+  const long long per_segment = (max_len + kTile - 1) / kTile, tiles = s.segments * per_segment;
+  if (tiles > INT_MAX / 2 || static_cast<long long>(s.groups) * per_segment >= kMaxQuotient ||
+      tiles / resident >= kMaxQuotient)
     return s;
+  // Two costs in ns. A CTA per segment: waves of a start (5 us) and a quarter of the segment's tiles for each warp, 1.7 us
+  // a tile with the card full. The line cut: a start for every segment that a CTA meets, an equal share of the tiles, the
+  // join (6 us). Measured, 8 rows x 4 heads a group, 192 rows of 192 positions: 8 and 59 us; 16 sessions of 24000: 330 and 64.
+  const long long whole = (s.segments + resident - 1) / resident * (5000 + per_segment * 425);
+  const long long cut = 5000 + 5000 * s.segments / resident + tiles * 425 / resident + 6000;
+  if (max_len <= kTile * kWarps || whole <= cut) return s;
   s.shares = static_cast<int>(std::min(resident, std::max(1ll, tiles / kWarps)));
   const long long slots = s.shares + s.segments;
   s.bytes = slots * 4 * s.ns * (d + 2) * 4 + (s.groups + 2 + 3) / 4 * 16;
@@ -760,9 +789,13 @@ int launch_int4(const char* fn, const Int4AttnParams& p, const Int4Plan& s) {
     }
   }
   G4_LAUNCH_PDL(fn, (attn_int4_kernel<D, NS>), dim3(ctas), dim3(kThreads), smem, st, p);
-  if (p.split)
-    G4_LAUNCH_PDL(fn, (attn_int4_join_kernel<D, NS>), dim3(static_cast<unsigned>(s.segments), static_cast<unsigned>(std::min(4 * NS, p.per * p.G))),
-                  dim3(kThreads), 0, st, p, s.shares);
+  if (p.split) {
+    const unsigned segments = static_cast<unsigned>(s.segments), columns = static_cast<unsigned>(std::min(4 * NS, p.per * p.G));
+    if (s.segments * columns <= 2ll * sm_count())
+      G4_LAUNCH_PDL(fn, (attn_int4_join_kernel<D, NS, 4>), dim3(segments, columns), dim3(kThreads), 0, st, p, s.shares);
+    else
+      G4_LAUNCH_PDL(fn, (attn_int4_join_kernel<D, NS, 1>), dim3(segments, (columns + kWarps - 1) / kWarps), dim3(kThreads), 0, st, p, s.shares);
+  }
   return 0;
 }
 
@@ -796,9 +829,14 @@ int attn_int4(const char* fn, Int4AttnParams p, int d, void* scratch, long long 
   }
 }
 
-// Chunks from this many rows on go through the tensor-core prefill kernels, which read an 8-bit pool.
-constexpr int kWidenRows = 32;
-bool widens(int rows, int Hq, int Hk, int d) { return rows >= kWidenRows && d == 128 && Hq == 4 * Hk; }
+// Which chunks go through the kernels for an 8-bit pool. Measured (32 / 8 heads of 128), decode form and widened, us: 64
+// rows after 0 positions 8 and 16, after 500 13 and 21, after 1203 23 and 22, after 16000 88 and 58; 192 rows after 0
+// positions 12 and 19, after 1203 29 and 27; 256 rows after 500 42 and 24; 48 rows after 0 positions 8 and 6, after 500
+// 13 and 23, after 16000 71 and 534 (below 64 rows those kernels walk the cache in one piece).
+bool widens(int rows, int base_pos, int Hq, int Hk, int d) {
+  if (rows < 32 || d != 128 || Hq != 4 * Hk) return false;
+  return rows < 64 ? base_pos <= 192 - rows : rows > 192 || base_pos > 768 - rows;
+}
 int prefill_group(int Hq, int Hk) { return std::max(1, 16 / (Hq / Hk)); }
 long long widened_bytes(long long n, int Hk) { return (2 * n * Hk * (128 + 4) + 63) / 16 * 16; }
 
@@ -836,7 +874,7 @@ int granite4_kernel_attn_decode_int4_paged(const uint16_t* d_q, const uint8_t* d
 
 long long granite4_prefill_attention_int4_scratch_bytes(int rows, int base_pos, int Hq, int Hk, int d) {
   if (rows <= 0 || base_pos < 0 || base_pos > INT_MAX - rows || !g4::int4_shape_ok(Hq, Hk, d, 1)) return -1;
-  if (g4::widens(rows, Hq, Hk, d)) return g4::widened_bytes(static_cast<long long>(base_pos) + rows, Hk);
+  if (g4::widens(rows, base_pos, Hq, Hk, d)) return g4::widened_bytes(static_cast<long long>(base_pos) + rows, Hk);
   return g4::plan_int4(rows, g4::prefill_group(Hq, Hk), Hq, Hk, d, base_pos + rows).bytes;
 }
 
@@ -854,7 +892,7 @@ int granite4_prefill_attention_int4(const uint16_t* d_q_rot, float scale, int Hq
   if (!g4::aligned16(d_q_rot) || !g4::aligned16(d_cache_k) || !g4::aligned16(d_cache_v))
     return g4::fail(fn, "q and the caches must be 16-byte aligned");
   const int n = base_pos + rows;
-  if (g4::widens(rows, Hq, Hk, d)) {
+  if (g4::widens(rows, base_pos, Hq, Hk, d)) {
     if (d_scratch == nullptr || !g4::aligned16(d_scratch) || scratch_bytes < g4::widened_bytes(n, Hk))
       return g4::fail(fn, "scratch missing, misaligned or smaller than the size the scratch query returns");
     const size_t codes = static_cast<size_t>(n) * Hk * 128, scales = static_cast<size_t>(n) * Hk;

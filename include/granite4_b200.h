@@ -553,11 +553,12 @@ int granite4_kernel_attn_decode_int4_paged(const uint16_t* d_q, const uint8_t* d
                                            int rows_per_group, int Hq, int Hk, int d, int stride,
                                            int max_len, int window, float scale, void* d_scratch,
                                            long long scratch_bytes, uint16_t* d_out);
-/* Added: granite4_prefill_attention_int8 over the 4-bit pool. Chunks of 32 rows or more
- * with d 128 and Hq == 4 Hk widen the sequence's rows into an 8-bit pool in d_scratch
- * (exact: a 4-bit code is an 8-bit code with the same scale; 264 bytes per position and kv
- * head) and run the kernels of that entry point; everything else runs on the decode
- * kernel, where d_scratch is optional (without it no range is split). d_scratch must hold
+/* Added: granite4_prefill_attention_int8 over the 4-bit pool. With d 128 and Hq == 4 Hk,
+ * chunks of 64 rows or more (at the start of a sequence: of over 192, or of 32 to 63)
+ * widen the sequence's rows into an 8-bit pool in d_scratch (exact: a 4-bit code is an
+ * 8-bit code with the same scale; 264 bytes per position and kv head) and run the kernels
+ * of that entry point; everything else runs on the decode kernel, where d_scratch is
+ * optional (without it no range is split). d_scratch must hold
  * granite4_prefill_attention_int4_scratch_bytes(...) bytes, 16-byte aligned. */
 long long granite4_prefill_attention_int4_scratch_bytes(int rows, int base_pos, int Hq, int Hk, int d);
 int granite4_prefill_attention_int4(const uint16_t* d_q_rot, float scale, int Hq, int Hk, int d,

@@ -369,7 +369,8 @@ def test_output_between_two_words_and_other_streams(K):
     assert torch.equal(odd, want)
 
 
-@pytest.mark.parametrize("rows,base", [(1, 0), (1, 77), (5, 1000), (31, 3), (32, 0), (33, 100), (77, 1203), (130, 5), (600, 2000)])
+@pytest.mark.parametrize("rows,base", [(1, 0), (1, 77), (5, 1000), (31, 3), (32, 0), (33, 100), (63, 129), (63, 130), (64, 704), (64, 705),
+                                       (77, 1203), (130, 5), (192, 3), (193, 3), (600, 2000)])
 @pytest.mark.parametrize("Hq,Hk,d", [(32, 8, 128), (16, 2, 64), (6, 6, 128)])
 def test_prefill_chunks(K, rows, base, Hq, Hk, d):
     g = gen(rows + base)
