@@ -27,11 +27,13 @@
 // moves only when it is passed by 4 (in powers of two): P is at most 16, v_scale 2^11, fp16 ends at 2^16, and most tiles
 // leave the accumulators as they are.
 //
-// Work split: the (group, kv head, column block) segments' tiles of 32 positions form one line, cut into equal
-// shares, one CTA each, whatever the sequences' lengths (read on the device). A CTA's four warps take every fourth
-// tile of a segment's piece, each with its own ring of asynchronous copies and its own running (max, sum, O); they
-// merge in shared memory. Pieces of a
-// segment that more than one CTA worked on are joined by a second small kernel, in order of the CTAs.
+// Work split, by size: a (group, kv head, column block) segment is one CTA's; or a cluster's, whose CTAs take equal parts
+// and join them through distributed shared memory; or, for long caches, the segments' tiles of 32 positions form one line,
+// cut into equal shares, one CTA each, whatever the sequences' lengths (read on the device), and pieces of a segment that
+// more than one CTA worked on are joined by a second small kernel, in order of the CTAs. A CTA's four warps take every
+// fourth tile of a piece, each with its own ring of asynchronous copies and its own running (max, sum, O); they merge in
+// shared memory.
+#include "g4_cluster.cuh"
 #include "g4_host.h"
 #include "g4_math.cuh"
 
@@ -76,7 +78,8 @@ struct Int4AttnParams {
   long long stride;
   int max_len, window;
   float scale_log2;
-  int split;  // the line of tiles is cut into gridDim.x shares (0: a CTA per segment)
+  int split;    // the line of tiles is cut into gridDim.x shares
+  int cluster;  // else: CTAs of a segment, a cluster (1: one CTA)
 };
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -209,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
   static_assert(kWarpBytes<D> >= kC * (D + kPad) * 4 + kC * 8, "a warp parks its state in its ring");
   __shared__ __align__(16) unsigned char s_q[8 * NS][D + 16];  // a row per column of the logit tiles
   __shared__ float s_scale[4 * NS];                            // of a pair's logits
+  __shared__ float2 s_cta[4 * NS];                             // (max, sum) of the CTA, where it is one of a cluster
   extern __shared__ __align__(128) unsigned char s_ring[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   unsigned char* const ring = s_ring + warp * kWarpBytes<D>;
@@ -283,7 +287,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
         pt = reinterpret_cast<const int*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(lane_pt), owner));
       }
     } else {
-      grp = blockIdx.x / per_group, sub = blockIdx.x - grp * per_group;
+      const int segment = p.cluster == 1 ? blockIdx.x : blockIdx.x / p.cluster;
+      grp = segment / per_group, sub = segment - grp * per_group;
       piece_begin = 0, piece_end = 1;
     }
     if (!p.split || lane_groups > 1) {
@@ -308,7 +313,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     first_tile = span_hi < 0 ? 0 : span_lo / kTile;
     n_tiles = span_hi < 0 ? 0 : span_hi / kTile - first_tile + 1;
     if (!p.split) {
-      piece_end = n_tiles;
+      const int rank = p.cluster == 1 ? 0 : blockIdx.x % p.cluster;
+      piece_begin = p.cluster == 1 ? 0 : rank * n_tiles / p.cluster, piece_end = p.cluster == 1 ? n_tiles : (rank + 1) * n_tiles / p.cluster;
     } else if (chunk > 0) {
       const int k = piece_begin, n = piece_end;
       piece_begin = quotient(k * n_tiles, n), piece_end = quotient((k + 1) * n_tiles, n);
@@ -579,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     }
 
     // the four warps' states meet in shared memory, each parked in the warp's own ring
-    if (p.split) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __syncwarp();
     float* const park = reinterpret_cast<float*>(ring);  // [kC][D + kPad], then [kC][2] (max, sum)
     const float back = 16777216.0f / v_mult;
@@ -614,7 +620,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
         const float f = mw[w] == -INFINITY ? 0.0f : exp2_fast(mw[w] - m);
         l += f * parked[kC * (D + kPad) + 2 * c + 1], acc += f * parked[c * (D + kPad) + dim];
       }
-      if (whole) {
+      if (p.cluster > 1) {  // (each value of warp 0's state is read by this thread alone)
+        reinterpret_cast<float*>(s_ring)[c * (D + kPad) + dim] = acc;
+        if (dim == 0) s_cta[c] = make_float2(m, l);
+      } else if (whole) {
         const int j = (c0 + c) * p.g_inv >> 16, hl = c0 + c - j * p.G;
         p.out[(static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + dim] =
             static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? __fdividef(acc, l) : 0.0f));
@@ -622,6 +631,46 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
         p.part_o[(slot * kC + c) * D + dim] = acc;
         if (dim == 0) p.part_ml[(slot * kC + c) * 2] = m, p.part_ml[(slot * kC + c) * 2 + 1] = l;
       }
+    }
+    if (p.cluster > 1) {
+      // the cluster's CTAs share the outputs out: each adds every CTA's part of its own
+      namespace cg = cooperative_groups;
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      const int rank = blockIdx.x % p.cluster;
+      for (int i = rank * kThreads + threadIdx.x; i < columns * D; i += p.cluster * kThreads) {
+        const int c = i / D, at = c * (D + kPad) + i % D;
+        float m = -INFINITY, l = 0.0f, acc = 0.0f;
+#pragma unroll 1
+        for (int r0_ = 0; r0_ < p.cluster; r0_ += 8) {
+          float2 ml[8];
+          float v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            ml[u] = make_float2(-INFINITY, 0.0f), v[u] = 0.0f;
+            if (r0_ + u < p.cluster) {
+              ml[u] = *cluster.map_shared_rank(s_cta + c, r0_ + u);
+              v[u] = *cluster.map_shared_rank(reinterpret_cast<const float*>(s_ring) + at, r0_ + u);
+            }
+          }
+          float top = m;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) top = fmaxf(top, ml[u].x);
+          if (top == -INFINITY) continue;
+          const float keep = exp2_fast(m - top);
+          l *= keep, acc *= keep, m = top;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const float f = exp2_fast(ml[u].x - top);
+            l += f * ml[u].y, acc += f * v[u];
+          }
+        }
+        const int j = (c0 + c) * p.g_inv >> 16, hl = c0 + c - j * p.G;
+        p.out[(static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + i % D] =
+            static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? __fdividef(acc, l) : 0.0f));
+      }
+      cluster.sync();  // nobody leaves while its memory is read
+      return;
     }
     if (!p.split) return;
     __syncthreads();
@@ -737,10 +786,10 @@ __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4Attn
   }
 }
 
-// How a launch is cut: `shares` CTAs over the line of tiles, or a CTA per segment (shares 0).
+// How a launch is cut: `shares` CTAs over the line of tiles, or (shares 0) `cluster` CTAs per segment.
 struct Int4Plan {
-  int ns, blocks, groups, shares;
-  long long segments, bytes;
+  int ns, blocks, groups, shares, cluster;
+  long long segments;
 };
 
 Int4Plan plan_int4(int rows, int per, int Hq, int Hk, int d, int max_len) {
@@ -750,22 +799,36 @@ Int4Plan plan_int4(int rows, int per, int Hq, int Hk, int d, int max_len) {
   s.blocks = (columns + 4 * s.ns - 1) / (4 * s.ns);
   s.groups = (rows + per - 1) / per;
   s.segments = static_cast<long long>(s.groups) * Hk * s.blocks;
+  s.cluster = 1;
+  if (s.segments > kMaxQuotient || max_len <= kTile * kWarps) return s;
   const long long resident = std::min(static_cast<long long>(ctas_per_sm(s.ns)) * sm_count(), static_cast<long long>(kMaxShares));
-  if (s.groups > kMaxGroups || s.segments > kMaxQuotient) return s;
   const long long per_segment = (max_len + kTile - 1) / kTile, tiles = s.segments * per_segment;
-  if (tiles > INT_MAX / 2 || static_cast<long long>(s.groups) * per_segment >= kMaxQuotient ||
+  // Costs in ns, fitted to measured calls (segments of 7 - 4096 tiles, 2 - 512 of them; within 15 % but for a few): a CTA
+  // starts and ends in 4 us; its four warps take a tile in 0.2 us, in twice that with the card full, more with more columns,
+  // less with narrow heads. A cluster's join costs 1.6 us; clusters leave an SM's last places empty here and there, those
+  // of more than eight CTAs a quarter of the card. The line cut: a start for every segment that a CTA meets, an equal share
+  // of the tiles (sequences are seldom all as long as the longest), 4.5 us for the join.
+  // 64 segments of 129 tiles: clusters 12 us, cut 14. 32 of 375: 21 (clusters of 13) and 15. 40 of 47: 9 and 12.
+  const auto tile_ns = [&](long long ctas) {
+    return (200 + 225 * std::min(ctas, resident) / resident) * (3 + s.ns) / 4 * (d == 128 ? 8 : 5) / 8;
+  };
+  const auto by_segment = [&](long long n) {
+    const long long ctas = s.segments * n, room = n == 1 ? resident : n <= 8 ? resident * 15 / 16 : resident * 3 / 4;
+    return (ctas + room - 1) / room * (4000 + (per_segment + n - 1) / n * tile_ns(ctas)) + (n == 1 ? 0 : n <= 8 ? 1600 : 1900);
+  };
+  long long best = by_segment(1);
+  if (cluster_enabled())
+    for (int n = 2; n <= kMaxClusterCtas; ++n)
+      if (by_segment(n) < best) best = by_segment(n), s.cluster = n;
+  const long long cut = 4000 + 3500 * s.segments / resident + tiles * tile_ns(resident) / resident * 7 / 8 + 4500;
+  if (cut >= best || s.groups > kMaxGroups || tiles > INT_MAX / 2 || static_cast<long long>(s.groups) * per_segment >= kMaxQuotient ||
       tiles / resident >= kMaxQuotient)
     return s;
-  // Two costs in ns. A CTA per segment: waves of a start (5 us) and a quarter of the segment's tiles for each warp, 1.7 us
-  // a tile with the card full. The line cut: a start for every segment that a CTA meets, an equal share of the tiles, the
-  // join (6 us). Measured, 8 rows x 4 heads a group, 192 rows of 192 positions: 8 and 59 us; 16 sessions of 24000: 330 and 64.
-  const long long whole = (s.segments + resident - 1) / resident * (5000 + per_segment * 425);
-  const long long cut = 5000 + 5000 * s.segments / resident + tiles * 425 / resident + 6000;
-  if (max_len <= kTile * kWarps || whole <= cut) return s;
   s.shares = static_cast<int>(std::min(resident, std::max(1ll, tiles / kWarps)));
-  const long long slots = s.shares + s.segments;
-  s.bytes = slots * 4 * s.ns * (d + 2) * 4 + (s.groups + 2 + 3) / 4 * 16;
   return s;
+}
+long long plan_bytes(const Int4Plan& s, int d) {
+  return s.shares == 0 ? 0 : (s.shares + s.segments) * 4 * s.ns * (d + 2) * 4 + (s.groups + 2 + 3) / 4 * 16;
 }
 
 bool int4_shape_ok(int Hq, int Hk, int d, int per) {
@@ -777,18 +840,30 @@ template <int D, int NS>
 int launch_int4(const char* fn, const Int4AttnParams& p, const Int4Plan& s) {
   const cudaStream_t st = current_stream();
   if (s.segments > INT_MAX) return fail(fn, "too many rows");
-  const unsigned ctas = static_cast<unsigned>(p.split ? s.shares : s.segments);
   constexpr int smem = kWarps * kWarpBytes<D>;
-  if (smem > 48 * 1024) {
-    static std::atomic<bool> attr_set[64];  // per device; relaxed: setting the attribute twice is harmless
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess) return fail(fn, "cannot identify the current device");
-    if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_relaxed)) {
-      G4_CUDA_TRY(fn, cudaFuncSetAttribute(attn_int4_kernel<D, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-      if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_relaxed);
+  static_assert(smem <= 48 * 1024, "no opt-in needed");
+  if (p.cluster > 1) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(s.segments * p.cluster)), cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(p.cluster), attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    void (*const kernel)(const Int4AttnParams) = attn_int4_kernel<D, NS>;
+    if (cluster_fits(reinterpret_cast<const void*>(kernel), cfg, p.cluster, kThreads)) {
+      cfg.numAttrs = pdl_enabled() ? 2 : 1;
+      G4_CUDA_TRY(fn, cudaLaunchKernelEx(&cfg, kernel, p));
+      return 0;
     }
+    Int4AttnParams one = p;  // a device that cannot place such a cluster
+    one.cluster = 1;
+    G4_LAUNCH_PDL(fn, kernel, dim3(static_cast<unsigned>(s.segments)), dim3(kThreads), smem, st, one);
+    return 0;
   }
-  G4_LAUNCH_PDL(fn, (attn_int4_kernel<D, NS>), dim3(ctas), dim3(kThreads), smem, st, p);
+  G4_LAUNCH_PDL(fn, (attn_int4_kernel<D, NS>), dim3(static_cast<unsigned>(p.split ? s.shares : s.segments)), dim3(kThreads), smem, st, p);
   if (p.split) {
     const unsigned segments = static_cast<unsigned>(s.segments), columns = static_cast<unsigned>(std::min(4 * NS, p.per * p.G));
     if (s.segments * columns <= 2ll * sm_count())
@@ -803,13 +878,18 @@ int launch_int4(const char* fn, const Int4AttnParams& p, const Int4Plan& s) {
 int attn_int4(const char* fn, Int4AttnParams p, int d, void* scratch, long long scratch_bytes, bool scratch_needed) {
   p.G = p.Hq / p.Hk;
   Int4Plan s = plan_int4(p.rows, p.per, p.Hq, p.Hk, d, p.max_len);
+  if (p.window > 0 && p.window < p.max_len - kTile) {  // what a window leaves may want no cut
+    const Int4Plan w = plan_int4(p.rows, p.per, p.Hq, p.Hk, d, p.window + kTile);
+    if (w.shares == 0) s = w;
+  }
   p.blocks = s.blocks, p.groups = s.groups;
   p.g_inv = (65536u + p.G - 1) / p.G;
-  const bool have = scratch != nullptr && scratch_bytes >= s.bytes && aligned16(scratch);
+  const bool have = scratch != nullptr && scratch_bytes >= plan_bytes(s, d) && aligned16(scratch);
   if (s.shares > 0 && !have) {
     if (scratch_needed) return fail(fn, "scratch missing, misaligned or smaller than the size the scratch query returns");
     s.shares = 0;
   }
+  p.cluster = s.shares > 0 ? 1 : s.cluster;
   p.split = s.shares > 0;
   if (p.split) {
     p.part_o = static_cast<float*>(scratch);
@@ -847,7 +927,7 @@ extern "C" {
 
 long long granite4_attn_decode_int4_scratch_bytes(int rows, int rows_per_group, int Hq, int Hk, int d, int max_len) {
   if (rows <= 0 || max_len <= 0 || !g4::int4_shape_ok(Hq, Hk, d, rows_per_group)) return -1;
-  return g4::plan_int4(rows, rows_per_group, Hq, Hk, d, max_len).bytes;
+  return g4::plan_bytes(g4::plan_int4(rows, rows_per_group, Hq, Hk, d, max_len), d);
 }
 
 int granite4_kernel_attn_decode_int4_paged(const uint16_t* d_q, const uint8_t* d_cache_k, const uint8_t* d_cache_v,
@@ -875,7 +955,7 @@ int granite4_kernel_attn_decode_int4_paged(const uint16_t* d_q, const uint8_t* d
 long long granite4_prefill_attention_int4_scratch_bytes(int rows, int base_pos, int Hq, int Hk, int d) {
   if (rows <= 0 || base_pos < 0 || base_pos > INT_MAX - rows || !g4::int4_shape_ok(Hq, Hk, d, 1)) return -1;
   if (g4::widens(rows, base_pos, Hq, Hk, d)) return g4::widened_bytes(static_cast<long long>(base_pos) + rows, Hk);
-  return g4::plan_int4(rows, g4::prefill_group(Hq, Hk), Hq, Hk, d, base_pos + rows).bytes;
+  return g4::plan_bytes(g4::plan_int4(rows, g4::prefill_group(Hq, Hk), Hq, Hk, d, base_pos + rows), d);
 }
 
 int granite4_prefill_attention_int4(const uint16_t* d_q_rot, float scale, int Hq, int Hk, int d, int base_pos, int rows,

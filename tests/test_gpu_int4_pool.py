@@ -308,6 +308,16 @@ def test_many_sequences(K, seqs, ctx):
     run_attention(K, seqs, 1, ctxs, 8, 2, 64, empty=(3,), max_len=ctx)
 
 
+@pytest.mark.parametrize("Hq,Hk,d", HEADS)
+def test_forms_agree(K, monkeypatch, Hq, Hk, d):
+    """A segment by one cluster, or with clusters off by shares of the line or one CTA: each within the bound."""
+    for seqs, per, ctxs in ((2, 1, [3000, 1]), (5, 1, [700, 33, 1500, 900, 64]), (1, 1, [260])):
+        for off in ("0", "1"):
+            monkeypatch.setenv("G4_CLUSTER", off)
+            run_attention(K, seqs, per, ctxs, Hq, Hk, d, empty=(1,) if seqs > 1 else (), scratch="poisoned", seed=3)
+            run_attention(K, seqs, per, ctxs, Hq, Hk, d, max_len=20000, scratch="poisoned", seed=4)
+
+
 def test_long_cache_of_one_kv_head(K):
     run_attention(K, 1, 1, [120000], 16, 1, 128, scratch="poisoned", sigma=0.5)
     run_attention(K, 2, 2, [60001, 3], 8, 4, 64, scratch="poisoned", sigma=0.5)

@@ -44,8 +44,8 @@ def test_read_refusals(lib, bad, capfd):
 
 
 def decode(lib, **kw):
-    a = dict(q=16, ck=16, cv=16, ks=16, vs=16, pos=16, row_pt=None, pt=None, rows=2, per=1, Hq=32, Hk=8, d=128, stride=4096,
-             max_len=4096, window=0, scale=0.1, scratch=None, bytes=0, out=16)
+    a = dict(q=16, ck=16, cv=16, ks=16, vs=16, pos=16, row_pt=None, pt=None, rows=2, per=1, Hq=32, Hk=8, d=128, stride=131072,
+             max_len=131072, window=0, scale=0.1, scratch=None, bytes=0, out=16)
     a.update(kw)
     return lib.granite4_kernel_attn_decode_int4_paged(*a.values())
 
@@ -53,7 +53,7 @@ def decode(lib, **kw):
 @pytest.mark.parametrize("bad", [
     {"q": None}, {"ck": None}, {"cv": None}, {"ks": None}, {"vs": None}, {"pos": None}, {"out": None}, {"rows": 0},
     {"per": 0}, {"per": 17}, {"Hq": 33}, {"Hk": 0}, {"Hq": 0}, {"Hq": 1040}, {"d": 96}, {"stride": 0}, {"max_len": 0},
-    {"max_len": 5000}, {"window": -1}, {"scale": float("nan")}, {"q": 18}, {"ck": 24}, {"cv": 8},
+    {"max_len": 131073}, {"window": -1}, {"scale": float("nan")}, {"q": 18}, {"ck": 24}, {"cv": 8},
     {},  # a scratch is wanted at this length
     {"scratch": 24, "bytes": 1 << 30}, {"scratch": 16, "bytes": 64}])
 def test_decode_refusals(lib, bad, capfd):
@@ -63,8 +63,9 @@ def test_decode_refusals(lib, bad, capfd):
 
 def test_scratch_sizes(lib):
     size = lib.granite4_attn_decode_int4_scratch_bytes
-    assert size(1, 1, 32, 8, 128, 4096) > 0
+    assert size(1, 1, 32, 8, 128, 131072) > 0
     assert size(1, 1, 32, 8, 128, 128) == 0  # one tile a warp: nothing is split
+    assert size(1, 1, 32, 8, 128, 4096) == 0  # a cluster per kv head
     assert size(1, 1, 33, 8, 128, 4096) == -1 and size(0, 1, 32, 8, 128, 4096) == -1
     assert size(1, 1, 32, 8, 96, 4096) == -1 and size(1, 1, 32, 8, 128, 0) == -1 and size(4, 17, 32, 8, 128, 64) == -1
     assert size(1 << 30, 4, 32, 8, 128, 1 << 30) >= 0
