@@ -105,7 +105,17 @@ T* ptr(PyObject* o, Types types = kAny) {
   return static_cast<T*>(t.data_ptr());
 }
 
-// The same of a tensor on `dev` that holds at least n elements (n < 0: of sizes the launcher refuses).
+// A tensor whose first dimension is an entry point's rows.
+const at::Tensor& rows_of(PyObject* o) {
+  const at::Tensor& t = tensor(o);
+  if (t.dim() < 2) {
+    PyErr_Format(PyExc_ValueError, "expected rows, got a tensor of %d dimensions", static_cast<int>(t.dim()));
+    throw PyErrorSet{};
+  }
+  return t;
+}
+
+// ptr() of a tensor on `dev` that holds at least n elements (n < 0: of sizes the launcher refuses).
 template <typename T = void>
 T* ptr_of(PyObject* o, Types types, c10::Device dev, long long n, const char* what) {
   T* p = ptr<T>(o, types);
@@ -432,7 +442,7 @@ OP(rope_kv_int8_paged, 16) {  // qkv, cos, sin, pos_rows, kv_rows, Hq, Hk, d, st
 
 OP(qk_norm_rope_kv_paged, 19) {
   // qkv, q_norm, k_norm, eps, cos, sin, pos_rows, kv_rows, Hq, Hk, d, stride, max_pos, bits, q_rot, ck, cv, ks, vs
-  const at::Tensor& t = matrix(a[0]);
+  const at::Tensor& t = rows_of(a[0]);
   enter(t);
   const auto dev = t.device();
   const long long rows = t.size(0), Hq = num(a[8]), Hk = num(a[9]), d = num(a[10]), stride = num(a[11]), max_pos = num(a[12]);
@@ -604,7 +614,7 @@ OP(prefill_attention_int8, 14) {  // q_rot, scale, Hq, Hk, d, base_pos, stride, 
 
 OP(attn_decode_int4_paged, 18) {
   // q, ck, cv, ks, vs, row_pos, Hq, Hk, d, stride, max_len, scale, out, rows_per_group, row_pt, pt, window, scratch
-  const at::Tensor& t = matrix(a[0]);
+  const at::Tensor& t = rows_of(a[0]);
   enter(t);
   const auto dev = t.device();
   const long long rows = t.size(0), Hq = num(a[6]), Hk = num(a[7]), d = num(a[8]), stride = num(a[9]);
@@ -618,7 +628,7 @@ OP(attn_decode_int4_paged, 18) {
   const auto* pos = ptr_of<const int>(a[5], kI32, dev, rows, "row_pos");
   auto* out = ptr_of<uint16_t>(a[12], kBf16, dev, rows * Hq * d, "out");
   const auto* row_pt = reinterpret_cast<const int* const*>(ptr_of<const int64_t>(a[14], kI64, dev, rows, "row_pt"));
-  const auto* pt = ptr_of<const int>(a[15], kI32, dev, max_len, "pt");
+  const auto* pt = ptr_of<const int>(a[15], kI32, dev, 0, "pt");  // read as far as a row sees
   void* scr = ptr_of(a[17], kU8, dev, 0, "scratch");
   const long long bytes = a[17] == Py_None ? 0 : tensor(a[17]).numel();
   return launched([&] {
@@ -629,7 +639,7 @@ OP(attn_decode_int4_paged, 18) {
 }
 
 OP(prefill_attention_int4, 14) {  // q_rot, scale, Hq, Hk, d, base_pos, stride, out, ck, cv, ks, vs, pt, scratch
-  const at::Tensor& t = matrix(a[0]);
+  const at::Tensor& t = rows_of(a[0]);
   enter(t);
   const auto dev = t.device();
   const float scale = real(a[1]);

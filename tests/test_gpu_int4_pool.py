@@ -85,7 +85,7 @@ class Pool:
 
 
 @pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("norm", ["both", "k", "none"])
+@pytest.mark.parametrize("norm", ["both", "q", "k", "none"])
 @pytest.mark.parametrize("rows,Hq,Hk,d", [(1, 32, 8, 128), (3, 4, 4, 64), (16, 32, 8, 128), (17, 5, 1, 128), (37, 16, 2, 64),
                                           (500, 32, 8, 128), (2500, 24, 8, 64), (1003, 40, 16, 128)])
 def test_write_equals_the_formula(K, rows, Hq, Hk, d, norm, bits):
@@ -96,7 +96,7 @@ def test_write_equals_the_formula(K, rows, Hq, Hk, d, norm, bits):
     qkv.view(rows, -1, d)[rows // 2, -1] = 0  # a value head of zeros
     qkv.view(rows, -1, d)[rows // 3, Hq] = 0  # a key head of zeros
     wq, wk = ((1 + 0.3 * torch.randn(d, generator=g, device=DEV)).to(torch.bfloat16) for _ in range(2))
-    wq, wk = (wq if norm == "both" else None), (wk if norm != "none" else None)
+    wq, wk = (wq if norm in ("both", "q") else None), (wk if norm in ("both", "k") else None)
     cos, sin = tables(max_pos, d)
     pos = torch.randint(0, max_pos, (rows,), generator=g, device=DEV, dtype=torch.int32)
     kvr = torch.randperm(stride, generator=g, device=DEV)[:rows].to(torch.int32)
@@ -403,6 +403,94 @@ def test_prefill_chunks(K, rows, base, Hq, Hk, d):
         tol = 0.01 + 2.0**-8 * want.abs()
     assert ((out[pick.to(DEV)].double().view(-1, Hq, d) - want).abs() <= tol).all()
     assert (out[rows] == 3.0).all() and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("Hq,Hk,d,per", [(32, 8, 128, 4), (16, 2, 64, 3), (8, 8, 64, 7), (32, 8, 128, 16)])
+@pytest.mark.parametrize("window", [0, 90])
+def test_rows_of_a_group_at_any_positions(K, Hq, Hk, d, per, window):
+    """Rows of one sequence in no order, the same position twice, idle rows among them, a last group that is not full."""
+    g = gen(per + window)
+    n, rows = 900, 2 * per + 1
+    p, codes = random_pool(n, Hk, d, g)
+    tab = torch.randperm(n, generator=g, device=DEV).to(torch.int32)
+    pos = torch.randint(0, n, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    pos[1], pos[2], pos[per] = -1, pos[0], -7
+    q = torch.randn(rows, Hq, d, generator=g, device=DEV).to(torch.bfloat16)
+    out = torch.full((rows, Hq, d), 3.0, dtype=torch.bfloat16, device=DEV)
+    assert K.attn_decode_int4_paged(q, *p.all, pos, Hq, Hk, d, n, n, 0.03, out, rows_per_group=per, pt=tab, window=window) == 0
+    want, tol = attention64(q.view(rows, -1), p, codes, [tab] * 3, pos, per, Hq, Hk, d, 0.03, window, 64)
+    assert ((out.double() - want).abs() <= tol).all()
+    assert (out[1] == 0).all() and (out[per] == 0).all()
+
+
+def test_offsets_past_32_bits(K):
+    """A pool whose codes, and whose byte offsets within a head's rows, pass 2^31: rows at its ends written, read, attended to."""
+    Hq, Hk, d, rows, max_pos = 8, 2, 128, 40, 64
+    stride = (1 << 31) // (d // 2) + 1000  # a head's codes alone are over 2 GiB
+    g = gen(9)
+    p = Pool(stride, Hk, d, 4, fill=0x88)
+    qkv = torch.randn(rows, (Hq + 2 * Hk) * d, generator=g, device=DEV).to(torch.bfloat16)
+    cos, sin = tables(max_pos, d)
+    pos = torch.arange(rows, dtype=torch.int32, device=DEV)
+    kvr = torch.cat((torch.arange(rows // 2, device=DEV), stride - 1 - torch.arange(rows - rows // 2, device=DEV))).to(torch.int32)
+    q_rot = torch.empty(rows, Hq * d, dtype=torch.bfloat16, device=DEV)
+    assert K.qk_norm_rope_kv_paged(qkv, None, None, EPS, cos, sin, pos, kvr, Hq, Hk, d, stride, max_pos, 4, q_rot, *p.all) == 0
+    _, ck, sk, cv, sv = write64(qkv, None, None, cos, sin, pos, Hq, Hk, d, 4)
+    ko, vo = (torch.empty(rows, Hk, d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    assert K.kv_read_paged(*p.all, kvr, 4, Hk, d, stride, ko, vo) == 0
+    assert torch.equal(ko, (ck.float() * sk[..., None]).to(torch.bfloat16))
+    assert torch.equal(vo, (cv.float() * sv[..., None]).to(torch.bfloat16))
+    last = torch.tensor([rows - 1], dtype=torch.int32, device=DEV)
+    small = Pool(rows, Hk, d, 4)
+    at = torch.arange(rows, dtype=torch.int32, device=DEV)
+    for t, s in zip(small.all, p.all):
+        t.copy_(s[:, kvr.long()])
+    out, want = (torch.empty(1, Hq * d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    assert K.attn_decode_int4_paged(q_rot[-1:], *p.all, last, Hq, Hk, d, stride, rows, 0.05, out, pt=kvr) == 0
+    assert K.attn_decode_int4_paged(q_rot[-1:], *small.all, last, Hq, Hk, d, rows, rows, 0.05, want, pt=at) == 0
+    assert torch.equal(out, want)
+    chunk = torch.empty(rows, Hq * d, dtype=torch.bfloat16, device=DEV)
+    assert K.prefill_attention_int4(q_rot, 0.05, Hq, Hk, d, 0, stride, chunk, *p.all, pt=kvr) == 0
+    ref = torch.empty_like(chunk)
+    assert K.prefill_attention_int4(q_rot, 0.05, Hq, Hk, d, 0, rows, ref, *small.all, pt=at) == 0
+    assert torch.equal(chunk, ref)
+
+
+def test_tensors_too_small_or_of_other_kinds_are_refused(K):
+    Hq, Hk, d, n = 8, 2, 128, 64
+    p, _ = random_pool(n, Hk, d, gen(1))
+    q = torch.zeros(2, Hq * d, dtype=torch.bfloat16, device=DEV)
+    pos = torch.zeros(2, dtype=torch.int32, device=DEV)
+    def call(**kw):
+        a = dict(q=q, ck=p.ck, cv=p.cv, ks=p.ks, vs=p.vs, pos=pos, out=torch.empty_like(q))
+        a.update(kw)
+        return K.attn_decode_int4_paged(a["q"], a["ck"], a["cv"], a["ks"], a["vs"], a["pos"], Hq, Hk, d, n, n, 0.1, a["out"])
+    assert call() == 0
+    for bad in ({"ck": p.ck[:1]}, {"ks": p.ks[:, :-1].contiguous()}, {"pos": pos[:1]}, {"out": q[:1].clone()}, {"q": q[:, ::2]},
+                {"vs": p.vs.cpu()}, {"cv": p.cv[:, :, ::2]}):
+        with pytest.raises(ValueError):
+            call(**bad)
+    for bad in ({"ck": p.ck.view(torch.int8)}, {"pos": pos.long()}, {"q": q.float()}, {"ks": p.ks.double()}):
+        with pytest.raises(TypeError):
+            call(**bad)
+    cos, sin = tables(16, d)
+    qkv = torch.zeros(2, (Hq + 2 * Hk) * d, dtype=torch.bfloat16, device=DEV)
+    def write(**kw):
+        a = dict(qkv=qkv, w=None, cos=cos, kvr=pos, q=torch.empty_like(q), ck=p.ck)
+        a.update(kw)
+        return K.qk_norm_rope_kv_paged(a["qkv"], a["w"], None, EPS, a["cos"], sin, pos, a["kvr"], Hq, Hk, d, n, 16, 4, a["q"],
+                                       a["ck"], p.cv, p.ks, p.vs)
+    for bad in ({"qkv": qkv[:, :-8].contiguous()}, {"w": qkv[0, : d - 1].clone()}, {"cos": cos[:8]}, {"kvr": pos[:1]},
+                {"q": q[:1].clone()}, {"ck": p.ck[:, :-1].contiguous()}):
+        with pytest.raises(ValueError):
+            write(**bad)
+    with pytest.raises(TypeError):
+        write(ck=p.ck.view(torch.int8))
+    ko = torch.empty(2, Hk, d, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError):
+        K.kv_read_paged(*p.all, pos, 4, Hk, d, n, ko, ko[:1])
+    with pytest.raises(ValueError):
+        K.prefill_attention_int4(q, 0.1, Hq, Hk, d, 5, n, torch.empty_like(q), *p.all, pt=pos)
 
 
 def test_repeats_to_the_bit(K):
