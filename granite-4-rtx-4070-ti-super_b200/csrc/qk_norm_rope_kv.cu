@@ -126,9 +126,8 @@ __device__ __noinline__ double2 key_pair(const uint16_t* a, const uint16_t* b, c
   return make_double2(x * cd - y * sd, y * cd + x * sd);
 }
 
-__device__ __forceinline__ void copy16_async(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src)
-               : "memory");
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -144,7 +143,8 @@ __device__ __forceinline__ void copies_wait() {
 // their way by asynchronous copies into slots of its own, so nothing is synchronised. Arithmetic is on pairs of f32 where
 // it can be. What bounds the kernel is memory, 22 KB a row of 48 heads in and out, and close behind it the issue slots.
 constexpr int kQkDepth = 4, kQkCtas = 6;
-template <int D, int BITS>
+// WHOLE: query heads and key / value heads fill their items, so the items of all rows lie one behind the other in qkv.
+template <int D, int BITS, bool WHOLE>
 __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(const QkNormParams p, int q_parts, int per_row, int run, int longer) {
   pdl_begin();
   constexpr int kLanes = D / 16, kHeads = 32 / kLanes, kTop = BITS == 4 ? 7 : 127;
@@ -157,20 +157,30 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
   const int begin = warp * run + min(warp, longer), end = begin + run + (warp < longer ? 1 : 0);
   if (begin >= end) return;
   int row = begin / per_row, part = begin - row * per_row, f_left = end - begin, f_part = part;
-  int f_slot = 0, slot = 0;
-  const uint4* f_row = reinterpret_cast<const uint4*>(p.qkv) + static_cast<size_t>(row) * heads * (D / 8) + g * (D / 8) + j;
+  constexpr unsigned kSlot = 2 * kQkThreads * 16;  // bytes
+  unsigned slot = 0, f_slot = 0;
+  unsigned char* const raw_bytes = reinterpret_cast<unsigned char*>(&s_raw[0][0][threadIdx.x]);
+  const uint32_t raw_at = static_cast<uint32_t>(__cvta_generic_to_shared(raw_bytes));
+  // where the next item's values lie (WHOLE), or its row's
+  const uint4* f_src = reinterpret_cast<const uint4*>(p.qkv) + (WHOLE ? static_cast<size_t>(begin) * (kHeads * D / 8) : static_cast<size_t>(row) * heads * (D / 8)) + g * (D / 8) + j;
   auto fetch = [&]() {  // the next item that is not on its way yet
     if (f_left > 0) {
-      const bool q = f_part < q_parts;
-      const int first = (q ? f_part : f_part - q_parts) * kHeads;  // of the item's heads, counted from the first q or k head
-      if (first + g < (q ? p.Hq : 2 * p.Hk)) {
-        const uint4* src = f_row + (q ? first : p.Hq + first) * (D / 8);
-        copy16_async(&s_raw[f_slot][0][threadIdx.x], src);
-        copy16_async(&s_raw[f_slot][1][threadIdx.x], src + kLanes);
+      if (WHOLE) {
+        copy16_async(raw_at + f_slot, f_src);
+        copy16_async(raw_at + f_slot + kQkThreads * 16, f_src + kLanes);
+        f_src += kHeads * D / 8;
+      } else {
+        const bool q = f_part < q_parts;
+        const int first = (q ? f_part : f_part - q_parts) * kHeads;  // of the item's heads, counted from the first q or k head
+        if (first + g < (q ? p.Hq : 2 * p.Hk)) {
+          const uint4* src = f_src + (q ? first : p.Hq + first) * (D / 8);
+          copy16_async(raw_at + f_slot, src);
+          copy16_async(raw_at + f_slot + kQkThreads * 16, src + kLanes);
+        }
+        if (++f_part == per_row) f_part = 0, f_src += heads * (D / 8);
       }
-      if (++f_part == per_row) f_part = 0, f_row += heads * (D / 8);
     }
-    --f_left, f_slot = (f_slot + 1) % kQkDepth;
+    --f_left, f_slot = (f_slot + kSlot) % (kQkDepth * kSlot);
     copies_commit();
   };
   int next_pos = __ldg(p.pos_rows + row), next_kv = __ldg(p.kv_rows + row);
@@ -202,14 +212,16 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
           ac[e] = mul2(a, ac[e]), as[e] = mul2(a, as[e]);
         }
       }
+      uint4* dst = reinterpret_cast<uint4*>(p.q_rot) + (static_cast<size_t>(row) * p.Hq + part * kHeads + g) * (D / 8) + j;
+      const int q_stop = min(q_parts - part, stop - item);
 #pragma unroll 1
-      for (; part < q_parts && item < stop; ++part, ++item) {
+      for (int i = 0; i < q_stop; ++i, dst += kHeads * D / 8) {
         fetch();
         copies_wait<kQkDepth - 1>();
-        const int head = part * kHeads + g;
-        const uint4 a4 = s_raw[slot][0][threadIdx.x], b4 = s_raw[slot][1][threadIdx.x];
-        slot = (slot + 1) % kQkDepth;
-        if (!sound || head >= p.Hq) continue;
+        const uint4 a4 = *reinterpret_cast<const uint4*>(raw_bytes + slot);
+        const uint4 b4 = *reinterpret_cast<const uint4*>(raw_bytes + slot + kQkThreads * 16);
+        slot = (slot + kSlot) % (kQkDepth * kSlot);
+        if (!sound || (!WHOLE && (part + i) * kHeads + g >= p.Hq)) continue;
         const F32x2 a[4] = {bf16x2_f32(a4.x), bf16x2_f32(a4.y), bf16x2_f32(a4.z), bf16x2_f32(a4.w)};
         const F32x2 b[4] = {bf16x2_f32(b4.x), bf16x2_f32(b4.y), bf16x2_f32(b4.z), bf16x2_f32(b4.w)};
         float rn = 1.0f;
@@ -235,10 +247,10 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
           f32x2_split(mul2(fma2(a[e], as[e], mul2(b[e], bc[e])), rn2), x, y);
           hi[e] = pack_bf16x2(x, y);
         }
-        uint4* dst = reinterpret_cast<uint4*>(p.q_rot + (static_cast<size_t>(row) * p.Hq + head) * D);
-        st_stream(dst + j, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-        st_stream(dst + kLanes + j, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+        st_stream(dst, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+        st_stream(dst + kLanes, make_uint4(hi[0], hi[1], hi[2], hi[3]));
       }
+      part += q_stop, item += q_stop;
     }
 
 #pragma unroll 1
@@ -246,9 +258,9 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
       fetch();
       copies_wait<kQkDepth - 1>();
       const int head = (part - q_parts) * kHeads + g;  // of k, then of v
-      const uint4* const raw = &s_raw[slot][0][threadIdx.x];
-      slot = (slot + 1) % kQkDepth;
-      if (!sound || head >= 2 * p.Hk) continue;
+      const uint4* const raw = reinterpret_cast<const uint4*>(raw_bytes + slot);
+      slot = (slot + kSlot) % (kQkDepth * kSlot);
+      if (!sound || (!WHOLE && head >= 2 * p.Hk)) continue;
       const bool is_k = head < p.Hk;
       const size_t srow = static_cast<size_t>(is_k ? head : head - p.Hk) * p.stride + kv_row;
       float lo[8], hi[8], zl[8], zh[8], sc;
@@ -368,8 +380,13 @@ int launch_qk_norm(const char* fn, const QkNormParams& p) {
   const long long items = static_cast<long long>(p.rows) * per_row;
   if (items > INT_MAX - kQkDepth) return fail(fn, "too many rows");
   const int grid = static_cast<int>(std::min((items + warps - 1) / warps, static_cast<long long>(kQkCtas) * sm_count()));
-  G4_LAUNCH_PDL(fn, (qk_norm_rope_kv_kernel<D, BITS>), dim3(static_cast<unsigned>(grid)), dim3(kQkThreads), 0, current_stream(), p,
-                q_parts, per_row, static_cast<int>(items / (grid * warps)), static_cast<int>(items % (grid * warps)));
+  const int run = static_cast<int>(items / (grid * warps)), longer = static_cast<int>(items % (grid * warps));
+  if (p.Hq % heads_per_item == 0 && 2 * p.Hk % heads_per_item == 0)
+    G4_LAUNCH_PDL(fn, (qk_norm_rope_kv_kernel<D, BITS, true>), dim3(static_cast<unsigned>(grid)), dim3(kQkThreads), 0, current_stream(), p,
+                  q_parts, per_row, run, longer);
+  else
+    G4_LAUNCH_PDL(fn, (qk_norm_rope_kv_kernel<D, BITS, false>), dim3(static_cast<unsigned>(grid)), dim3(kQkThreads), 0, current_stream(), p,
+                  q_parts, per_row, run, longer);
   return 0;
 }
 
