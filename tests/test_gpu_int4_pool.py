@@ -557,6 +557,39 @@ def test_a_decode_loop_captured_into_a_graph(K):
     assert torch.equal(vo, (cv.float() * sv[..., None]).to(torch.bfloat16))
 
 
+def test_two_captured_calls_at_once(K):
+    """Two graphs, of a cut call and of one by clusters, replayed side by side on two streams, each with a scratch of its own."""
+    Hq, Hk, d, n = 32, 8, 128, 40000
+    g = gen(21)
+    p, _ = random_pool(n, Hk, d, g)
+    jobs = []
+    for rows, per, length in ((1, 1, n), (6, 3, 3000)):
+        q = torch.randn(rows, Hq * d, generator=g, device=DEV).to(torch.bfloat16)
+        pos = torch.full((rows,), length - 1, dtype=torch.int32, device=DEV) - torch.arange(rows, device=DEV, dtype=torch.int32) % per
+        scratch = torch.empty(max(16, K.attn_decode_int4_scratch_bytes(rows, per, Hq, Hk, d, length)), dtype=torch.uint8, device=DEV)
+        out = torch.empty_like(q)
+
+        def call(q=q, pos=pos, length=length, per=per, out=out, scratch=scratch):
+            assert K.attn_decode_int4_paged(q, *p.all, pos, Hq, Hk, d, n, length, 0.02, out, rows_per_group=per, scratch=scratch) == 0
+        call()
+        torch.cuda.synchronize()
+        want = out.clone()
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=stream):
+            for _ in range(20):
+                call()
+        jobs.append((graph, stream, out, want, call))  # (call keeps what the graph reads)
+    for _ in range(5):
+        for _, _, out, _, _ in jobs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream, _, _, _ in jobs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for _, _, out, want, _ in jobs)
+
+
 def test_kv_move_of_a_4_bit_pool(K):
     Hk, d, stride = 4, 128, 64
     p, _ = random_pool(stride, Hk, d, gen(3))
