@@ -121,6 +121,11 @@ __device__ __forceinline__ uint32_t halves(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// A row's value over the sum of its probabilities; 0 where it saw nothing. What is not a number stays one.
+__device__ __forceinline__ uint16_t quotient_bf16(float acc, float l) {
+  return static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : __fdividef(acc, l), 0.0f));
+}
+
 // First and last position that any row of a group sees; last < first: none.
 __device__ __forceinline__ void group_span(const Int4AttnParams& p, int grp, int& lo, int& hi) {
   lo = INT_MAX, hi = -1;
@@ -380,8 +385,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       unsigned top_bits = 0;
 #pragma unroll
       for (int e = 0; e < kPer; ++e) top_bits = max(top_bits, __float_as_uint(f[e]) & 0x7fffffffu);
-      const float top = fmaxf(__uint_as_float(__reduce_max_sync(0xffffffffu, top_bits)), 1e-30f);
-      const float to_int = top < INFINITY ? 32639.0f / top : 0.0f;
+      top_bits = __reduce_max_sync(0xffffffffu, top_bits);
+      const bool sound = top_bits < 0x7f800000u;  // a head that holds an infinity or a NaN gives NaN
+      const float top = fmaxf(__uint_as_float(top_bits), 1e-30f), to_int = sound ? 32639.0f / top : 0.0f;
       uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};  // even dims, odd dims
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
@@ -398,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
           dst[4 * u] = static_cast<unsigned char>(hi[u]), dst[4 * u + sizeof(s_q[0])] = static_cast<unsigned char>(lo[u]);
         }
       }
-      if (lane == 0) s_scale[c] = top < INFINITY ? p.scale_log2 * top / 32639.0f : 0.0f;
+      if (lane == 0) s_scale[c] = sound ? p.scale_log2 * top / 32639.0f : __int_as_float(0x7fc00000);
     }
     __syncthreads();
     uint32_t qb[NS][kW][2];  // the lane's column g of tile i: pair 4 i + g / 2, hi (g even) or lo
@@ -600,7 +606,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       l += __shfl_xor_sync(0xffffffffu, l, 4);
       l += __shfl_xor_sync(0xffffffffu, l, 8);
       l += __shfl_xor_sync(0xffffffffu, l, 16);
-      if (g == 0) park[kC * (D + kPad) + 2 * c] = m_run[i], park[kC * (D + kPad) + 2 * c + 1] = l / v_mult;
+      // (a sum that is not a number has to outlive the merges, in which a maximum of -inf means: saw nothing)
+      if (g == 0) park[kC * (D + kPad) + 2 * c] = l == l ? m_run[i] : 0.0f, park[kC * (D + kPad) + 2 * c + 1] = l / v_mult;
       const float off = osum[n][e] * (8.0f / 16777216.0f);
 #pragma unroll
       for (int m = 0; m < kM; ++m)  // rows g, g + 8: dims 32 (m / 2) + 4 g + 2 (m % 2), + 1
@@ -630,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       } else if (whole) {
         const int j = (c0 + c) * p.g_inv >> 16, hl = c0 + c - j * p.G;
         p.out[(static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + dim] =
-            static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? __fdividef(acc, l) : 0.0f));
+            quotient_bf16(acc, l);
       } else {
         p.part_o[(slot * kC + c) * D + dim] = acc;
         if (dim == 0) p.part_ml[(slot * kC + c) * 2] = m, p.part_ml[(slot * kC + c) * 2 + 1] = l;
@@ -671,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
         }
         const int j = (c0 + c) * p.g_inv >> 16, hl = c0 + c - j * p.G;
         p.out[(static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + i % D] =
-            static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? __fdividef(acc, l) : 0.0f));
+            quotient_bf16(acc, l);
       }
       cluster.sync();  // nobody leaves while its memory is read
       return;
@@ -781,12 +788,12 @@ __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4Attn
     const int dim = threadIdx.x;
     if (dim < D) {
       const float sum = (s_acc[0][dim] + s_acc[1 % W][dim]) + (s_acc[2 % W][dim] + s_acc[3 % W][dim]);
-      out[dim] = static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? __fdividef(sum, l) : 0.0f));
+      out[dim] = quotient_bf16(sum, l);
     }
   } else {
 #pragma unroll
     for (int e = 0; e < kPer; ++e)  // (the output may lie on any 2-byte boundary)
-      out[lane * kPer + e] = static_cast<uint16_t>(f32_to_bf16_bits(l > 0.0f ? __fdividef(acc[e], l) : 0.0f));
+      out[lane * kPer + e] = quotient_bf16(acc[e], l);
   }
 }
 

@@ -288,8 +288,9 @@ int granite4_kernel_rope_kv_int8_paged(const uint16_t* d_qkv, const float* d_cos
  * bits 8: top 127, the int8 pool [Hk][stride][d] of the entry points above. bits 4:
  * top 7, uint8 [Hk][stride][d / 2], code + 8 in a nibble, the even dim in the low half
  * of its byte. Scales are f32 [Hk][stride] for both. Codes are those of exact
- * arithmetic on the bf16 inputs and the f32 tables (a row that holds an infinity
- * or a NaN gets unspecified codes in [-top, top]). d is 64 or 128; eps > 0; norm weights,
+ * arithmetic on the bf16 inputs and the f32 tables (a head that holds an infinity
+ * or a NaN gets unspecified codes; a normed query head's squares are summed in f32, so
+ * its values have to stay under 1e18). d is 64 or 128; eps > 0; norm weights,
  * tables, qkv, q_rot and caches 16-byte aligned. d_pos_rows / d_kv_rows as in
  * granite4_kernel_rope_kv_int8_paged: a row with an index out of range is skipped;
  * pool rows of one call are distinct. For granite4_kernel_kv_move a 4-bit pool is one
@@ -541,7 +542,8 @@ int granite4_attn_split_int8(const uint16_t* d_q, const int8_t* d_cache_k8, cons
  * must hold granite4_attn_decode_int4_scratch_bytes(...) bytes of the same device, 16-byte
  * aligned (0: NULL will do), and belongs to one call at a time. The rows' table entries
  * are read only for positions that some row of the group sees. A row with a negative
- * position gets zeros; the rows of a group may have any positions. The cache is cut into
+ * position gets zeros; the rows of a group may have any positions. A query head
+ * that holds an infinity or a NaN gives NaN, the others are not touched by it. The cache is cut into
  * equal shares whatever the sequences' lengths, and the order of every sum follows from
  * the arguments and positions alone: the same call gives the same bits. */
 long long granite4_attn_decode_int4_scratch_bytes(int rows, int rows_per_group, int Hq, int Hk, int d,

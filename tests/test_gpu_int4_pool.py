@@ -361,6 +361,26 @@ def test_a_table_for_all_rows_identity_and_positions_past_max_len(K):
         assert ((out.double().view(3, Hq, d) - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("n", [60, 900, 30000])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_head_that_is_not_a_number_stays_one(K, n, bad):
+    Hq, Hk, d = 32, 8, 128
+    g = gen(n)
+    p, _ = random_pool(n, Hk, d, g)
+    q = torch.randn(2, Hq, d, generator=g, device=DEV).to(torch.bfloat16)
+    pos = torch.tensor([n - 1, n - 2], dtype=torch.int32, device=DEV)
+    outs = []
+    for spoilt in (False, True):
+        if spoilt:
+            q[1, 5, 17] = bad
+        out = torch.empty_like(q)
+        assert K.attn_decode_int4_paged(q, *p.all, pos, Hq, Hk, d, n, n, 0.05, out, rows_per_group=2) == 0
+        outs.append(out)
+    assert outs[1][1, 5].isnan().all()
+    outs[1][1, 5] = outs[0][1, 5]
+    assert torch.equal(outs[0], outs[1])
+
+
 def test_output_between_two_words_and_other_streams(K):
     Hq, Hk, d, n = 32, 8, 128, 2000
     g = gen(6)
