@@ -617,30 +617,50 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     __syncthreads();
     const bool whole = piece_begin == 0 && piece_end == n_tiles;
     const size_t slot = blockIdx.x + (chunk > 0 ? 0 : static_cast<size_t>(grp) * per_group + sub);
-    const int dim = threadIdx.x % D;
-    for (int c = threadIdx.x / D; c < columns; c += kThreads / D) {
-      float mw[kWarps], m = -INFINITY, l = 0.0f, acc = 0.0f;
+    constexpr int kPer = D / 32;  // a warp merges every fourth column, a lane so many of its dims
+    for (int c = warp; c < columns; c += kWarps) {
+      float mw[kWarps], m = -INFINITY, l = 0.0f, acc[kPer];
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         mw[w] = reinterpret_cast<const float*>(s_ring + w * kWarpBytes<D>)[kC * (D + kPad) + 2 * c];
         m = fmaxf(m, mw[w]);
       }
 #pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
+#pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float* parked = reinterpret_cast<const float*>(s_ring + w * kWarpBytes<D>);
         const float f = mw[w] == -INFINITY ? 0.0f : exp2_fast(mw[w] - m);
-        l += f * parked[kC * (D + kPad) + 2 * c + 1], acc += f * parked[c * (D + kPad) + dim];
+        l += f * parked[kC * (D + kPad) + 2 * c + 1];
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(parked + c * (D + kPad) + lane * kPer + e);
+          acc[e] += f * v.x, acc[e + 1] += f * v.y;
+        }
       }
-      if (p.cluster > 1) {  // (each value of warp 0's state is read by this thread alone)
-        reinterpret_cast<float*>(s_ring)[c * (D + kPad) + dim] = acc;
-        if (dim == 0) s_cta[c] = make_float2(m, l);
+      if (p.cluster > 1) {  // (the values of warp 0's state are read by this lane alone)
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2)
+          *reinterpret_cast<float2*>(reinterpret_cast<float*>(s_ring) + c * (D + kPad) + lane * kPer + e) = make_float2(acc[e], acc[e + 1]);
+        if (lane == 0) s_cta[c] = make_float2(m, l);
       } else if (whole) {
         const int j = (c0 + c) * p.g_inv >> 16, hl = c0 + c - j * p.G;
-        p.out[(static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + dim] =
-            quotient_bf16(acc, l);
+        uint16_t* const out = p.out + (static_cast<size_t>(r0 + j) * p.Hq + static_cast<size_t>(hkv) * p.G + hl) * D + lane * kPer;
+        uint16_t v[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) v[e] = quotient_bf16(acc[e], l);
+        if ((reinterpret_cast<uintptr_t>(p.out) & 3u) == 0) {
+#pragma unroll
+          for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(out + e) = v[e] | static_cast<uint32_t>(v[e + 1]) << 16;
+        } else {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) out[e] = v[e];
+        }
       } else {
-        p.part_o[(slot * kC + c) * D + dim] = acc;
-        if (dim == 0) p.part_ml[(slot * kC + c) * 2] = m, p.part_ml[(slot * kC + c) * 2 + 1] = l;
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2)
+          *reinterpret_cast<float2*>(p.part_o + (slot * kC + c) * D + lane * kPer + e) = make_float2(acc[e], acc[e + 1]);
+        if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * kC + c) * 2) = make_float2(m, l);
       }
     }
     if (p.cluster > 1) {
