@@ -123,7 +123,14 @@ __global__ void __launch_bounds__(kReadThreads) kv_widen_kernel(const WidenParam
     const uint2 w = __ldg(reinterpret_cast<const uint2*>((kv ? p.cv : p.ck) + srow * 64) + part);
     const uint2 a = nibbles_to_bytes(w.x), b = nibbles_to_bytes(w.y);
     reinterpret_cast<uint4*>(kv ? p.ov : p.ok)[i] = make_uint4(a.x, a.y, b.x, b.y);
-    if (part == 0) (kv ? p.ovs : p.oks)[hp] = __ldg((kv ? p.vs : p.ks) + srow);
+  }
+  if (part == 0) {
+    // A value scale that is not finite, or takes values past fp16's range (V's type in those kernels), goes over to the
+    // key's: as a logit it is masked for the rows that do not see the position, as an element of V it would reach them
+    // (0 times infinity), and who sees it gets NaN either way.
+    const float ks = __ldg(p.ks + srow), vs = __ldg(p.vs + srow);
+    const bool sound = fabsf(vs) * 7.0f <= 65504.0f;
+    p.oks[hp] = sound ? ks : __int_as_float(0x7fc00000), p.ovs[hp] = sound ? vs : 0.0f;
   }
 }
 

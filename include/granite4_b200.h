@@ -543,7 +543,9 @@ int granite4_attn_split_int8(const uint16_t* d_q, const int8_t* d_cache_k8, cons
  * aligned (0: NULL will do), and belongs to one call at a time. The rows' table entries
  * are read only for positions that some row of the group sees. A row with a negative
  * position gets zeros; the rows of a group may have any positions. A query head
- * that holds an infinity or a NaN gives NaN, the others are not touched by it. The cache is cut into
+ * that holds an infinity or a NaN gives NaN, the others are not touched by it; a row
+ * scale that is a NaN, or an infinite value scale, gives NaN to the rows that see its
+ * position and to no others. The cache is cut into
  * equal shares whatever the sequences' lengths, and the order of every sum follows from
  * the arguments and positions alone: the same call gives the same bits. */
 long long granite4_attn_decode_int4_scratch_bytes(int rows, int rows_per_group, int Hq, int Hk, int d,
@@ -560,7 +562,9 @@ int granite4_kernel_attn_decode_int4_paged(const uint16_t* d_q, const uint8_t* d
  * widen the sequence's rows into an 8-bit pool in d_scratch (exact: a 4-bit code is an
  * 8-bit code with the same scale; 264 bytes per position and kv head) and run the kernels
  * of that entry point; everything else runs on the decode kernel, where d_scratch is
- * optional (without it no range is split). d_scratch must hold
+ * optional (without it no range is split). Those kernels hold V in fp16: values under
+ * 6e-5 lose bits there, and a position with 7 * v_scale over 65504 gives NaN to the rows
+ * that see it, as a scale that is not a number does in both forms. d_scratch must hold
  * granite4_prefill_attention_int4_scratch_bytes(...) bytes, 16-byte aligned. */
 long long granite4_prefill_attention_int4_scratch_bytes(int rows, int base_pos, int Hq, int Hk, int d);
 int granite4_prefill_attention_int4(const uint16_t* d_q_rot, float scale, int Hq, int Hk, int d,

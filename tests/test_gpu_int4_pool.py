@@ -381,6 +381,31 @@ def test_a_head_that_is_not_a_number_stays_one(K, n, bad):
     assert torch.equal(outs[0], outs[1])
 
 
+@pytest.mark.parametrize("which,bad", [("k", float("nan")), ("v", float("nan")), ("v", float("inf"))])
+@pytest.mark.parametrize("n,per,window", [(60, 3, 0), (900, 4, 0), (30000, 3, 0), (5000, 2, 40), (129, 16, 3)])
+def test_a_scale_that_is_not_a_number_stays_with_the_rows_that_see_it(K, n, per, window, which, bad):
+    Hq, Hk, d, scale = 8, 4, 128, 1.0 / 64
+    g = gen(n + per)
+    p, codes = random_pool(n, Hk, d, g)
+    q = torch.randn(per, Hq * d, generator=g, device=DEV).to(torch.bfloat16)
+    pos = torch.arange(n - per, n, device=DEV, dtype=torch.int32)
+    tab = torch.arange(n, dtype=torch.int32, device=DEV)
+    want, tol = attention64(q, p, codes, [tab] * per, pos, per, Hq, Hk, d, scale, window, 2 * n // 32 + 2)
+    for at in (n - 1, max(0, n - per + 1 - window) if window else n - per + 1):
+        t = p.ks if which == "k" else p.vs
+        old = t[2, at].item()
+        t[2, at] = bad
+        out = torch.empty(per, Hq * d, dtype=torch.bfloat16, device=DEV)
+        assert K.attn_decode_int4_paged(q, *p.all, pos, Hq, Hk, d, n, n, scale, out, rows_per_group=per, window=window) == 0
+        t[2, at] = old
+        got = out.double().view(per, Hq, d)
+        sees = (pos >= at) & (pos - window < at if window else pos >= at)
+        hit = sees[:, None] & (torch.arange(Hq, device=DEV) // (Hq // Hk) == 2)[None]
+        assert hit.any() and not hit.all()
+        assert got[hit].isnan().all()
+        assert ((got - want).abs() <= tol)[~hit].all()
+
+
 def test_output_between_two_words_and_other_streams(K):
     Hq, Hk, d, n = 32, 8, 128, 2000
     g = gen(6)
@@ -620,3 +645,47 @@ def test_kv_move_of_a_4_bit_pool(K):
         assert torch.equal(t[:, 2], b[:, 5]) and torch.equal(t[:, 3], b[:, 9])
         b[:, 2], b[:, 3] = b[:, 5], b[:, 9]
         assert torch.equal(t, b)
+
+
+@pytest.mark.parametrize("rows,base", [(20, 5), (40, 0), (130, 2000), (300, 0), (64, 16000)])
+@pytest.mark.parametrize("which,bad", [("k", float("nan")), ("v", float("nan")), ("v", float("inf"))])
+def test_a_chunk_with_a_scale_that_is_not_a_number(K, rows, base, which, bad):
+    """The rows before the position are as without it, to the bit; those that see it NaN."""
+    Hq, Hk, d = 32, 8, 128
+    g = gen(rows + base)
+    n = base + rows
+    p, _ = random_pool(n, Hk, d, g)
+    q = torch.randn(rows, Hq, d, generator=g, device=DEV).to(torch.bfloat16)
+    outs = []
+    first = rows // 2 + 1
+    for spoilt in (False, True):
+        if spoilt:
+            (p.ks if which == "k" else p.vs)[3, base + first] = bad
+        out = torch.empty_like(q)
+        assert K.prefill_attention_int4(q, 1.0 / 64, Hq, Hk, d, base, n, out, *p.all) == 0
+        outs.append(out)
+    assert torch.isfinite(outs[0]).all()
+    assert outs[1][first:, 12:16].isnan().all()
+    assert torch.equal(outs[0][:first], outs[1][:first])
+    assert torch.equal(outs[0][:, :12], outs[1][:, :12]) and torch.equal(outs[0][:, 16:], outs[1][:, 16:])
+
+
+@pytest.mark.parametrize("rows,base", [(40, 0), (130, 2000)])
+def test_a_chunk_with_values_past_fp16(K, rows, base):
+    """A widened chunk holds V in fp16: a position past its range gives NaN where it is seen and nothing elsewhere."""
+    Hq, Hk, d = 32, 8, 128
+    g = gen(rows)
+    n = base + rows
+    p, _ = random_pool(n, Hk, d, g)
+    q = torch.randn(rows, Hq, d, generator=g, device=DEV).to(torch.bfloat16)
+    first = rows - 3
+    outs = []
+    for vs in (1.0, 9300.0, 9400.0):  # times 7: 65100, 65800
+        p.vs[3, base + first] = vs
+        out = torch.empty_like(q)
+        assert K.prefill_attention_int4(q, 1.0 / 64, Hq, Hk, d, base, n, out, *p.all) == 0
+        outs.append(out)
+    assert torch.isfinite(outs[1]).all()
+    assert outs[2][first:, 12:16].isnan().all()
+    outs[2][first:, 12:16] = outs[1][first:, 12:16]
+    assert torch.equal(outs[1], outs[2]) and torch.equal(outs[0][:first], outs[1][:first])
