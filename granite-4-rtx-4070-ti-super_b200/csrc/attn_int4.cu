@@ -8,8 +8,11 @@
 // A position costs d + 8 bytes a kv head and 4 d multiply-adds a query head: memory bounds it as long as the
 // conversion of the codes stays cheap, so nothing is converted that need not be:
 //  * A nibble u = c + 8 masked out of a word IS a number of the mma's operand type. K: in the low half of a byte it is a
-//    u8; two ANDs and a shift give the eight operand elements of a word. V: in bits 0-3 of a half it is the fp16
-//    subnormal u 2^-24, in bits 4-7 u 2^-20; the powers of two come out of the output rows, exactly.
+//    u8; two ANDs and a shift give the eight operand elements of a word. V: in bits 4-7 of a half it is the fp16
+//    subnormal u 2^-20, and the power of two comes out of the output, exactly. The tensor cores line products up by the
+//    operands' exponent fields, and a subnormal's is that of 2^-14: of a sum they keep what is above 2^-24 of p 2^-14. With
+//    nibbles in bits 0-3 too, as u 2^-24 (two shifts a word less: 16 sessions 65.5 us instead of 67), sums were off by 2^-13 of the
+//    largest p v_scale, more than the other positions of a peaked softmax are worth; in bits 4-7 it is 2^-17.
 //  * The 8 of u = c + 8 is one number per column: sum_d q_d (u_d - 8) = sum q u - 8 sum q, and
 //    sum_t p_t (u_t - 8) = sum p u - 8 sum p, with sum p from one more mma against ones.
 //  * The row scales multiply a logit (K) and a probability (V), never an element.
@@ -590,12 +593,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
           load_8x8_trans(v, at + piece_at<D>(r, c + (lane >> 4)) * 16);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const uint32_t a = v[2 * u], b = v[2 * u + 1], a8 = a >> 8, b8 = b >> 8;
+            const uint32_t a = v[2 * u], b = v[2 * u + 1];
+            constexpr uint32_t kNibble = 0x00f000f0u;
 #pragma unroll
             for (int n = 0; n < kNP; ++n) {
-              mma16816(o[n][2 * (c + u)], a & 0x000f000fu, a & 0x00f000f0u, b & 0x000f000fu, b & 0x00f000f0u, pb[n][h][0],
+              mma16816(o[n][2 * (c + u)], (a << 4) & kNibble, a & kNibble, (b << 4) & kNibble, b & kNibble, pb[n][h][0],
                        pb[n][h][1]);
-              mma16816(o[n][2 * (c + u) + 1], a8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x000f000fu, b8 & 0x00f000f0u,
+              mma16816(o[n][2 * (c + u) + 1], (a >> 4) & kNibble, (a >> 8) & kNibble, (b >> 4) & kNibble, (b >> 8) & kNibble,
                        pb[n][h][0], pb[n][h][1]);
             }
           }
@@ -610,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __syncwarp();
     float* const park = reinterpret_cast<float*>(ring);  // [kC][D + kPad], then [kC][2] (max, sum)
-    const float back = 16777216.0f / v_mult;
+    const float back = 1048576.0f / v_mult;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const int n = i >> 1, e = i & 1, c = 4 * i + t;
@@ -620,11 +624,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       l += __shfl_xor_sync(0xffffffffu, l, 16);
       // (a sum that is not a number has to outlive the merges, in which a maximum of -inf means: saw nothing)
       if (g == 0) park[kC * (D + kPad) + 2 * c] = l == l ? m_run[i] : 0.0f, park[kC * (D + kPad) + 2 * c + 1] = l / v_mult;
-      const float off = osum[n][e] * (8.0f / 16777216.0f);
+      const float off = osum[n][e] * (8.0f / 1048576.0f);
 #pragma unroll
       for (int m = 0; m < kM; ++m)  // rows g, g + 8: dims 32 (m / 2) + 4 g + 2 (m % 2), + 1
         *reinterpret_cast<float2*>(park + c * (D + kPad) + 32 * (m >> 1) + 4 * g + 2 * (m & 1)) =
-            make_float2((o[n][m][e] - off) * back, (o[n][m][2 + e] * 0.0625f - off) * back);
+            make_float2((o[n][m][e] - off) * back, (o[n][m][2 + e] - off) * back);
     }
     __syncthreads();
     const bool whole = piece_begin == 0 && piece_end == n_tiles;
