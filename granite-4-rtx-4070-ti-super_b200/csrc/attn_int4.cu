@@ -26,10 +26,13 @@
 //    2^-11 that P is rounded by. (Measured at 16 sessions of up to 24000: fp16 operands, which take five instructions
 //    instead of three per eight codes and twice the mma, 86 us; two e4m3 columns, which sm_100 widens to fp16 instruction
 //    by instruction, 82; u8 x s8 72, the rest alike.)
-// P is rounded to fp16 (11 bits; everything else is f32) after the multiplication with v_scale and a power of two that
-// puts the largest v_scale seen at 2^8, so that values of any magnitude keep the format's precision. The running maximum
-// moves only when it is passed by 4 (in powers of two): P is at most 16, v_scale 2^11, fp16 ends at 2^16, and most tiles
-// leave the accumulators as they are.
+// What goes into the second contraction is p v_scale, rounded to fp16 (11 bits; everything else is f32). So what a column's
+// probabilities are taken against, p = exp2(l - m - under), is not its largest logit but its largest l + log2(v_scale) of the
+// positions that it sees, less 10: the largest p v_scale so far is kept at 2^10, whatever its magnitude, and a scale at a position
+// that a column does not see, or gives no weight to, takes no bits from the others. That moves only when a position passes it by
+// 14: products reach 2^14, fp16 ends at 2^16, and most tiles leave the accumulators as they are. m is a logit, and everything
+// else a difference to it, so that large logits cost no bits of the rest. p reaches 2^54 where v_scale is small: a scale, a
+// zero too, counts as 2^-40 at least, so that neither a sum of p nor the factor of a move leaves f32 for scales up to 2^60.
 //
 // Work split, by size: a (group, kv head, column block) segment is one CTA's; or a cluster's, whose CTAs take equal parts
 // and join them through distributed shared memory; or, for long caches, the segments' tiles of 32 positions form one line,
@@ -65,6 +68,9 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kMaxGroups = 256;   // of a launch that cuts the line of tiles
 constexpr int kMaxShares = 640;   // it is cut into
 constexpr int kMaxColumns = 64;   // rows of a group x query heads of a kv head
+constexpr float kNone = -1e38f;  // the m of what has seen nothing: below every logit, and differences of two are finite
+constexpr float kUnset = -1e30f;  // the same of `under`
+constexpr float kLift = 10.0f, kSlack = 14.0f, kLeastLogScale = -40.0f;
 
 struct Int4AttnParams {
   const uint16_t* q;
@@ -117,6 +123,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ uint32_t halves(float a, float b) {
@@ -226,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
   static_assert(kWarpBytes<D> >= kC * (D + kPad) * 4 + kC * 8, "a warp parks its state in its ring");
   __shared__ __align__(16) unsigned char s_q[8 * NS][D + 16];  // a row per column of the logit tiles
   __shared__ float s_scale[4 * NS];                            // of a pair's logits
-  __shared__ float2 s_cta[4 * NS];                             // (max, sum) of the CTA, where it is one of a cluster
+  __shared__ float2 s_cta[4 * NS];                             // (m, sum) of the CTA, where it is one of a cluster
   extern __shared__ __align__(128) unsigned char s_ring[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   unsigned char* const ring = s_ring + warp * kWarpBytes<D>;
@@ -440,8 +451,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, o));
     }
 
-    float o[kNP][kM][4], osum[kNP][4], m_run[NS], l_run[NS];  // l_run times v_mult
-    float e_base[NS];  // what is taken off a logit: m_run - log2(v_mult)
+    float o[kNP][kM][4], osum[kNP][4], m_ref[NS], under[NS], l_run[NS];  // p = exp2(l - m_ref - under)
 #pragma unroll
     for (int n = 0; n < kNP; ++n) {
 #pragma unroll
@@ -449,8 +459,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       osum[n][0] = osum[n][1] = osum[n][2] = osum[n][3] = 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < NS; ++i) m_run[i] = -INFINITY, e_base[i] = l_run[i] = 0.0f;
-    float v_mult = 1.0f, v_cap = -1.0f;  // power of two on v_scale, and the largest v_scale it is good for
+    for (int i = 0; i < NS; ++i) m_ref[i] = l_run[i] = 0.0f, under[i] = kUnset;
 
     for (int stage = 0; tile < tile_end; tile += kWarps, stage ^= 1) {
       copies_wait();
@@ -494,12 +503,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       float fk[4], fv[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) fk[i] = raw_ks[g + 8 * i], fv[i] = raw_vs[g + 8 * i];
-      float l[NS][4], l_top[NS];  // logits in powers of two of pair 4 i + t at positions g + 8 u
+      float dl[NS][4];  // logits in powers of two, less m_ref, of pair 4 i + t at positions g + 8 u
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          l[i][u] = static_cast<float>(s[i][u >> 1][2 * (u & 1)] * 256 + s[i][u >> 1][2 * (u & 1) + 1] - l_off[i]) * (fk[u] * l_scale[i]);
+          dl[i][u] = fmaf(static_cast<float>(s[i][u >> 1][2 * (u & 1)] * 256 + s[i][u >> 1][2 * (u & 1) + 1] - l_off[i]), fk[u] * l_scale[i], -m_ref[i]);
       const bool masked = !(t0 >= all_lo && t0 + kTile - 1 <= all_hi);  // the same for the whole warp
       if (masked) {
         asm volatile("" ::: "memory");  // (a branch, not selects)
@@ -508,46 +517,38 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int pos = t0 + g + 8 * u;
-            if (pos > pos_col[i] || (p.window > 0 && pos_col[i] != INT_MAX && pos <= pos_col[i] - p.window)) l[i][u] = -INFINITY;
+            if (pos > pos_col[i] || (p.window > 0 && pos_col[i] != INT_MAX && pos <= pos_col[i] - p.window)) dl[i][u] = -INFINITY;
           }
       }
-      const float v_top = fmaxf(fmaxf(fv[0], fv[1]), fmaxf(fv[2], fv[3]));
-      bool moves = v_top > v_cap;
+      float lv[4], z_top[NS];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) lv[u] = fminf(fmaxf(log2_fast(fabsf(fv[u])), kLeastLogScale), 127.0f);  // (of what is not finite: 127 or the least)
+      bool moves = false;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        l_top[i] = fmaxf(fmaxf(l[i][0], l[i][1]), fmaxf(l[i][2], l[i][3]));
-        moves |= l_top[i] > m_run[i] + 4.0f;
+        z_top[i] = fmaxf(fmaxf(dl[i][0] + lv[0], dl[i][1] + lv[1]), fmaxf(dl[i][2] + lv[2], dl[i][3] + lv[3]));
+        moves |= z_top[i] > under[i] + kSlack;
       }
       if (__any_sync(0xffffffffu, moves)) {
-        float f = 1.0f;
-        if (__any_sync(0xffffffffu, v_top > v_cap)) {
-          float top = 0.0f;  // of the finite ones: an infinity is seen by some columns only
-#pragma unroll
-          for (int u = 0; u < 4; ++u) top = fmaxf(top, fv[u] < INFINITY ? fv[u] : 0.0f);
-          top = warp_max(top);
-          float mult = 1.0f;
-          v_cap = 0.0f;
-          if (top > 0.0f) {
-            const int ex = min(max(((__float_as_int(top) >> 23) & 0xff) - 127, -100), 100);
-            mult = __int_as_float((127 + 8 - ex) << 23);
-            v_cap = __int_as_float((127 + 3 + ex) << 23);  // 2^11 once multiplied
-          }
-          f = mult / v_mult;
-          v_mult = mult;
-        }
-        const float log_mult = static_cast<float>(((__float_as_int(v_mult) >> 23) & 0xff) - 127);
         float corr[2 * kNP];
         corr[2 * kNP - 1] = 1.0f;
+        const auto over_positions = [](float x) {
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        };
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          float top = l_top[i];
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const float m_new = fmaxf(m_run[i], top);
-          corr[i] = m_new == -INFINITY ? 1.0f : exp2_fast(m_run[i] - m_new) * f;
-          l_run[i] *= corr[i], m_run[i] = m_new;
-          e_base[i] = (m_new == -INFINITY ? 0.0f : m_new) - log_mult;
+        for (int i = 0; i < NS; ++i) {  // each column by what it sees itself
+          const bool grows = over_positions(z_top[i]) > under[i] + kSlack;
+          const float top = over_positions(fmaxf(fmaxf(dl[i][0], dl[i][1]), fmaxf(dl[i][2], dl[i][3])));
+          const float m_new = grows ? m_ref[i] + top : m_ref[i], up = m_new - m_ref[i];
+          float z = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) dl[i][u] -= up, z = fmaxf(z, dl[i][u] + lv[u]);
+          z = over_positions(z);
+          const float next = grows ? z - kLift : under[i];
+          corr[i] = exp2_fast(under[i] - next - up);
+          l_run[i] *= corr[i], m_ref[i] = m_new, under[i] = next;
         }
 #pragma unroll
         for (int n = 0; n < kNP; ++n) {
@@ -570,13 +571,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
           if (i >= NS) break;
           float pr[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) pr[u] = exp2_fast(l[i][u] - e_base[i]), pv[e][u] = pr[u] * fv[u];
+          for (int u = 0; u < 4; ++u) pr[u] = exp2_fast(dl[i][u] - under[i]), pv[e][u] = pr[u] * fv[u];
           l_run[i] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
           if (masked) {  // a scale that is not finite stays with the columns that see it
             asm volatile("" ::: "memory");
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-              if (l[i][u] == -INFINITY) pv[e][u] = 0.0f;
+              if (dl[i][u] == -INFINITY) pv[e][u] = 0.0f;
           }
         }
 #pragma unroll
@@ -613,8 +614,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     // the four warps' states meet in shared memory, each parked in the warp's own ring
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __syncwarp();
-    float* const park = reinterpret_cast<float*>(ring);  // [kC][D + kPad], then [kC][2] (max, sum)
-    const float back = 1048576.0f / v_mult;
+    float* const park = reinterpret_cast<float*>(ring);  // [kC][D + kPad], then [kC][2] (m, sum), as of p = exp2(l - m)
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const int n = i >> 1, e = i & 1, c = 4 * i + t;
@@ -622,8 +622,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       l += __shfl_xor_sync(0xffffffffu, l, 4);
       l += __shfl_xor_sync(0xffffffffu, l, 8);
       l += __shfl_xor_sync(0xffffffffu, l, 16);
-      // (a sum that is not a number has to outlive the merges, in which a maximum of -inf means: saw nothing)
-      if (g == 0) park[kC * (D + kPad) + 2 * c] = l == l ? m_run[i] : 0.0f, park[kC * (D + kPad) + 2 * c + 1] = l / v_mult;
+      const float shift = exp2_fast(under[i]), back = 1048576.0f * shift;
+      if (g == 0) park[kC * (D + kPad) + 2 * c] = under[i] == kUnset ? kNone : m_ref[i], park[kC * (D + kPad) + 2 * c + 1] = l * shift;
       const float off = osum[n][e] * (8.0f / 1048576.0f);
 #pragma unroll
       for (int m = 0; m < kM; ++m)  // rows g, g + 8: dims 32 (m / 2) + 4 g + 2 (m % 2), + 1
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     const size_t slot = blockIdx.x + (chunk > 0 ? 0 : static_cast<size_t>(grp) * per_group + sub);
     constexpr int kPer = D / 32;  // a warp merges every fourth column, a lane so many of its dims
     for (int c = warp; c < columns; c += kWarps) {
-      float mw[kWarps], m = -INFINITY, l = 0.0f, acc[kPer];
+      float mw[kWarps], m = kNone, l = 0.0f, acc[kPer];
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         mw[w] = reinterpret_cast<const float*>(s_ring + w * kWarpBytes<D>)[kC * (D + kPad) + 2 * c];
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float* parked = reinterpret_cast<const float*>(s_ring + w * kWarpBytes<D>);
-        const float f = mw[w] == -INFINITY ? 0.0f : exp2_fast(mw[w] - m);
+        const float f = exp2_fast(mw[w] - m);
         l += f * parked[kC * (D + kPad) + 2 * c + 1];
 #pragma unroll
         for (int e = 0; e < kPer; e += 2) {
@@ -687,14 +687,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       const int rank = blockIdx.x % p.cluster;
       for (int i = rank * kThreads + threadIdx.x; i < columns * D; i += p.cluster * kThreads) {
         const int c = i / D, at = c * (D + kPad) + i % D;
-        float m = -INFINITY, l = 0.0f, acc = 0.0f;
+        float m = kNone, l = 0.0f, acc = 0.0f;
 #pragma unroll 1
         for (int r0_ = 0; r0_ < p.cluster; r0_ += 8) {
           float2 ml[8];
           float v[8];
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            ml[u] = make_float2(-INFINITY, 0.0f), v[u] = 0.0f;
+            ml[u] = make_float2(kNone, 0.0f), v[u] = 0.0f;
             if (r0_ + u < p.cluster) {
               ml[u] = *cluster.map_shared_rank(s_cta + c, r0_ + u);
               v[u] = *cluster.map_shared_rank(reinterpret_cast<const float*>(s_ring) + at, r0_ + u);
@@ -703,7 +703,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
           float top = m;
 #pragma unroll
           for (int u = 0; u < 8; ++u) top = fmaxf(top, ml[u].x);
-          if (top == -INFINITY) continue;
           const float keep = exp2_fast(m - top);
           l *= keep, acc *= keep, m = top;
 #pragma unroll
@@ -765,10 +764,10 @@ __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4Attn
     }
   };
   auto ml_of = [&](int i) {
-    return i < n ? __ldcg(reinterpret_cast<const float2*>(part_ml + static_cast<size_t>(i) * (kC * 2))) : make_float2(-INFINITY, 0.0f);
+    return i < n ? __ldcg(reinterpret_cast<const float2*>(part_ml + static_cast<size_t>(i) * (kC * 2))) : make_float2(kNone, 0.0f);
   };
   load(first);
-  float m = -INFINITY, l = 0.0f;
+  float m = kNone, l = 0.0f;
   if (W == 4) {
     constexpr int kEach = (kMaxShares + kThreads - 1) / kThreads;
     float2 ml[kEach];
@@ -781,7 +780,7 @@ __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4Attn
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
       const int i = threadIdx.x + k * kThreads;
-      const float f = ml[k].x == -INFINITY ? 0.0f : exp2_fast(ml[k].x - m);
+      const float f = exp2_fast(ml[k].x - m);
       if (i < n) s_w[i] = f;
       l += f * ml[k].y;
     }
@@ -806,7 +805,7 @@ __global__ void __launch_bounds__(kThreads) attn_int4_join_kernel(const Int4Attn
         if (i + u * W < n) f = s_w[i + u * W];
       } else {
         const float2 ml = ml_of(i + u);
-        f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - m);
+        f = exp2_fast(ml.x - m);
         l += f * ml.y;
       }
 #pragma unroll

@@ -8,9 +8,10 @@ The reference, in 64 bits, takes q as the kernel holds it, the 16-bit integer ro
   p v_scale as fp16      2^-11 sum p |v|; its floor: the largest p s is held at 2^10 or more and steps under fp16's normal range
                          are 2^-24, so each of the n positions is off by at most 2^-35 max(p s), times |c| <= 7 (and 1 % for the
                          logarithm that decides on it); a scale counts as 2^-40 at least: 7 n (1.01 2^-35 max(p s) + 2^-75)
-  logits                 an exact integer, to f32 (1), times k_scale (scale log2(e) max |q| / 32639) (4), less the base (1 of its
-                         own size): in powers of two 6 * 2^-24 |l| + 2^-24 (|l| + |base|), |base| <= max |l| + 40 + 24;
-                         exp2 itself 2^-22; numerator and sum both: twice
+  logits                 an exact integer, to f32 (1), times k_scale (scale log2(e) max |q| / 32639) (5, the constant's among
+                         them), less a logit in an fma and less a number under 64 (what is left is under 64 for every position
+                         whose weight counts): in powers of two under 8 * 2^-24 |l| + 64 * 2^-24; exp2 itself 2^-22; numerator
+                         and sum both: twice
   sums                   16 sum p s (steps + 16) 2^-23 over u = c + 8, steps = 16-position steps of a warp
 """
 import math
@@ -99,6 +100,76 @@ def check(got, want, bar, sharp):
     assert (want.abs() / bar.clamp(min=1e-300)).median().item() >= sharp
 
 
+@pytest.mark.parametrize("loud", [1e6, 1e12, 1e18])
+@pytest.mark.parametrize("Hq,Hk,d", [(8, 4, 128), (16, 2, 64), (32, 8, 128)])
+@pytest.mark.parametrize("n,per,window", [(4, 4, 0), (60, 3, 0), (900, 4, 0), (30000, 3, 0), (5000, 2, 40), (129, 4, 3)])
+def test_a_large_value_scale_stays_with_the_rows_that_see_it(K, n, per, window, Hq, Hk, d, loud):
+    """At the last row's own position, and where a window has left later rows behind."""
+    g = gen(n + per + d)
+    p = Pool(g, n, Hk, d)
+    q = torch.randn(per, Hq, d, generator=g, device=DEV).to(torch.bfloat16)
+    pos = torch.arange(n - per, n, device=DEV, dtype=torch.int32)
+    for at in (n - 1, max(0, n - per + 1 - window) if window else n - per + 1):
+        old = p.vs[:, at].clone()
+        p.vs[:, at] = loud
+        want, bar = reference(p, q, pos, 1.0 / 64, window)
+        check(decode(K, p, q, pos, 1.0 / 64, per, window), want, bar, 0.0)
+        p.vs[:, at] = old
+
+
+@pytest.mark.parametrize("n,per", [(33, 1), (700, 2), (30000, 1)])
+def test_a_large_value_scale_without_weight(K, n, per):
+    """A position whose value is 2^20 - 2^50 times the others' and whose weight is as far below: what is left of it counts,
+    and takes nothing from the others, wherever in the cache it lies."""
+    Hq, Hk, d = 32, 8, 128
+    g = gen(n)
+    p = Pool(g, n, Hk, d)
+    q = (0.2 * torch.randn(per, Hk, 1, d, generator=g, device=DEV)).expand(per, Hk, Hq // Hk, d).to(torch.bfloat16).contiguous()
+    pos = torch.arange(n - per, n, device=DEV, dtype=torch.int32)
+    for at in (0, n // 2, n - per):
+        for bits in (20, 35, 50):
+            # codes of the key against q's signs: a logit far under the others'
+            side = -torch.sign(q.float().mean(0)[:, 0]).to(torch.int8) * 7
+            keep = [t[:, at].clone() for t in (p.codes[0], p.ck, p.ks, p.vs)]
+            p.codes[0][:, at] = side
+            p.ck[:, at] = ((side[:, 0::2] + 8) | ((side[:, 1::2] + 8) << 4)).to(torch.uint8)
+            size = 7 * q.float().abs().sum(-1).amin() * 0.5
+            p.ks[:, at] = bits * math.log(2.0) / (size * 0.25)
+            p.vs[:, at] = 0.2 * 2.0**bits
+            want, bar = reference(p, q.view(per, Hq, d), pos, 0.25)
+            check(decode(K, p, q.view(per, Hq, d), pos, 0.25, per), want, bar, 1.0)
+            for t, k in zip((p.codes[0], p.ck, p.ks, p.vs), keep):
+                t[:, at] = k
+
+
+@pytest.mark.parametrize("spread", [2.0, 6.0, 10.0])
+@pytest.mark.parametrize("n", [40, 3000, 40000])
+@pytest.mark.parametrize("Hq,Hk,d", [(32, 8, 128), (16, 2, 64)])
+def test_value_scales_over_many_magnitudes(K, n, spread, Hq, Hk, d):
+    """Row scales from 2^-3 spread to 2^+3 spread, the largest anywhere; logits of ordinary size."""
+    for seed in range(3):
+        g = gen(seed + n)
+        vs = 0.2 * torch.exp2((spread * torch.randn(Hk, n, generator=g, device=DEV)).clamp(-35, 50))
+        p = Pool(g, n, Hk, d, vs)
+        q = torch.randn(2, Hq, d, generator=g, device=DEV).to(torch.bfloat16)
+        pos = torch.tensor([n - 1, n // 2], dtype=torch.int32, device=DEV)
+        want, bar = reference(p, q, pos, 1.0 / 16)
+        check(decode(K, p, q, pos, 1.0 / 16), want, bar, 10.0 if n < 10000 else 2.0)  # (the bound of the sums grows with n)
+
+
+@pytest.mark.parametrize("small", [1e-3, 1e-6, 1e-9, 1e-11])
+def test_small_values_keep_their_bits(K, small):
+    Hq, Hk, d = 32, 8, 128
+    for n in (50, 2000):
+        g = gen(n)
+        p = Pool(g, n, Hk, d)
+        p.vs *= small
+        q = torch.randn(1, Hq, d, generator=g, device=DEV).to(torch.bfloat16)
+        pos = torch.tensor([n - 1], dtype=torch.int32, device=DEV)
+        want, bar = reference(p, q, pos, 1.0 / 16)
+        check(decode(K, p, q, pos, 1.0 / 16), want, bar, 10.0)
+
+
 @pytest.mark.parametrize("scale", [0.25, -0.5, 1.0, 4.0])
 @pytest.mark.parametrize("n,per,window", [(37, 1, 0), (700, 4, 0), (4099, 3, 500), (40000, 1, 0)])
 @pytest.mark.parametrize("Hq,Hk,d", [(32, 8, 128), (16, 2, 64), (16, 1, 128)])
@@ -110,3 +181,35 @@ def test_peaked_softmax(K, n, per, window, scale, Hq, Hk, d):
     pos = torch.arange(n - per, n, device=DEV, dtype=torch.int32)
     want, bar = reference(p, q, pos, scale, window)
     check(decode(K, p, q, pos, scale, per, window), want, bar, 10.0)
+
+
+def test_weight_on_values_of_zero(K):
+    """The largest weight lies on a position whose value scale is zero; the others' share is 2^-20 and counts in full."""
+    Hq, Hk, d, n = 32, 8, 128, 1000
+    g = gen(2)
+    p = Pool(g, n, Hk, d)
+    q = torch.rand(1, Hq, d, generator=g, device=DEV).to(torch.bfloat16) + 0.5
+    p.codes[0][:, 7], p.ck[:, 7] = 7, 0xFF
+    p.vs[:, 7] = 0.0
+    p.ks[:, 7] = 20 * math.log(2.0) / (7 * q.float().sum(-1).mean().item() / 64)
+    pos = torch.tensor([n - 1], dtype=torch.int32, device=DEV)
+    want, bar = reference(p, q, pos, 1.0 / 64)
+    check(decode(K, p, q, pos, 1.0 / 64), want, bar, 10.0)
+    p.vs[:] = 0.0
+    assert (decode(K, p, q, pos, 1.0 / 64) == 0).all()
+
+
+def test_columns_do_not_depend_on_their_neighbours(K):
+    """The bits of a query head are the same whatever the other heads and rows of its group hold."""
+    Hq, Hk, d = 32, 8, 128
+    for n in (300, 30000):
+        g = gen(n)
+        p = Pool(g, n, Hk, d)
+        q = (2.0 * torch.randn(3, Hq, d, generator=g, device=DEV)).to(torch.bfloat16)
+        pos = torch.tensor([n - 1, n - 2, n - 1], dtype=torch.int32, device=DEV)
+        first = decode(K, p, q, pos, 1.0, 3)
+        other = q.clone()
+        other[1] = (5.0 * torch.randn(Hq, d, generator=g, device=DEV)).to(torch.bfloat16)
+        other[2, ::2] = float("nan")
+        second = decode(K, p, other, pos, 1.0, 3)
+        assert torch.equal(first[0], second[0]) and torch.equal(first[2, 1::2], second[2, 1::2])
