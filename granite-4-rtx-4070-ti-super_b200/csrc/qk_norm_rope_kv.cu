@@ -15,7 +15,8 @@
 // scale is f32(r max |y| / top) and the quotients are y (r / scale). r is a double, y is f32, off by at most 2^-22 of the
 // head's max |y|. In double are only y of the pairs that may hold the maximum (those within 2^-19 of it: hardly ever
 // more than one a head), and y of a pair with a quotient so near to the border of two codes that f32 may be wrong, where
-// the sign of fma(-(code +- 1/2), scale, |r y|) decides, which an fma gives exactly.
+// the sign of fma(-(code +- 1/2), scale, |r y|) decides, which an fma gives exactly. A head whose y may leave f32 on the way
+// (max |y| not in [2^-100, 2^126)) is all doubles.
 // V: value and amax have eight significant bits each, so a quotient top v / amax is a border exactly or further from it
 // than 1 / (2 top 255) >= 2^-16 of itself. Exact ones (v = amax / 2 is one in every third head) fall to the side that the
 // rounding of the scale pushes them to: the scale's reciprocal, moved by 2^-19 of itself to that side, decides all.
@@ -68,9 +69,19 @@ __device__ __forceinline__ float settle(float c, double x, float s) {
 __device__ __noinline__ float code_by_division(double x, float s, float top) {
   if (!(s > 0.0f)) return 0.0f;
   const double ax = fabs(x);
-  const float c = settle(fminf(rintf(static_cast<float>(ax / static_cast<double>(s))), top), ax, s);
+  const float c = fminf(settle(fminf(rintf(static_cast<float>(ax / static_cast<double>(s))), top), ax, s), top);  // (a subnormal scale may be short)
   return x < 0.0 ? -c : c;
 }
+
+// The larger, NaN where either is.
+__device__ __forceinline__ float max_or_nan(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+// Float bits of the largest |y| of a key head for which f32 does: [2^-100, 2^126), the products of weights and tables
+// included (what overflows shows as an infinity or NaN, what underflows is 2^-149 of 2^-100).
+constexpr unsigned kLeastY = (127u - 100u) << 23, kPastY = (127u + 126u) << 23;
 
 // Eight quotients x inv rounded to the nearest integer, as z = code + magic in f32: 1.5 2^23 (and the 8 of a nibble)
 // leaves the integer in the low bits of the sum. Returns the largest distance |quotient - code|.
@@ -124,6 +135,43 @@ __device__ __noinline__ double2 key_pair(const uint16_t* a, const uint16_t* b, c
   if (wa != nullptr) x *= bf16_to_f32(__ldg(wa + e)), y *= bf16_to_f32(__ldg(wb + e));
   const double cd = __ldg(c + e), sd = __ldg(s + e);
   return make_double2(x * cd - y * sd, y * cd + x * sd);
+}
+
+// A lane's part of a key head whose y may leave f32: everything in double, codes by division. (Doubles in key_pair instead:
+// 16384 rows 1.3 us more, for the registers of its callers.)
+struct FarHead {
+  uint2 lo, hi;
+  float scale;
+};
+template <int D, int BITS>
+__device__ __noinline__ FarHead far_key_head(const uint16_t* a, const uint16_t* b, const uint16_t* wa, const uint16_t* wb,
+                                             const float* c, const float* s, double rn, unsigned mask) {
+  constexpr float kTop = BITS == 4 ? 7.0f : 127.0f;
+  const auto pair = [&](int e) {
+    const double x = static_cast<double>(bf16_to_f32(a[e])) * (wa != nullptr ? bf16_to_f32(__ldg(wa + e)) : 1.0f);
+    const double y = static_cast<double>(bf16_to_f32(b[e])) * (wa != nullptr ? bf16_to_f32(__ldg(wb + e)) : 1.0f);
+    const double cd = __ldg(c + e), sd = __ldg(s + e);
+    return make_double2((x * cd - y * sd) * rn, (y * cd + x * sd) * rn);
+  };
+  double amax = 0.0;
+#pragma unroll 1
+  for (int e = 0; e < 8; ++e) {
+    const double2 y = pair(e);
+    amax = fmax(amax, fmax(fabs(y.x), fabs(y.y)));
+  }
+  __syncwarp(mask);
+#pragma unroll
+  for (int o = 1; o < D / 16; o <<= 1) amax = fmax(amax, __shfl_xor_sync(mask, amax, o));
+  FarHead h;
+  h.scale = static_cast<float>(amax * (1.0 / kTop));
+  float lo[8], hi[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const double2 y = pair(e);
+    lo[e] = code_by_division(y.x, h.scale, kTop) + kMagic<BITS>, hi[e] = code_by_division(y.y, h.scale, kTop) + kMagic<BITS>;
+  }
+  h.lo = pack_codes<BITS>(lo), h.hi = pack_codes<BITS>(hi);
+  return h;
 }
 
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
@@ -266,6 +314,8 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
       const bool is_k = head < p.Hk;
       const size_t srow = static_cast<size_t>(is_k ? head : head - p.Hk) * p.stride + kv_row;
       float lo[8], hi[8], zl[8], zh[8], sc;
+      uint2 cl, ch;
+      bool far_head = false;
       unpack8(raw[0], lo);
       unpack8(raw[kQkThreads], hi);
       if (is_k) {
@@ -301,45 +351,51 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
             const int e = 4 * h + i;
             const float a = lo[e], b = hi[e];
             lo[e] = fmaf(a, c[i], -(b * s[i])), hi[e] = fmaf(b, c[i], a * s[i]);
-            const unsigned key = (__float_as_uint(fmaxf(fabsf(lo[e]), fabsf(hi[e]))) & ~7u) | e;
+            const unsigned key = (__float_as_uint(max_or_nan(fabsf(lo[e]), fabsf(hi[e]))) & ~7u) | e;
             second = max(second, min(best, key)), best = max(best, key);
           }
         }
         unsigned top = best;
 #pragma unroll
         for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-        const unsigned floor_key = top > 32u ? top - 32u : 0u;  // what y lost, and the three bits
         const uint16_t* const ra = reinterpret_cast<const uint16_t*>(raw);
         const uint16_t* const rb = reinterpret_cast<const uint16_t*>(raw + kQkThreads);
         const float* const ct = reinterpret_cast<const float*>(cp);
         const float* const st = reinterpret_cast<const float*>(sp);
-        double amax = 0.0;
-        if (best >= floor_key) {
-          const bool several = second >= floor_key;
-          const int from = several ? 0 : best & 7, to = several ? 7 : from;
+        far_head = top - kLeastY >= kPastY - kLeastY;
+        if (far_head) {
+          const FarHead h = far_key_head<D, BITS>(ra, rb, wa, wa + D / 2, ct, st, rn, mask);
+          cl = h.lo, ch = h.hi, sc = h.scale;
+        } else {
+          const unsigned floor_key = top - 32u;  // what y lost, and the three bits
+          double amax = 0.0;
+          if (best >= floor_key) {
+            const bool several = second >= floor_key;
+            const int from = several ? 0 : best & 7, to = several ? 7 : from;
 #pragma unroll 1
-          for (int e = from; e <= to; ++e) {
-            const double2 y = key_pair(ra, rb, wa, wa + D / 2, ct, st, e);
-            amax = fmax(amax, fmax(fabs(y.x), fabs(y.y)));
-          }
-        }
-        __syncwarp(mask);
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) {
-          const double x = __shfl_xor_sync(mask, amax, o);
-          amax = x > amax ? x : amax;
-        }
-        sc = static_cast<float>(amax * rn * (1.0 / kTop));
-        const bool plain = sc > 1e-30f;
-        const float inv = plain ? static_cast<float>(rn) / sc : 0.0f;
-        const float far = fmaxf(round8<BITS>(lo, inv, zl), round8<BITS>(hi, inv, zh));
-        if (!plain || !(far < kNearBorder<BITS>)) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float dl = fabsf(lo[e] * inv - (zl[e] - kMagic<BITS>)), dh = fabsf(hi[e] * inv - (zh[e] - kMagic<BITS>));
-            if (!plain || !(fmaxf(dl, dh) < 2.0f * kNearBorder<BITS> - 0.5f)) {  // (these products may be rounded elsewhere)
+            for (int e = from; e <= to; ++e) {
               const double2 y = key_pair(ra, rb, wa, wa + D / 2, ct, st, e);
-              zl[e] = settled<BITS>(zl[e], y.x * rn, sc, plain), zh[e] = settled<BITS>(zh[e], y.y * rn, sc, plain);
+              amax = fmax(amax, fmax(fabs(y.x), fabs(y.y)));
+            }
+          }
+          __syncwarp(mask);
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1) {
+            const double x = __shfl_xor_sync(mask, amax, o);
+            amax = x > amax ? x : amax;
+          }
+          sc = static_cast<float>(amax * rn * (1.0 / kTop));
+          const bool plain = sc > 1e-30f;
+          const float inv = plain ? static_cast<float>(rn) / sc : 0.0f;
+          const float far = fmaxf(round8<BITS>(lo, inv, zl), round8<BITS>(hi, inv, zh));
+          if (!plain || !(far < kNearBorder<BITS>)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float dl = fabsf(lo[e] * inv - (zl[e] - kMagic<BITS>)), dh = fabsf(hi[e] * inv - (zh[e] - kMagic<BITS>));
+              if (!plain || !(fmaxf(dl, dh) < 2.0f * kNearBorder<BITS> - 0.5f)) {  // (these products may be rounded elsewhere)
+                const double2 y = key_pair(ra, rb, wa, wa + D / 2, ct, st, e);
+                zl[e] = settled<BITS>(zl[e], y.x * rn, sc, plain), zh[e] = settled<BITS>(zh[e], y.y * rn, sc, plain);
+              }
             }
           }
         }
@@ -360,7 +416,7 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
           for (int e = 0; e < 8; ++e) zl[e] = settled<BITS>(zl[e], lo[e], sc, false), zh[e] = settled<BITS>(zh[e], hi[e], sc, false);
         }
       }
-      const uint2 cl = pack_codes<BITS>(zl), ch = pack_codes<BITS>(zh);
+      if (!far_head) cl = pack_codes<BITS>(zl), ch = pack_codes<BITS>(zh);
       if (j == 0) (is_k ? p.k_scale : p.v_scale)[srow] = sc;
       uint8_t* cache = (is_k ? p.cache_k : p.cache_v) + srow * (D * BITS / 8);
       if (BITS == 4) {
