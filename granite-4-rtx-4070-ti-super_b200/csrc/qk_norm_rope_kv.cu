@@ -16,7 +16,8 @@
 // head's max |y|. In double are only y of the pairs that may hold the maximum (those within 2^-19 of it: hardly ever
 // more than one a head), and y of a pair with a quotient so near to the border of two codes that f32 may be wrong, where
 // the sign of fma(-(code +- 1/2), scale, |r y|) decides, which an fma gives exactly. A head whose y may leave f32 on the way
-// (max |y| not in [2^-100, 2^126)) is all doubles.
+// (max |y| not in [2^-100, 2^126)) is all doubles. A key or value head that holds an infinity or a NaN has codes 0 and a scale
+// that is not finite, so that whoever reads it gets NaN.
 // V: value and amax have eight significant bits each, so a quotient top v / amax is a border exactly or further from it
 // than 1 / (2 top 255) >= 2^-16 of itself. Exact ones (v = amax / 2 is one in every third head) fall to the side that the
 // rounding of the scale pushes them to: the scale's reciprocal, moved by 2^-19 of itself to that side, decides all.
@@ -65,9 +66,9 @@ __device__ __forceinline__ float settle(float c, double x, float s) {
   return c > 0.0f && fma(-static_cast<double>(c - 0.5f), static_cast<double>(s), x) < 0.0 ? c - 1.0f : c;
 }
 
-// A code under a scale whose reciprocal, or the fma's difference, may lie outside of f32 (or that is zero).
+// A code under a scale whose reciprocal, or the fma's difference, may lie outside of f32 (or that is zero or not finite).
 __device__ __noinline__ float code_by_division(double x, float s, float top) {
-  if (!(s > 0.0f)) return 0.0f;
+  if (!(s > 0.0f && s < INFINITY)) return 0.0f;
   const double ax = fabs(x);
   const float c = fminf(settle(fminf(rintf(static_cast<float>(ax / static_cast<double>(s))), top), ax, s), top);  // (a subnormal scale may be short)
   return x < 0.0 ? -c : c;
@@ -154,16 +155,18 @@ __device__ __noinline__ FarHead far_key_head(const uint16_t* a, const uint16_t* 
     return make_double2((x * cd - y * sd) * rn, (y * cd + x * sd) * rn);
   };
   double amax = 0.0;
+  bool numbers = true;
 #pragma unroll 1
   for (int e = 0; e < 8; ++e) {
     const double2 y = pair(e);
     amax = fmax(amax, fmax(fabs(y.x), fabs(y.y)));
+    numbers = numbers && fabs(y.x) < INFINITY && fabs(y.y) < INFINITY;
   }
-  __syncwarp(mask);
+  numbers = __all_sync(mask, numbers);
 #pragma unroll
   for (int o = 1; o < D / 16; o <<= 1) amax = fmax(amax, __shfl_xor_sync(mask, amax, o));
   FarHead h;
-  h.scale = static_cast<float>(amax * (1.0 / kTop));
+  h.scale = numbers ? static_cast<float>(amax * (1.0 / kTop)) : __int_as_float(0x7fc00000);
   float lo[8], hi[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -402,11 +405,11 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
       } else {
         float amax = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
+        for (int e = 0; e < 8; ++e) amax = max_or_nan(amax, max_or_nan(fabsf(lo[e]), fabsf(hi[e])));
 #pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
+        for (int o = 1; o < kLanes; o <<= 1) amax = max_or_nan(amax, __shfl_xor_sync(mask, amax, o));
         sc = __fdiv_rn(amax, static_cast<float>(kTop));  // eight significant bits over 7 or 127: never half way between floats
-        const bool plain = sc > 1e-30f;
+        const bool plain = sc > 1e-30f && sc < INFINITY;
         const float side = fmaf(sc, static_cast<float>(kTop), -amax) > 0.0f ? 1.0f - 1.0f / 524288.0f : 1.0f + 1.0f / 524288.0f;
         const float inv = plain ? __fdividef(side, sc) : 0.0f;
         round8<BITS>(lo, inv, zl);

@@ -288,9 +288,10 @@ int granite4_kernel_rope_kv_int8_paged(const uint16_t* d_qkv, const float* d_cos
  * bits 8: top 127, the int8 pool [Hk][stride][d] of the entry points above. bits 4:
  * top 7, uint8 [Hk][stride][d / 2], code + 8 in a nibble, the even dim in the low half
  * of its byte. Scales are f32 [Hk][stride] for both. Codes are those of exact
- * arithmetic on the bf16 inputs and the f32 tables (a head that holds an infinity
- * or a NaN gets unspecified codes, one with a NaN an unspecified scale too; a normed
- * query head's squares are summed in f32, so its values have to stay under 1e18). d is 64 or 128; eps > 0; norm weights,
+ * arithmetic on the bf16 inputs and the f32 tables. A key or value head that holds
+ * an infinity or a NaN gets codes 0 and a scale that is not finite: it reads back as
+ * NaN, and attention gives NaN to the rows that see it. (A normed query head's squares
+ * are summed in f32, so its values have to stay under 1e18.) d is 64 or 128; eps > 0; norm weights,
  * tables, qkv, q_rot and caches 16-byte aligned. d_pos_rows / d_kv_rows as in
  * granite4_kernel_rope_kv_int8_paged: a row with an index out of range is skipped;
  * pool rows of one call are distinct. For granite4_kernel_kv_move a 4-bit pool is one

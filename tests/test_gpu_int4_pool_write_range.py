@@ -89,3 +89,59 @@ def test_keys_and_values_near_the_ends_of_f32(K, x, w, eps, d, bits):
     codes, scales = formula(qkv[:, Hq + Hk:].double(), None, eps, None, None, bits)
     assert torch.equal(c.scales[1], scales)
     assert torch.equal(c.codes[1], codes)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("side", ["k", "v"])
+@pytest.mark.parametrize("bits,d", [(4, 128), (4, 64), (8, 128), (8, 64)])
+def test_a_head_that_is_not_a_number_stays_one(K, bits, d, side, norm, bad):
+    """Codes 0 and a scale that is not finite; the row reads back as NaN; every other head as without it."""
+    rows, Hq, Hk = 40, 4, 2
+    g = gen(d + bits)
+    qkv = torch.randn(rows, Hq + 2 * Hk, d, generator=g, device=DEV).to(torch.bfloat16)
+    wk = (1 + 0.1 * torch.randn(d, generator=g, device=DEV)).to(torch.bfloat16) if norm else None
+    clean = Case(K, qkv, wk, 1e-6, Hq, Hk, d, bits)
+    spoilt = qkv.clone()
+    hit = torch.zeros(rows, Hk, dtype=torch.bool, device=DEV)
+    for row, dim in ((0, 0), (0, d - 1), (3, 5), (17, d // 2 + 1), (39, d // 2 - 1)):  # row 0 is not turned
+        head = (row + dim) % Hk
+        spoilt[row, Hq + (Hk if side == "v" else 0) + head, dim] = bad
+        hit[row, head] = True
+    c = Case(K, spoilt, wk, 1e-6, Hq, Hk, d, bits)
+    mine, other = (0, 1) if side == "k" else (1, 0)
+    assert not torch.isfinite(c.scales[mine][hit]).any() and (c.codes[mine][hit] == 0).all()
+    assert torch.equal(c.scales[mine][~hit], clean.scales[mine][~hit]) and torch.equal(c.codes[mine][~hit], clean.codes[mine][~hit])
+    assert torch.equal(c.scales[other], clean.scales[other]) and torch.equal(c.codes[other], clean.codes[other])
+    assert torch.equal(c.q, clean.q)
+    outs = [torch.empty(rows, Hk, d, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    at = torch.arange(rows, dtype=torch.int32, device=DEV)
+    assert K.kv_read_paged(c.ck, c.cv, c.ks, c.vs, at, bits, Hk, d, rows, *outs) == 0
+    assert outs[mine][hit].isnan().all() and torch.isfinite(outs[mine][~hit]).all() and torch.isfinite(outs[other]).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("side", ["k", "v"])
+@pytest.mark.parametrize("rows", [40, 100, 260])
+def test_what_is_not_a_number_reaches_who_sees_it(K, rows, side, bad):
+    """Written, then attended to by rows one by one, in groups and as a chunk: the rows before it are as without it."""
+    Hq, Hk, d = 8, 2, 128
+    g = gen(rows)
+    qkv = torch.randn(rows, Hq + 2 * Hk, d, generator=g, device=DEV).to(torch.bfloat16)
+    first = rows // 2 + 3
+    spoilt = qkv.clone()
+    spoilt[first, Hq + (Hk if side == "v" else 0) + 1, 9] = bad
+    pos = torch.arange(rows, dtype=torch.int32, device=DEV)
+    seen = []
+    for x in (qkv, spoilt):
+        c = Case(K, x, None, 1e-6, Hq, Hk, d, 4)
+        outs = [torch.empty(rows, Hq, d, dtype=torch.bfloat16, device=DEV) for _ in range(3)]
+        pool = (c.ck, c.cv, c.ks, c.vs)
+        assert K.attn_decode_int4_paged(c.q, *pool, pos, Hq, Hk, d, rows, rows, 1.0 / 64, outs[0]) == 0
+        assert K.attn_decode_int4_paged(c.q, *pool, pos, Hq, Hk, d, rows, rows, 1.0 / 64, outs[1], rows_per_group=4) == 0
+        assert K.prefill_attention_int4(c.q, 1.0 / 64, Hq, Hk, d, 0, rows, outs[2], *pool) == 0
+        seen.append(outs)
+    for a, b in zip(*seen):
+        assert torch.isfinite(a).all()
+        assert b[first:, 4:].isnan().all()
+        assert torch.equal(a[:first], b[:first]) and torch.equal(a[:, :4], b[:, :4])
