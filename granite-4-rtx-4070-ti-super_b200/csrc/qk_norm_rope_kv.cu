@@ -57,10 +57,6 @@ template <int BITS>
 constexpr float kNearBorder = 0.5f - (BITS == 4 ? 1.0f / 131072.0f : 1.0f / 16384.0f);
 
 // |x| against the borders of code c: the code itself.
-__device__ __forceinline__ float settle(float c, float x, float s) {
-  if (fmaf(-(c + 0.5f), s, x) >= 0.0f) return c + 1.0f;
-  return c > 0.0f && fmaf(-(c - 0.5f), s, x) < 0.0f ? c - 1.0f : c;
-}
 __device__ __forceinline__ float settle(float c, double x, float s) {
   if (fma(-static_cast<double>(c + 0.5f), static_cast<double>(s), x) >= 0.0) return c + 1.0f;
   return c > 0.0f && fma(-static_cast<double>(c - 0.5f), static_cast<double>(s), x) < 0.0 ? c - 1.0f : c;
@@ -104,12 +100,12 @@ __device__ __forceinline__ float round8(const float (&x)[8], float inv, float (&
   }
   return far;
 }
-// z settled against the exact value x.
-template <int BITS, typename T>
-__device__ __forceinline__ float settled(float z, T x, float s, bool plain) {
+// z of a key settled against its exact value x.
+template <int BITS>
+__device__ __forceinline__ float settled(float z, double x, float s, bool plain) {
   if (!plain) return code_by_division(x, s, BITS == 4 ? 7.0f : 127.0f) + kMagic<BITS>;
-  const float c = settle(fabsf(z - kMagic<BITS>), x < T(0) ? -x : x, s);
-  return (x < T(0) ? -c : c) + kMagic<BITS>;
+  const float c = settle(fabsf(z - kMagic<BITS>), fabs(x), s);
+  return (x < 0.0 ? -c : c) + kMagic<BITS>;
 }
 // The words of the pool: 4 bits, code + 8, or 8.
 template <int BITS>
@@ -416,7 +412,7 @@ __global__ void __launch_bounds__(kQkThreads, kQkCtas) qk_norm_rope_kv_kernel(co
         round8<BITS>(hi, inv, zh);
         if (!plain) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) zl[e] = settled<BITS>(zl[e], lo[e], sc, false), zh[e] = settled<BITS>(zh[e], hi[e], sc, false);
+          for (int e = 0; e < 8; ++e) zl[e] = code_by_division(lo[e], sc, kTop) + kMagic<BITS>, zh[e] = code_by_division(hi[e], sc, kTop) + kMagic<BITS>;
         }
       }
       if (!far_head) cl = pack_codes<BITS>(zl), ch = pack_codes<BITS>(zh);
