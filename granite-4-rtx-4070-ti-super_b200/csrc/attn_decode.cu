@@ -643,7 +643,7 @@ namespace g4 {
 // csrc/attn_prefill.cu
 int attn_prefill_flash(const char* fn, const uint16_t* d_q, float scale, int Hq, int Hk, int base_pos, int rows,
                        int stride, uint16_t* d_out, const int8_t* d_ck, const int8_t* d_cv, const float* d_ks,
-                       const float* d_vs, const int* d_pt);
+                       const float* d_vs, const int* d_pt, const float* d_v_tops, int n_tops);
 }  // namespace g4
 
 namespace g4 {
@@ -818,7 +818,7 @@ int granite4_prefill_attention_int8(const uint16_t* d_q_rot, float scale, int Hq
     if (!g4::aligned16(d_cache_k8) || !g4::aligned16(d_cache_v8) || !g4::aligned16(d_q_rot))
       return g4::fail(fn, "q and the caches must be 16-byte aligned");
     return g4::attn_prefill_flash(fn, d_q_rot, scale, Hq, Hk, base_pos, rows, stride, d_out, d_cache_k8, d_cache_v8,
-                                  d_k_scale, d_v_scale, d_pt);
+                                  d_k_scale, d_v_scale, d_pt, nullptr, 0);
   }
   g4::AttnRows r;
   r.base_pos = base_pos, r.d_pt = d_pt;

@@ -57,8 +57,13 @@
 namespace g4 {
 
 // kv_read.cu
+int widen_tops(long long n);
 int widen_int4(const char* fn, const uint8_t* ck, const uint8_t* cv, const float* ks, const float* vs, const int* pt,
-               int Hk, long long stride, long long n, int8_t* ok, int8_t* ov, float* oks, float* ovs);
+               int Hk, long long stride, long long n, int8_t* ok, int8_t* ov, float* oks, float* ovs, float* tops);
+// attn_prefill.cu
+int attn_prefill_flash(const char* fn, const uint16_t* d_q, float scale, int Hq, int Hk, int base_pos, int rows,
+                       int stride, uint16_t* d_out, const int8_t* d_ck, const int8_t* d_cv, const float* d_ks,
+                       const float* d_vs, const int* d_pt, const float* d_v_tops, int n_tops);
 
 namespace {
 
@@ -964,7 +969,7 @@ bool widens(int rows, int base_pos, int Hq, int Hk, int d) {
   return rows < 64 ? base_pos <= 192 - rows : rows > 192 || base_pos > 768 - rows;
 }
 int prefill_group(int Hq, int Hk) { return std::max(1, 16 / (Hq / Hk)); }
-long long widened_bytes(long long n, int Hk) { return (2 * n * Hk * (128 + 4) + 63) / 16 * 16; }
+long long widened_bytes(long long n, int Hk) { return (2 * n * Hk * (128 + 4) + 4ll * Hk * widen_tops(n) + 63) / 16 * 16; }
 
 }  // namespace
 }  // namespace g4
@@ -1018,7 +1023,8 @@ int granite4_prefill_attention_int4(const uint16_t* d_q_rot, float scale, int Hq
   if (!g4::aligned16(d_q_rot) || !g4::aligned16(d_cache_k) || !g4::aligned16(d_cache_v))
     return g4::fail(fn, "q and the caches must be 16-byte aligned");
   const int n = base_pos + rows;
-  if (g4::widens(rows, base_pos, Hq, Hk, d)) {
+  // (an output that those kernels cannot store to in their words takes the decode form)
+  if (g4::widens(rows, base_pos, Hq, Hk, d) && reinterpret_cast<uintptr_t>(d_out) % (rows < 64 ? 4 : 16) == 0) {
     if (d_scratch == nullptr || !g4::aligned16(d_scratch) || scratch_bytes < g4::widened_bytes(n, Hk))
       return g4::fail(fn, "scratch missing, misaligned or smaller than the size the scratch query returns");
     const size_t codes = static_cast<size_t>(n) * Hk * 128, scales = static_cast<size_t>(n) * Hk;
@@ -1026,9 +1032,11 @@ int granite4_prefill_attention_int4(const uint16_t* d_q_rot, float scale, int Hq
     int8_t* cv = ck + codes;
     float* ks = reinterpret_cast<float*>(cv + codes);
     float* vs = ks + scales;
-    if (g4::widen_int4(fn, d_cache_k, d_cache_v, d_k_scale, d_v_scale, d_pt, Hk, stride, n, ck, cv, ks, vs) != 0) return -1;
-    return granite4_prefill_attention_int8(d_q_rot, scale, Hq, Hk, d, base_pos, rows, n, d_out, ck, cv, ks, vs, nullptr,
-                                           nullptr, 0);
+    float* tops = vs + scales;
+    if (g4::widen_int4(fn, d_cache_k, d_cache_v, d_k_scale, d_v_scale, d_pt, Hk, stride, n, ck, cv, ks, vs, tops) != 0) return -1;
+    const int rc = g4::attn_prefill_flash(fn, d_q_rot, scale, Hq, Hk, base_pos, rows, n, d_out, ck, cv, ks, vs, nullptr, tops,
+                                          g4::widen_tops(n));
+    if (rc <= 0) return rc;
   }
   g4::Int4AttnParams p{};
   p.q = d_q_rot, p.ck = d_cache_k, p.cv = d_cache_v, p.ks = d_k_scale, p.vs = d_v_scale, p.out = d_out;

@@ -55,6 +55,8 @@ struct PrefillParams {
   int rows, base_pos, Hq, Hk;
   long long stride;
   float scale_log2;  // softmax scale x log2(e)
+  const float* v_tops;  // attn_prefill2_kernel: [Hk][n_tops] maxima over the value scales (NULL: V is taken as it is)
+  int n_tops;
 };
 
 struct PrefillSmem {
@@ -296,6 +298,7 @@ constexpr int kWarps2 = 4;  // warp w: row tile w % 2, output dims 64 (w / 2) ..
 struct PrefillSmem2 {
   PrefillSmem t;
   __half qh[kQRows2][kHPitch];
+  uint32_t v_top;  // the largest of p.v_tops, as float bits
 };
 
 __global__ void __launch_bounds__(kWarps2 * 32, 2) attn_prefill2_kernel(const PrefillParams p) {
@@ -333,6 +336,18 @@ __global__ void __launch_bounds__(kWarps2 * 32, 2) attn_prefill2_kernel(const Pr
   };
   gather(0, 0);
 
+  // a power of two on V and back, as in the tensor-core form
+  if (tid == 0) sm2.v_top = 0u;
+  if (p.v_tops != nullptr) {
+    uint32_t top = 0u;
+    for (int i = tid; i < p.n_tops; i += kWarps2 * 32) top = max(top, __float_as_uint(__ldg(p.v_tops + static_cast<size_t>(hkv) * p.n_tops + i)));
+    top = __reduce_max_sync(0xffffffffu, top);
+    __syncthreads();
+    if (lane == 0) atomicMax(&sm2.v_top, top);
+  }
+  __syncthreads();
+  const float v_up = v_up_factor(sm2.v_top);
+
   // the Q rows -> fp16 in shared memory (rows past the chunk repeat the last row); read behind the tile loop's barrier
   for (int i = tid; i < kQRows2 * (kD / 8); i += kWarps2 * 32) {
     const int row = i >> 4, piece = i & 15;
@@ -358,7 +373,7 @@ __global__ void __launch_bounds__(kWarps2 * 32, 2) attn_prefill2_kernel(const Pr
       const int item = it * (kWarps2 * 32) + tid, row = item >> 4, piece = item & 15;
       const uint2 rk = *reinterpret_cast<const uint2*>(&sm.raw_k[stage][row][piece * 8]);
       const uint2 rv = *reinterpret_cast<const uint2*>(&sm.raw_v[stage][row][piece * 8]);
-      const __half2 vs2 = __float2half2_rn(sm.vs[stage][row]);
+      const __half2 vs2 = __float2half2_rn(sm.vs[stage][row] * v_up);
       __half2 kh2[4], vh2[4];
       pf_codes4(rk.x, kh2[0], kh2[1]), pf_codes4(rk.y, kh2[2], kh2[3]);
       pf_codes4(rv.x, vh2[0], vh2[1]), pf_codes4(rv.y, vh2[2], vh2[3]);
@@ -456,8 +471,9 @@ __global__ void __launch_bounds__(kWarps2 * 32, 2) attn_prefill2_kernel(const Pr
       l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
       l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
     }
-    const float inv_a = l_run[0] > 0.0f ? 1.0f / l_run[0] : 0.0f;
-    const float inv_b = l_run[1] > 0.0f ? 1.0f / l_run[1] : 0.0f;
+    const float v_down = v_down_factor(sm2.v_top);
+    const float inv_a = (l_run[0] > 0.0f ? 1.0f / l_run[0] : 0.0f) * v_down;
+    const float inv_b = (l_run[1] > 0.0f ? 1.0f / l_run[1] : 0.0f) * v_down;
     const int ra = mt * 16 + g, rb = ra + 8;
     uint16_t* out_a = p.out + (static_cast<size_t>(r0 + ra) * p.Hq + head) * kD + nb0 * 8 + 2 * t;
     uint16_t* out_b = p.out + (static_cast<size_t>(r0 + rb) * p.Hq + head) * kD + nb0 * 8 + 2 * t;
@@ -474,17 +490,19 @@ __global__ void __launch_bounds__(kWarps2 * 32, 2) attn_prefill2_kernel(const Pr
 // csrc/attn_prefill_tc.cu: the tcgen05 form (0 done, 1 not available here, -1 launch error)
 int attn_prefill_tc(const char* fn, const uint16_t* d_q, float scale, int Hq, int Hk, int base_pos, int rows,
                     int stride, uint16_t* d_out, const int8_t* d_ck, const int8_t* d_cv, const float* d_ks,
-                    const float* d_vs, const int* d_pt);
+                    const float* d_vs, const int* d_pt, const float* d_v_tops, int n_tops);
 
 // Launch of the flash form for a whole chunk; arguments as granite4_prefill_attention_int8 (validated there).
 // Chunks of 64 rows or more run on the tcgen05 kernel; the mma.sync kernels below take shorter ones, an output
-// that is not 16-byte aligned and, with G4_PREFILL_TC=0, everything (A/B runs, tests that compare the two).
+// that is not 16-byte aligned and, with G4_PREFILL_TC=0, everything (A/B runs, tests that compare the two). With
+// d_v_tops (the 4-bit pool's chunks) 1 where none of the forms that know it is to be had.
 int attn_prefill_flash(const char* fn, const uint16_t* d_q, float scale, int Hq, int Hk, int base_pos, int rows,
                        int stride, uint16_t* d_out, const int8_t* d_ck, const int8_t* d_cv, const float* d_ks,
-                       const float* d_vs, const int* d_pt) {
+                       const float* d_vs, const int* d_pt, const float* d_v_tops, int n_tops) {
   const char* tc_env = std::getenv("G4_PREFILL_TC");
   if (rows >= 64 && aligned16(d_out) && !(tc_env != nullptr && tc_env[0] == '0')) {
-    const int rc = attn_prefill_tc(fn, d_q, scale, Hq, Hk, base_pos, rows, stride, d_out, d_ck, d_cv, d_ks, d_vs, d_pt);
+    const int rc = attn_prefill_tc(fn, d_q, scale, Hq, Hk, base_pos, rows, stride, d_out, d_ck, d_cv, d_ks, d_vs, d_pt,
+                                   d_v_tops, n_tops);
     if (rc <= 0) return rc;
   }
   static bool attr_set[64];
@@ -501,6 +519,7 @@ int attn_prefill_flash(const char* fn, const uint16_t* d_q, float scale, int Hq,
   p.q = d_q, p.ck = d_ck, p.cv = d_cv, p.ks = d_ks, p.vs = d_vs, p.pt = d_pt, p.out = d_out;
   p.rows = rows, p.base_pos = base_pos, p.Hq = Hq, p.Hk = Hk, p.stride = stride;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.v_tops = d_v_tops, p.n_tops = n_tops;
   // Below 64 rows a few CTAs walk the whole prefix, and one head per CTA spreads them over more SMs. A longer chunk
   // has CTAs enough: there the conversion of K and V is shared by four heads (2048 rows 209 us, 384 with one head per
   // CTA; 8192 rows 2.36 ms and 5.3). G4_PREFILL_ROWS32=0: 16 positions and four heads always.
@@ -510,6 +529,7 @@ int attn_prefill_flash(const char* fn, const uint16_t* d_q, float scale, int Hq,
     G4_LAUNCH_PDL(fn, attn_prefill2_kernel, grid, dim3(kWarps2 * 32), sizeof(PrefillSmem2), current_stream(), p);
     return 0;
   }
+  if (d_v_tops != nullptr) return 1;
   const dim3 grid(static_cast<unsigned>((rows + kQRows - 1) / kQRows), static_cast<unsigned>(Hk));
   G4_LAUNCH_PDL(fn, attn_prefill_kernel, grid, dim3(kPfWarps * 32), sizeof(PrefillSmem), current_stream(), p);
   return 0;

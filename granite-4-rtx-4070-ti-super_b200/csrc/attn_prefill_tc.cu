@@ -98,6 +98,7 @@ struct TcSmem {
   uint64_t s_full[kRowTiles][2], p_full[kRowTiles][2], pv_done[kRowTiles][2];
   uint64_t q_ready;
   uint32_t q_amax;  // max |q| over the CTA's rows, as float bits
+  uint32_t v_top;   // the largest of p.v_tops, as float bits
   uint32_t tmem_base;
   int abort;
 };
@@ -115,6 +116,8 @@ struct TcParams {
   unsigned int* status;
   int rows, base_pos, Hq, Hk;
   int splits;  // CTAs of a cluster that share a block's cache range
+  const float* v_tops;  // [Hk][n_tops] maxima over the value scales (NULL: V is taken as it is)
+  int n_tops;
   long long stride;
   float scale_log2;
 };
@@ -223,6 +226,9 @@ __device__ __forceinline__ int q_exponent(uint32_t amax_bits) {
 __device__ __forceinline__ float q_down_factor(uint32_t amax_bits) { return __int_as_float((127 - q_exponent(amax_bits)) << 23); }
 __device__ __forceinline__ float q_up_factor(uint32_t amax_bits) { return __int_as_float((127 + q_exponent(amax_bits)) << 23); }
 
+// Where the largest value scale of the head is known, V is scaled by a power of two (v_up_factor, g4_math.cuh) on its way to f16,
+// so that small values keep their bits, and the output scaled back: exact both ways.
+template <bool TOPS>
 __global__ void __launch_bounds__(kThreads, 1) attn_prefill_tc_kernel(const TcParams p) {
   pdl_begin();
   extern __shared__ uint8_t smem_raw[];
@@ -266,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_tc_kernel(const TcPa
     }
     mbar_init(&sm->q_ready, 8);
     sm->abort = 0;
-    sm->q_amax = 0u;
+    sm->q_amax = sm->v_top = 0u;
     mbar_init_fence();
     fence_async_smem();
   }
@@ -380,10 +386,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_tc_kernel(const TcPa
   } else if (warp < 4 || warp >= 12) {
     // ---- converters -----------------------------------------------------------------------------
     const int c = (warp < 4 ? warp - 2 : warp - 10) * 32 + lane;  // 0..127
+    // V's power of two; the softmax warps read it behind the last P V, or behind the exchange
+    if (TOPS) {
+      uint32_t top = 0u;
+#pragma unroll 1
+      for (int i = c; i < p.n_tops; i += 128) top = max(top, __float_as_uint(__ldg(p.v_tops + static_cast<size_t>(hkv) * p.n_tops + i)));
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) atomicMax(&sm->v_top, top);
+      asm volatile("bar.sync 2, 128;" ::: "memory");  // the four converter warps
+    }
     // the logit factor of a column: its K scale x (softmax scale x log2 e x 2^qexp); the last two are
     // known once the Q rows have been scaled
     bool okc = wait_tc(&sm->q_ready, 0, sm, p.status);
-    const float col_scale = p.scale_log2 * q_up_factor(sm->q_amax);
+    const float col_scale = p.scale_log2 * q_up_factor(sm->q_amax), v_up = TOPS ? v_up_factor(sm->v_top) : 1.0f;
     for (int j = 0; j < n_kv && okc; ++j) {
       const int s = j % kRaw, b = j % kBufs;
       if (!wait_tc(&sm->raw_full[s], (j / kRaw) & 1, sm, p.status)) break;
@@ -412,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_tc_kernel(const TcPa
         const int half = piece >> 2, ch = (piece & 3) * 2, flip = half;
         uint4 lo, hi;
         codes16_to_half(raw[i], lo, hi);
-        const __half2 sv = __float2half2_rn(sm->raw_vs[s][row]);  // V = code x scale, rounded to f16
+        const __half2 sv = __float2half2_rn(TOPS ? sm->raw_vs[s][row] * v_up : sm->raw_vs[s][row]);  // V = code x scale, rounded to f16
         mul8(lo, sv), mul8(hi, sv);
         uint8_t* vt = sm->v16[b] + half * (kKvTileBytes / 2);
         *reinterpret_cast<uint4*>(vt + sw128(row, ch + flip)) = flip ? hi : lo;
@@ -611,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_tc_kernel(const TcPa
           o[0] += x.x * w, o[1] += x.y * w, o[2] += x.z * w, o[3] += x.w * w;
           o[4] += y.x * w, o[5] += y.y * w, o[6] += y.z * w, o[7] += y.w * w;
         }
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float inv = (l > 0.0f ? 1.0f / l : 0.0f) * (TOPS ? v_down_factor(sm->v_top) : 1.0f);
         uint4 u;
         u.x = pack_bf16x2(o[0] * inv, o[1] * inv), u.y = pack_bf16x2(o[2] * inv, o[3] * inv);
         u.z = pack_bf16x2(o[4] * inv, o[5] * inv), u.w = pack_bf16x2(o[6] * inv, o[7] * inv);
@@ -619,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_tc_kernel(const TcPa
       }
     } else if (ok && n_mine > 0) {
       // ---- the finished row: O / l -> bf16
-      const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+      const float inv = (l_run > 0.0f ? 1.0f / l_run : 0.0f) * (TOPS ? v_down_factor(sm->v_top) : 1.0f);
       uint16_t* dst = p.out + (static_cast<size_t>(live ? crow : 0) * p.Hq + hkv * 4 + hl) * kD;
 #pragma unroll 1
       for (int oc = 0; oc < 4; ++oc) {
@@ -677,8 +692,8 @@ static int resident_ctas(int splits) {
   int n = 0;
   if (splits == 1) {
     n = sm_count();
-  } else if (splits <= 8 || cudaFuncSetAttribute(attn_prefill_tc_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) ==
-                                cudaSuccess) {
+  } else if (splits <= 8 || (cudaFuncSetAttribute(attn_prefill_tc_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                             cudaFuncSetAttribute(attn_prefill_tc_kernel<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess)) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(splits)), cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kTcSmemBytes;
@@ -686,7 +701,7 @@ static int resident_ctas(int splits) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = static_cast<unsigned>(splits), attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr, cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, attn_prefill_tc_kernel, &cfg) != cudaSuccess) n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, attn_prefill_tc_kernel<false>, &cfg) != cudaSuccess) n = 0;
     n *= splits;
   }
   (void)cudaGetLastError();
@@ -733,25 +748,26 @@ static int plan_splits(int rows, int base_pos, int Hk) {
 // mma.sync form), 0 on success, -1 on a launch error.
 int attn_prefill_tc(const char* fn, const uint16_t* d_q, float scale, int Hq, int Hk, int base_pos, int rows,
                     int stride, uint16_t* d_out, const int8_t* d_ck, const int8_t* d_cv, const float* d_ks,
-                    const float* d_vs, const int* d_pt) {
+                    const float* d_vs, const int* d_pt, const float* d_v_tops, int n_tops) {
   unsigned int* status = device_status_ptr();
   if (status == nullptr) return 1;
   static std::atomic<bool> attr_set[64];
   int dev = -1;
   G4_CUDA_TRY(fn, cudaGetDevice(&dev));
   if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_relaxed)) {
-    G4_CUDA_TRY(fn, cudaFuncSetAttribute(attn_prefill_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(kTcSmemBytes)));
+    for (auto* k : {attn_prefill_tc_kernel<false>, attn_prefill_tc_kernel<true>})
+      G4_CUDA_TRY(fn, cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTcSmemBytes)));
     attr_set[dev].store(true, std::memory_order_relaxed);
   }
   TcParams p{};
   p.q = d_q, p.ck = d_ck, p.cv = d_cv, p.ks = d_ks, p.vs = d_vs, p.pt = d_pt, p.out = d_out, p.status = status;
   p.rows = rows, p.base_pos = base_pos, p.Hq = Hq, p.Hk = Hk, p.stride = stride;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.splits = plan_splits(rows, base_pos, Hk);
+  p.splits = plan_splits(rows, base_pos, Hk), p.v_tops = d_v_tops, p.n_tops = n_tops;
   const dim3 grid(static_cast<unsigned>((rows + kCtaPos - 1) / kCtaPos * p.splits), static_cast<unsigned>(Hk));
+  auto* const kernel = d_v_tops != nullptr ? attn_prefill_tc_kernel<true> : attn_prefill_tc_kernel<false>;
   if (p.splits == 1) {
-    G4_LAUNCH_PDL(fn, attn_prefill_tc_kernel, grid, dim3(kThreads), kTcSmemBytes, current_stream(), p);
+    G4_LAUNCH_PDL(fn, kernel, grid, dim3(kThreads), kTcSmemBytes, current_stream(), p);
     return 0;
   }
   cudaLaunchConfig_t cfg{};
@@ -763,7 +779,7 @@ int attn_prefill_tc(const char* fn, const uint16_t* d_q, float scale, int Hq, in
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 2u : 1u;
-  G4_CUDA_TRY(fn, cudaLaunchKernelEx(&cfg, attn_prefill_tc_kernel, p));
+  G4_CUDA_TRY(fn, cudaLaunchKernelEx(&cfg, kernel, p));
   return 0;
 }
 

@@ -353,6 +353,14 @@ __device__ __forceinline__ uint4 ld_l2_hint(const uint4* p, uint64_t pol) {
   return v;
 }
 
+// Power of two that brings a head's largest value scale (float bits; 0: none known) to 2^12 - 2^13, so that seven of it and
+// its smaller ones sit in f16's normal range; never less than 1, and its inverse.
+__device__ __forceinline__ int v_exponent(uint32_t top_bits) {
+  return top_bits == 0u ? 0 : min(max(12 + 127 - static_cast<int>(top_bits >> 23), 0), 90);
+}
+__device__ __forceinline__ float v_up_factor(uint32_t top_bits) { return __int_as_float((127 + v_exponent(top_bits)) << 23); }
+__device__ __forceinline__ float v_down_factor(uint32_t top_bits) { return __int_as_float((127 - v_exponent(top_bits)) << 23); }
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));

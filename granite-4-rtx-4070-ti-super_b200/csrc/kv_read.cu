@@ -102,35 +102,47 @@ struct WidenParams {
   int8_t* ov;
   float* oks;
   float* ovs;
-  int Hk;
+  float* tops;
+  int blocks;  // of a head
   long long stride, n;
 };
 
-// Positions [0, n) of a sequence out of the 4-bit pool into an 8-bit pool [Hk][n][128] in their order.
+// Positions [0, n) of a sequence out of the 4-bit pool into an 8-bit pool [Hk][n][128] in their order; a block's 32 positions
+// of a head also leave their largest value scale.
+constexpr int kWidenPositions = kReadThreads / 8;
 __global__ void __launch_bounds__(kReadThreads) kv_widen_kernel(const WidenParams p) {
   pdl_begin();
+  __shared__ unsigned s_top[kReadThreads / 32];
   constexpr int kParts = 128 / 16;  // a thread: 8 bytes in, 16 out
-  const long long i = static_cast<long long>(blockIdx.x) * kReadThreads + threadIdx.x;
-  if (i >= p.n * p.Hk * kParts) return;
-  const int part = static_cast<int>(i % kParts);
-  const long long hp = i / kParts, pos = hp % p.n;
-  const int h = static_cast<int>(hp / p.n);
-  long long row = p.pt != nullptr ? __ldg(p.pt + pos) : pos;
-  row = row < 0 ? 0 : (row >= p.stride ? p.stride - 1 : row);
-  const size_t srow = static_cast<size_t>(h) * p.stride + row;
+  const int h = blockIdx.x / p.blocks, part = threadIdx.x % kParts;
+  const long long pos = static_cast<long long>(blockIdx.x - h * p.blocks) * kWidenPositions + threadIdx.x / kParts;
+  unsigned top = 0;
+  if (pos < p.n) {
+    long long row = p.pt != nullptr ? __ldg(p.pt + pos) : pos;
+    row = row < 0 ? 0 : (row >= p.stride ? p.stride - 1 : row);
+    const size_t srow = static_cast<size_t>(h) * p.stride + row, hp = static_cast<size_t>(h) * p.n + pos;
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    const uint2 w = __ldg(reinterpret_cast<const uint2*>((kv ? p.cv : p.ck) + srow * 64) + part);
-    const uint2 a = nibbles_to_bytes(w.x), b = nibbles_to_bytes(w.y);
-    reinterpret_cast<uint4*>(kv ? p.ov : p.ok)[i] = make_uint4(a.x, a.y, b.x, b.y);
+    for (int kv = 0; kv < 2; ++kv) {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>((kv ? p.cv : p.ck) + srow * 64) + part);
+      const uint2 a = nibbles_to_bytes(w.x), b = nibbles_to_bytes(w.y);
+      reinterpret_cast<uint4*>(kv ? p.ov : p.ok)[hp * kParts + part] = make_uint4(a.x, a.y, b.x, b.y);
+    }
+    if (part == 0) {
+      // A value scale that is not finite, or takes values past fp16's range (V's type in those kernels), goes over to the
+      // key's: as a logit it is masked for the rows that do not see the position, as an element of V it would reach them
+      // (0 times infinity), and who sees it gets NaN either way.
+      const float ks = __ldg(p.ks + srow), vs = __ldg(p.vs + srow);
+      const bool sound = fabsf(vs) * 7.0f <= 65504.0f;
+      p.oks[hp] = sound ? ks : __int_as_float(0x7fc00000), p.ovs[hp] = sound ? vs : 0.0f;
+      if (sound) top = __float_as_uint(fabsf(vs));
+    }
   }
-  if (part == 0) {
-    // A value scale that is not finite, or takes values past fp16's range (V's type in those kernels), goes over to the
-    // key's: as a logit it is masked for the rows that do not see the position, as an element of V it would reach them
-    // (0 times infinity), and who sees it gets NaN either way.
-    const float ks = __ldg(p.ks + srow), vs = __ldg(p.vs + srow);
-    const bool sound = fabsf(vs) * 7.0f <= 65504.0f;
-    p.oks[hp] = sound ? ks : __int_as_float(0x7fc00000), p.ovs[hp] = sound ? vs : 0.0f;
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (threadIdx.x % 32 == 0) s_top[threadIdx.x / 32] = top;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    top = __reduce_max_sync(0xffffffffu, threadIdx.x < kReadThreads / 32 ? s_top[threadIdx.x] : 0u);
+    if (threadIdx.x == 0) p.tops[blockIdx.x] = __uint_as_float(top);
   }
 }
 
@@ -148,11 +160,13 @@ int launch_read(const char* fn, const ReadParams& p) {
 
 }  // namespace
 
-// Used by the prefill attention over a 4-bit pool (attn_int4.cu); out: codes [2][Hk][n][128], scales [2][Hk][n].
+// Used by the prefill attention over a 4-bit pool (attn_int4.cu); out: codes [2][Hk][n][128], scales [2][Hk][n], and the
+// largest value scales of every 32 positions [Hk][widen_tops(n)].
+int widen_tops(long long n) { return static_cast<int>((n + kWidenPositions - 1) / kWidenPositions); }
 int widen_int4(const char* fn, const uint8_t* ck, const uint8_t* cv, const float* ks, const float* vs, const int* pt,
-               int Hk, long long stride, long long n, int8_t* ok, int8_t* ov, float* oks, float* ovs) {
-  WidenParams p{ck, cv, ks, vs, pt, ok, ov, oks, ovs, Hk, stride, n};
-  const long long blocks = (n * Hk * 8 + kReadThreads - 1) / kReadThreads;
+               int Hk, long long stride, long long n, int8_t* ok, int8_t* ov, float* oks, float* ovs, float* tops) {
+  WidenParams p{ck, cv, ks, vs, pt, ok, ov, oks, ovs, tops, widen_tops(n), stride, n};
+  const long long blocks = static_cast<long long>(p.blocks) * Hk;
   if (blocks > INT_MAX) return fail(fn, "too many positions");
   G4_LAUNCH_PDL(fn, kv_widen_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kReadThreads), 0, current_stream(), p);
   return 0;

@@ -561,11 +561,13 @@ int granite4_kernel_attn_decode_int4_paged(const uint16_t* d_q, const uint8_t* d
 /* Added: granite4_prefill_attention_int8 over the 4-bit pool. With d 128 and Hq == 4 Hk,
  * chunks of 64 rows or more (at the start of a sequence: of over 192, or of 32 to 63)
  * widen the sequence's rows into an 8-bit pool in d_scratch (exact: a 4-bit code is an
- * 8-bit code with the same scale; 264 bytes per position and kv head) and run the kernels
- * of that entry point; everything else runs on the decode kernel, where d_scratch is
- * optional (without it no range is split). Those kernels hold V in fp16: values under
- * 6e-5 lose bits there, and a position with 7 * v_scale over 65504 gives NaN to the rows
- * that see it, as a scale that is not a number does in both forms. d_scratch must hold
+ * 8-bit code with the same scale; 265 bytes per position and kv head) and run the kernels
+ * of that entry point; everything else, and an output that is not aligned to 16 bytes (4
+ * below 64 rows), runs on the decode kernel, where d_scratch is optional (without it no
+ * range is split). Those kernels hold V as fp16(code * fp16(v_scale)) after a power of two
+ * of each head that puts its largest v_scale under 9360 at 2^12 or more: v_scale down to
+ * 2^-26 of that keeps its bits. A position with 7 * v_scale over 65504 gives NaN to the
+ * rows that see it, as a scale that is not a number does in both forms. d_scratch must hold
  * granite4_prefill_attention_int4_scratch_bytes(...) bytes, 16-byte aligned. */
 long long granite4_prefill_attention_int4_scratch_bytes(int rows, int base_pos, int Hq, int Hk, int d);
 int granite4_prefill_attention_int4(const uint16_t* d_q_rot, float scale, int Hq, int Hk, int d,
