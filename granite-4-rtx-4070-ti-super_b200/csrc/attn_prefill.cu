@@ -298,7 +298,7 @@ constexpr int kWarps2 = 4;  // warp w: row tile w % 2, output dims 64 (w / 2) ..
 struct PrefillSmem2 {
   PrefillSmem t;
   __half qh[kQRows2][kHPitch];
-  uint32_t v_top;  // the largest of p.v_tops, as float bits
+  uint32_t v_top, q_amax;  // the largest of p.v_tops and, with them, max |q| of the rows, as float bits
 };
 
 __global__ void __launch_bounds__(kWarps2 * 32, 2) attn_prefill2_kernel(const PrefillParams p) {
@@ -336,25 +336,41 @@ __global__ void __launch_bounds__(kWarps2 * 32, 2) attn_prefill2_kernel(const Pr
   };
   gather(0, 0);
 
-  // a power of two on V and back, as in the tensor-core form
-  if (tid == 0) sm2.v_top = 0u;
-  if (p.v_tops != nullptr) {
-    uint32_t top = 0u;
-    for (int i = tid; i < p.n_tops; i += kWarps2 * 32) top = max(top, __float_as_uint(__ldg(p.v_tops + static_cast<size_t>(hkv) * p.n_tops + i)));
-    top = __reduce_max_sync(0xffffffffu, top);
-    __syncthreads();
-    if (lane == 0) atomicMax(&sm2.v_top, top);
+  // the Q rows (rows past the chunk repeat the last row), and powers of two on Q and V and back, as in the tensor-core form
+  uint4 q_raw[kQRows2 * (kD / 8) / (kWarps2 * 32)];
+#pragma unroll
+  for (int u = 0; u < kQRows2 * (kD / 8) / (kWarps2 * 32); ++u) {
+    const int i = u * (kWarps2 * 32) + tid, row = i >> 4, piece = i & 15;
+    q_raw[u] = __ldg(reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(r0 + min(row, nrows - 1)) * p.Hq + head) * kD) + piece);
   }
+  if (tid == 0) sm2.v_top = sm2.q_amax = 0u;
   __syncthreads();
-  const float v_up = v_up_factor(sm2.v_top);
+  if (p.v_tops != nullptr) {
+    uint32_t top = 0u, q_top = 0u;
+    for (int i = tid; i < p.n_tops; i += kWarps2 * 32) top = max(top, __float_as_uint(__ldg(p.v_tops + static_cast<size_t>(hkv) * p.n_tops + i)));
+#pragma unroll
+    for (int u = 0; u < kQRows2 * (kD / 8) / (kWarps2 * 32); ++u) {
+      float f[8];
+      unpack8(q_raw[u], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q_top = max(q_top, fabsf(f[e]) < INFINITY ? __float_as_uint(fabsf(f[e])) : 0u);
+    }
+    top = __reduce_max_sync(0xffffffffu, top), q_top = __reduce_max_sync(0xffffffffu, q_top);
+    if (lane == 0) atomicMax(&sm2.v_top, top), atomicMax(&sm2.q_amax, q_top);
+    __syncthreads();
+  }
+  const float v_up = v_up_factor(sm2.v_top), q_down = p.v_tops != nullptr ? q_down_factor(sm2.q_amax) : 1.0f;
+  const float logit_scale = p.v_tops != nullptr ? p.scale_log2 * q_up_factor(sm2.q_amax) : p.scale_log2;
 
-  // the Q rows -> fp16 in shared memory (rows past the chunk repeat the last row); read behind the tile loop's barrier
-  for (int i = tid; i < kQRows2 * (kD / 8); i += kWarps2 * 32) {
-    const int row = i >> 4, piece = i & 15;
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(r0 + min(row, nrows - 1)) * p.Hq + head) * kD) + piece);
+  // Q -> fp16 in shared memory, read behind the tile loop's barrier
+#pragma unroll
+  for (int u = 0; u < kQRows2 * (kD / 8) / (kWarps2 * 32); ++u) {
+    const int i = u * (kWarps2 * 32) + tid, row = i >> 4, piece = i & 15;
+    float f[8];
+    unpack8(q_raw[u], f);
     uint4 h;
-    h.x = pf_pack(bf16_lo(w.x), bf16_hi(w.x)), h.y = pf_pack(bf16_lo(w.y), bf16_hi(w.y));
-    h.z = pf_pack(bf16_lo(w.z), bf16_hi(w.z)), h.w = pf_pack(bf16_lo(w.w), bf16_hi(w.w));
+    h.x = pf_pack(f[0] * q_down, f[1] * q_down), h.y = pf_pack(f[2] * q_down, f[3] * q_down);
+    h.z = pf_pack(f[4] * q_down, f[5] * q_down), h.w = pf_pack(f[6] * q_down, f[7] * q_down);
     *reinterpret_cast<uint4*>(&sm2.qh[row][piece * 8]) = h;
   }
 
@@ -382,7 +398,7 @@ __global__ void __launch_bounds__(kWarps2 * 32, 2) attn_prefill2_kernel(const Pr
       *reinterpret_cast<uint4*>(&sm.kh[row][piece * 8]) = *reinterpret_cast<const uint4*>(&kh2[0]);
       *reinterpret_cast<uint4*>(&sm.vh[row][piece * 8]) = *reinterpret_cast<const uint4*>(&vh2[0]);
     }
-    if (tid < kTileP) sm.ks[stage][tid] *= p.scale_log2;
+    if (tid < kTileP) sm.ks[stage][tid] *= logit_scale;
     __syncthreads();
 
 #pragma unroll 1

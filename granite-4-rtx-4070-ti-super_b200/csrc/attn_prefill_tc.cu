@@ -216,16 +216,6 @@ __device__ __forceinline__ void mul8(uint4& v, __half2 f) {
   for (int i = 0; i < 4; ++i) h[i] = __hmul2(h[i], f);
 }
 
-// The CTA's Q rows are scaled by 2^-e, e = exponent(max |q|) - 10, so that they sit in f16's range
-// whatever their magnitude (bf16 reaches 3e38); 2^e goes into the logit factor.
-__device__ __forceinline__ int q_exponent(uint32_t amax_bits) {
-  const float a = __uint_as_float(amax_bits);
-  if (!(a > 0.0f) || !(a < INFINITY)) return 0;
-  return min(max(static_cast<int>((amax_bits >> 23) & 0xffu) - 127 - 10, -100), 100);
-}
-__device__ __forceinline__ float q_down_factor(uint32_t amax_bits) { return __int_as_float((127 - q_exponent(amax_bits)) << 23); }
-__device__ __forceinline__ float q_up_factor(uint32_t amax_bits) { return __int_as_float((127 + q_exponent(amax_bits)) << 23); }
-
 // Where the largest value scale of the head is known, V is scaled by a power of two (v_up_factor, g4_math.cuh) on its way to f16,
 // so that small values keep their bits, and the output scaled back: exact both ways.
 template <bool TOPS>

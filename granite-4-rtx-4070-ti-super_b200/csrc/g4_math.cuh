@@ -353,6 +353,15 @@ __device__ __forceinline__ uint4 ld_l2_hint(const uint4* p, uint64_t pol) {
   return v;
 }
 
+// The prefill attentions scale a CTA's Q rows by 2^-e, e = exponent(max |q|) - 10, so that they sit in
+// f16's range whatever their magnitude (bf16 reaches 3e38); 2^e goes into the logit factor.
+__device__ __forceinline__ int q_exponent(uint32_t amax_bits) {
+  const float a = __uint_as_float(amax_bits);
+  if (!(a > 0.0f) || !(a < INFINITY)) return 0;
+  return min(max(static_cast<int>((amax_bits >> 23) & 0xffu) - 127 - 10, -100), 117);
+}
+__device__ __forceinline__ float q_down_factor(uint32_t amax_bits) { return __int_as_float((127 - q_exponent(amax_bits)) << 23); }
+__device__ __forceinline__ float q_up_factor(uint32_t amax_bits) { return __int_as_float((127 + q_exponent(amax_bits)) << 23); }
 // Power of two that brings a head's largest value scale (float bits; 0: none known) to 2^12 - 2^13, so that seven of it and
 // its smaller ones sit in f16's normal range; never less than 1, and its inverse.
 __device__ __forceinline__ int v_exponent(uint32_t top_bits) {

@@ -179,3 +179,25 @@ def test_an_output_on_any_boundary(K, rows, base, shift):
     # (which form an unaligned output takes is not said here: the bound of both)
     check(out[pick], want, bound + 2 * 7 * 128 * 2.0**-16 * 0.3 / 16 * 5.0 * want.abs().amax())
     assert (buf[:shift] == 3.0).all() and (buf[shift + rows * Hq * d:] == 3.0).all()
+
+
+@pytest.mark.parametrize("rows,base", [(20, 7), (40, 60), (63, 129), (64, 800), (300, 5)])
+@pytest.mark.parametrize("size", [3e38, 1e9, 7e4, 1e-6, 1e-12])
+def test_queries_of_any_size(K, rows, base, size):
+    """Queries that fp16 does not hold, with a softmax scale that leaves their logits as they are: to the bit those of the queries
+    scaled by a power of two, within the bound else."""
+    Hq, Hk, d = 32, 8, 128
+    g = gen(rows)
+    p = Pool(g, base + rows, Hk, d)
+    unit = torch.rand(rows, Hq, d, generator=g, device=DEV, dtype=torch.float64) * 2 - 1
+    q = (unit * size).to(torch.bfloat16)
+    assert torch.isfinite(q).all()
+    pick = [0, rows // 2, rows - 1]
+    unit = (q.double() / size).float()  # (what q stands for, in a type that holds it)
+    want, bound = reference(p, unit, base, 1.0 / 16, pick)
+    check(chunk(K, p, q, base, 1.0 / 16 / size)[pick], want, bound)
+    power = 2.0 ** round(torch.log2(torch.tensor(size)).item() - 2)
+    one = (unit * 4).to(torch.bfloat16)
+    if size > 1e38:  # scale * log2(e) = 1.44 * 2^-132 is a multiple of 2^-149 in f32: a factor of the logits off by up to 2^-18
+        return
+    assert torch.equal(chunk(K, p, (one.float() * power).to(torch.bfloat16), base, 1.0 / 64 / power), chunk(K, p, one, base, 1.0 / 64))
