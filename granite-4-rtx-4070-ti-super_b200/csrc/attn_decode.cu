@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kCtasPerSmT : kCtasPerS
     qmax = warp_max(qmax);
     int qexp = 0;
     if (qmax > 0.0f && qmax < INFINITY)
-      qexp = min(max(((__float_as_int(qmax) >> 23) & 0xff) - 127 - 10, -100), 100);
+      qexp = min(max(((__float_as_int(qmax) >> 23) & 0xff) - 127 - 10, -100), 117);
     const float qdown = __int_as_float((127 - qexp) << 23);
     logit_scale = p.scale_log2 * __int_as_float((127 + qexp) << 23);
 #pragma unroll
