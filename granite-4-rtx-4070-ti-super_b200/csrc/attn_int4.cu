@@ -848,12 +848,12 @@ Int4Plan plan_int4(int rows, int per, int Hq, int Hk, int d, int max_len) {
   const int columns = per * (Hq / Hk);
   s.ns = columns <= 4 ? 1 : columns <= 8 ? 2 : columns <= 12 ? 3 : 4;
   s.blocks = (columns + 4 * s.ns - 1) / (4 * s.ns);
-  s.groups = (rows + per - 1) / per;
+  s.groups = rows / per + (rows % per != 0);
   s.segments = static_cast<long long>(s.groups) * Hk * s.blocks;
   s.cluster = 1;
   if (s.segments > kMaxQuotient || max_len <= kTile * kWarps) return s;
   const long long resident = std::min(static_cast<long long>(ctas_per_sm(s.ns)) * sm_count(), static_cast<long long>(kMaxShares));
-  const long long per_segment = (max_len + kTile - 1) / kTile, tiles = s.segments * per_segment;
+  const long long per_segment = (static_cast<long long>(max_len) + kTile - 1) / kTile, tiles = s.segments * per_segment;
   // Costs in ns, fitted to measured calls (segments of 7 - 4096 tiles, 2 - 512 of them; within 15 % but for a few): a CTA
   // starts and ends in 4 us; its four warps take a tile in 0.2 us, in twice that with the card full, more with more columns,
   // less with narrow heads. A cluster's join costs 1.6 us; clusters leave an SM's last places empty here and there, those
