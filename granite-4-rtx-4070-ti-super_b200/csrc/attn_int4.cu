@@ -31,8 +31,8 @@
 // positions that it sees, less 10: the largest p v_scale so far is kept at 2^10, whatever its magnitude, and a scale at a position
 // that a column does not see, or gives no weight to, takes no bits from the others. That moves only when a position passes it by
 // 14: products reach 2^14, fp16 ends at 2^16, and most tiles leave the accumulators as they are. m is a logit, and everything
-// else a difference to it, so that large logits cost no bits of the rest. p reaches 2^54 where v_scale is small: a scale, a
-// zero too, counts as 2^-40 at least, so that neither a sum of p nor the factor of a move leaves f32 for scales up to 2^60.
+// else a difference to it, so that large logits cost no bits of the rest. p reaches 2^94 where v_scale is small: a scale, a
+// zero too, counts as 2^-80 at least, so that a sum of p stays within f32. Scales up to 2^100 are as good.
 //
 // Work split, by size: a (group, kv head, column block) segment is one CTA's; or a cluster's, whose CTAs take equal parts
 // and join them through distributed shared memory; or, for long caches, the segments' tiles of 32 positions form one line,
@@ -75,7 +75,7 @@ constexpr int kMaxShares = 640;   // it is cut into
 constexpr int kMaxColumns = 64;   // rows of a group x query heads of a kv head
 constexpr float kNone = -1e38f;  // the m of what has seen nothing: below every logit, and differences of two are finite
 constexpr float kUnset = -1e30f;  // the same of `under`
-constexpr float kLift = 10.0f, kSlack = 14.0f, kLeastLogScale = -40.0f;
+constexpr float kLift = 10.0f, kSlack = 14.0f, kLeastLogScale = -80.0f;
 
 struct Int4AttnParams {
   const uint16_t* q;
@@ -552,8 +552,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
           for (int u = 0; u < 4; ++u) dl[i][u] -= up, z = fmaxf(z, dl[i][u] + lv[u]);
           z = over_positions(z);
           const float next = grows ? z - kLift : under[i];
-          corr[i] = exp2_fast(under[i] - next - up);
-          l_run[i] *= corr[i], m_ref[i] = m_new, under[i] = next;
+          const float down = under[i] - next - up, half = exp2_fast(0.5f * down);
+          corr[i] = exp2_fast(down);
+          l_run[i] *= half, l_run[i] *= half;  // (a sum of 2^94 outlives a factor under f32's range)
+          m_ref[i] = m_new, under[i] = next;
         }
 #pragma unroll
         for (int n = 0; n < kNP; ++n) {
@@ -619,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
     // the four warps' states meet in shared memory, each parked in the warp's own ring
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __syncwarp();
-    float* const park = reinterpret_cast<float*>(ring);  // [kC][D + kPad], then [kC][2] (m, sum), as of p = exp2(l - m)
+    float* const park = reinterpret_cast<float*>(ring);  // [kC][D + kPad], then [kC][2] (m, sum), as of p = exp2(l - m), 1 <= sum < 2
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const int n = i >> 1, e = i & 1, c = 4 * i + t;
@@ -627,13 +629,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(co
       l += __shfl_xor_sync(0xffffffffu, l, 4);
       l += __shfl_xor_sync(0xffffffffu, l, 8);
       l += __shfl_xor_sync(0xffffffffu, l, 16);
-      const float shift = exp2_fast(under[i]), back = 1048576.0f * shift;
-      if (g == 0) park[kC * (D + kPad) + 2 * c] = under[i] == kUnset ? kNone : m_ref[i], park[kC * (D + kPad) + 2 * c + 1] = l * shift;
+      const int ex = ((__float_as_int(l) >> 23) & 0xff) - 127;
+      const float shift = __int_as_float((127 - ex) << 23);
+      if (g == 0) park[kC * (D + kPad) + 2 * c] = l == 0.0f ? kNone : m_ref[i] + (under[i] + static_cast<float>(ex)), park[kC * (D + kPad) + 2 * c + 1] = l * shift;
       const float off = osum[n][e] * (8.0f / 1048576.0f);
 #pragma unroll
       for (int m = 0; m < kM; ++m)  // rows g, g + 8: dims 32 (m / 2) + 4 g + 2 (m % 2), + 1
         *reinterpret_cast<float2*>(park + c * (D + kPad) + 32 * (m >> 1) + 4 * g + 2 * (m & 1)) =
-            make_float2((o[n][m][e] - off) * back, (o[n][m][2 + e] - off) * back);
+            make_float2((o[n][m][e] - off) * 1048576.0f * shift, (o[n][m][2 + e] - off) * 1048576.0f * shift);
     }
     __syncthreads();
     const bool whole = piece_begin == 0 && piece_end == n_tiles;

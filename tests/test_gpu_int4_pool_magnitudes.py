@@ -7,7 +7,7 @@ The reference, in 64 bits, takes q as the kernel holds it, the 16-bit integer ro
   store                  2^-8 |exact|
   p v_scale as fp16      2^-11 sum p |v|; its floor: the largest p s is held at 2^10 or more and steps under fp16's normal range
                          are 2^-24, so each of the n positions is off by at most 2^-35 max(p s), times |c| <= 7 (and 1 % for the
-                         logarithm that decides on it); a scale counts as 2^-40 at least: 7 n (1.01 2^-35 max(p s) + 2^-75)
+                         logarithm that decides on it); a scale counts as 2^-80 at least: 7 n (1.01 2^-35 max(p s) + 2^-115)
   logits                 an exact integer, to f32 (1), times k_scale (scale log2(e) max |q| / 32639) (5, the constant's among
                          them), less a logit in an fma and less a number under 64 (what is left is under 64 for every position
                          whose weight counts): in powers of two under 8 * 2^-24 |l| + 64 * 2^-24; exp2 itself 2^-22; numerator
@@ -79,7 +79,7 @@ def reference(p, q, pos, scale, window=0, table=None):
         size = logits.abs().amax(-1) / math.log(2.0)
         rel = 2.0**-11 + 2 * (2.0**-22 + math.log(2.0) * 2.0**-24 * (8 * size + 64))
         steps = 2 * -(-n // 32)
-        off = 2.0**-8 * e.abs() + rel[..., None] * mass + (7 * n * (1.01 * 2.0**-35 * ws.amax(-1) + 2.0**-75) + 16 * (steps + 16) * 2.0**-23 * ws.sum(-1))[..., None]
+        off = 2.0**-8 * e.abs() + rel[..., None] * mass + (7 * n * (1.01 * 2.0**-35 * ws.amax(-1) + 2.0**-115) + 16 * (steps + 16) * 2.0**-23 * ws.sum(-1))[..., None]
         exact[r], bar[r] = e.view(Hq, d), off.view(Hq, d)
     return exact, bar
 
@@ -100,7 +100,7 @@ def check(got, want, bar, sharp):
     assert (want.abs() / bar.clamp(min=1e-300)).median().item() >= sharp
 
 
-@pytest.mark.parametrize("loud", [1e6, 1e12, 1e18])
+@pytest.mark.parametrize("loud", [1e6, 1e12, 1e18, 1e28])
 @pytest.mark.parametrize("Hq,Hk,d", [(8, 4, 128), (16, 2, 64), (32, 8, 128)])
 @pytest.mark.parametrize("n,per,window", [(4, 4, 0), (60, 3, 0), (900, 4, 0), (30000, 3, 0), (5000, 2, 40), (129, 4, 3)])
 def test_a_large_value_scale_stays_with_the_rows_that_see_it(K, n, per, window, Hq, Hk, d, loud):
@@ -157,7 +157,7 @@ def test_value_scales_over_many_magnitudes(K, n, spread, Hq, Hk, d):
         check(decode(K, p, q, pos, 1.0 / 16), want, bar, 10.0 if n < 10000 else 2.0)  # (the bound of the sums grows with n)
 
 
-@pytest.mark.parametrize("small", [1e-3, 1e-6, 1e-9, 1e-11])
+@pytest.mark.parametrize("small", [1e-3, 1e-6, 1e-9, 1e-11, 1e-16, 1e-22])
 def test_small_values_keep_their_bits(K, small):
     Hq, Hk, d = 32, 8, 128
     for n in (50, 2000):
@@ -197,6 +197,23 @@ def test_weight_on_values_of_zero(K):
     check(decode(K, p, q, pos, 1.0 / 64), want, bar, 10.0)
     p.vs[:] = 0.0
     assert (decode(K, p, q, pos, 1.0 / 64) == 0).all()
+
+
+@pytest.mark.parametrize("n", [40, 2000, 40000])
+def test_zeros_then_a_large_value(K, n):
+    """Value scales of zero or 1e-20, then 1e12 - 1e28 at one position: what the others weigh is not lost on the way."""
+    Hq, Hk, d = 32, 8, 128
+    g = gen(n)
+    p = Pool(g, n, Hk, d)
+    q = torch.randn(1, Hq, d, generator=g, device=DEV).to(torch.bfloat16)
+    pos = torch.tensor([n - 1], dtype=torch.int32, device=DEV)
+    for low in (0.0, 1e-20):
+        for loud in (1e12, 1e20, 1e28):
+            for at in (n - 2, 3, n // 2):
+                p.vs[:] = low
+                p.vs[:, at] = loud
+                want, bar = reference(p, q, pos, 1.0 / 16)
+                check(decode(K, p, q, pos, 1.0 / 16), want, bar, 10.0 if n < 10000 else 2.0)
 
 
 def test_columns_do_not_depend_on_their_neighbours(K):
