@@ -963,13 +963,21 @@ int attn_int4(const char* fn, Int4AttnParams p, int d, void* scratch, long long 
   }
 }
 
-// Which chunks go through the kernels for an 8-bit pool. Measured (32 / 8 heads of 128), decode form and widened, us: 64
-// rows after 0 positions 8 and 16, after 500 13 and 21, after 1203 23 and 22, after 16000 88 and 58; 192 rows after 0
-// positions 12 and 19, after 1203 29 and 27; 256 rows after 500 42 and 24; 48 rows after 0 positions 8 and 6, after 500
-// 13 and 23, after 16000 71 and 534 (below 64 rows those kernels walk the cache in one piece).
+// Which chunks go through the kernels for an 8-bit pool. From 64 rows on the decode form pays for its tiles (every 16 / G rows
+// unpack the prefix again), the widened one a start of some 20 us and a pass over the prefix, so the first is taken up to 1.4
+// million rows x kv heads x positions, or until its segments no longer run at once. Measured, G 4, decode form and widened, us:
+// 8 kv heads, 64 rows after 1203 positions 18 and 22, after 2500 27 and 26, after 16000 88 and 58; 77 after 1203 21 and 25;
+// 192 after 0 10 and 19, after 1203 29 and 27; 256 after 0 26 and 20; 2 kv heads, 256 after 1203 19 and 23, 128 after 4000 21 and
+// 28, 192 after 16000 71 and 42; 16 kv heads, 128 after 1203 46 and 30. Over 360 such calls (1 - 16 kv heads) the rule costs
+// 1.4 % against the better of the two; worst are long prefixes of one kv head (64 rows after 60000: 48 and 98).
+// Below 64 rows those kernels walk the cache in one piece: 48 rows after 0 positions 7 and 6, after 500 13 and 23, after 16000 70
+// and 534.
 bool widens(int rows, int base_pos, int Hq, int Hk, int d) {
   if (rows < 32 || d != 128 || Hq != 4 * Hk) return false;
-  return rows < 64 ? base_pos <= 192 - rows : rows > 192 || base_pos > 768 - rows;
+  if (rows < 64) return base_pos <= 192 - rows;
+  const long long segments = static_cast<long long>((rows + 3) / 4) * Hk;
+  return segments > static_cast<long long>(ctas_per_sm(4)) * sm_count() ||
+         (2ll * base_pos + rows) * rows * Hk >= 2800000;
 }
 int prefill_group(int Hq, int Hk) { return std::max(1, 16 / (Hq / Hk)); }
 long long widened_bytes(long long n, int Hk) { return (2 * n * Hk * (128 + 4) + 4ll * Hk * widen_tops(n) + 63) / 16 * 16; }

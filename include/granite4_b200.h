@@ -559,8 +559,8 @@ int granite4_kernel_attn_decode_int4_paged(const uint16_t* d_q, const uint8_t* d
                                            int max_len, int window, float scale, void* d_scratch,
                                            long long scratch_bytes, uint16_t* d_out);
 /* Added: granite4_prefill_attention_int8 over the 4-bit pool. With d 128 and Hq == 4 Hk,
- * chunks of 64 rows or more (at the start of a sequence: of over 192, or of 32 to 63)
- * widen the sequence's rows into an 8-bit pool in d_scratch (exact: a 4-bit code is an
+ * chunks of 64 rows or more with enough work (about 1.4 million rows x kv heads x
+ * positions) and those of 32 to 63 rows at the start of a sequence widen the sequence's rows into an 8-bit pool in d_scratch (exact: a 4-bit code is an
  * 8-bit code with the same scale; 265 bytes per position and kv head) and run the kernels
  * of that entry point; everything else, and an output that is not aligned to 16 bytes (4
  * below 64 rows), runs on the decode kernel, where d_scratch is optional (without it no
