@@ -216,6 +216,37 @@ def test_zeros_then_a_large_value(K, n):
                 check(decode(K, p, q, pos, 1.0 / 16), want, bar, 10.0 if n < 10000 else 2.0)
 
 
+@pytest.mark.parametrize("scale", [1e5, -1e6, 1e8, 1e12])
+@pytest.mark.parametrize("n", [37, 3000, 40000])
+def test_logits_of_any_size(K, n, scale):
+    """Logits of 1e6 to 1e14, a few hundred thousand steps of f32 apart: the output is the value of the largest one's position, whatever
+    the others' scales are."""
+    Hq, Hk, d = 32, 8, 128
+    g = gen(n)
+    p = Pool(g, n, Hk, d)
+    q = torch.randn(1, Hq, d, generator=g, device=DEV).to(torch.bfloat16)
+    pos = torch.tensor([n - 1], dtype=torch.int32, device=DEV)
+    k = p.codes[0].double() * p.ks.double()[..., None]
+    logits = scale * torch.einsum("hgd,htd->hgt", held_q(q)[0].view(Hk, Hq // Hk, d), k)
+    top2 = logits.topk(2, -1)
+    clear = (top2.values[..., 0] - top2.values[..., 1] > 200 + 20 * 2.0**-24 * logits.abs().amax(-1)).view(Hq)
+    assert clear.float().mean() > 0.8
+    at = top2.indices[..., 0].view(Hq)
+    kv = torch.arange(Hq, device=DEV) // (Hq // Hk)
+    for loud in (0.0, 1e12):
+        vs = p.vs.clone()
+        if loud:
+            best = torch.zeros(Hk, n, dtype=torch.bool, device=DEV)
+            best[kv, at] = True
+            p.vs[~best & (torch.rand(Hk, n, generator=g, device=DEV) < 0.1)] = loud
+        got = decode(K, p, q, pos, scale)[0]
+        want = p.codes[1][kv, at].double() * p.vs[kv, at].double()[:, None]
+        # the store, the fp16 product, the sums over u, of a position of weight 1
+        bar = (2.0**-8 + 2.0**-11) * want.abs() + 16 * p.vs[kv, at].double()[:, None] * (2 * -(-n // 32) + 16) * 2.0**-23
+        check(got[clear], want[clear], bar[clear], 10.0 if n < 10000 else 2.0)
+        p.vs.copy_(vs)
+
+
 def test_columns_do_not_depend_on_their_neighbours(K):
     """The bits of a query head are the same whatever the other heads and rows of its group hold."""
     Hq, Hk, d = 32, 8, 128
