@@ -214,3 +214,43 @@ def test_queries_of_any_size(K, rows, base, size):
     if size > 1e38:  # scale * log2(e) = 1.44 * 2^-132 is a multiple of 2^-149 in f32: a factor of the logits off by up to 2^-18
         return
     assert torch.equal(chunk(K, p, (one.float() * power).to(torch.bfloat16), base, 1.0 / 64 / power), chunk(K, p, one, base, 1.0 / 64))
+
+
+@pytest.mark.parametrize("rows,base", [(20, 300), (40, 60), (64, 3000), (300, 5)])
+def test_chunks_captured_and_replayed(K, rows, base):
+    """Two graphs of a chunk each, with a scratch of its own, replayed side by side with inputs that change in between: to the bit what
+    the calls give."""
+    from granite4_b200 import capi
+    Hq, Hk, d, scale = 32, 8, 128, 1.0 / 16
+    g = gen(rows)
+    need = max(16, capi.lib().granite4_prefill_attention_int4_scratch_bytes(rows, base, Hq, Hk, d))
+    jobs = []
+    for _ in range(2):
+        p = Pool(g, base + rows, Hk, d)
+        q = torch.randn(rows, Hq, d, generator=g, device=DEV).to(torch.bfloat16)
+        out, scratch = torch.empty_like(q), torch.full((need,), 0xFF, dtype=torch.uint8, device=DEV)
+
+        def call(p=p, q=q, out=out, scratch=scratch):
+            assert K.prefill_attention_int4(q, scale, Hq, Hk, d, base, p.stride, out, *p.all, scratch=scratch) == 0
+        call()
+        torch.cuda.synchronize()
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=stream):
+            for _ in range(3):
+                call()
+        jobs.append((p, q, out, call, graph, stream))
+    for size in (1.0, 1e-3, 30.0):
+        want = []
+        for p, q, out, call, _, _ in jobs:
+            q.copy_(torch.randn(rows, Hq, d, generator=g, device=DEV))
+            p.vs.copy_((torch.rand(Hk, base + rows, generator=g, device=DEV) + 0.5) * size)
+            call()
+            want.append(out.clone())
+            out.zero_()
+        torch.cuda.synchronize()
+        for _, _, _, _, graph, stream in jobs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, out, _, _, _), w in zip(jobs, want):
+            assert torch.equal(out, w)
