@@ -41,9 +41,10 @@
 // fourth tile of a piece, each with its own ring of asynchronous copies and its own running (max, sum, O); they merge in
 // shared memory.
 //
-// 16 sessions of up to 24000 positions (32 / 8 heads of 128, 302 MB): 62 us, rows at 6 TB/s once they stream, 4 us before
+// 16 sessions of up to 24000 positions (32 / 8 heads of 128, 302 MB): 64 us, rows at 6 TB/s once they stream, 4 us before
 // and 4 to join; one session at 131072 (143 MB): 36 us; without the two contractions 4 us less each. One session of 37
-// positions 3.7 us, five groups of three rows at 4100 15 us.
+// positions 3.6 us, five groups of three rows at 4100 15 us, 16 groups of four at 16000 100, 118 where the softmax is so
+// peaked that the base moves all the time. (GPU time, replayed from a graph; called one by one 0.3 - 2 us more.)
 #include "g4_cluster.cuh"
 #include "g4_host.h"
 #include "g4_math.cuh"
@@ -230,8 +231,9 @@ constexpr int kPad = 4;  // floats after a parked row of O
 // NS logit tiles of four columns each: column 4 i + t of column block cb is pair c = 4 NS cb + 4 i + t, query row c / G,
 // query head c % G. P and O have a tile of eight columns for two of them: column 2 t + e of tile n is pair 4 (2 n + e) + t
 // (an odd NS: the odd columns of the last tile are zero).
-// Registers: 128 a thread for one or two logit tiles, 168 for three or four. Four tiles at two CTAs per SM: 16 groups of
-// four rows at 16000 83 us instead of 79, two of them at 33 positions 6.1 instead of 6.5.
+// Registers: 128 a thread for one or two logit tiles, 168 for three or four; four tiles of wide heads spill 176 bytes of them.
+// Four tiles at two CTAs per SM: 16 groups of four rows at 16000 5 % slower, two of them at 33 positions 6 %
+// faster.
 constexpr int ctas_per_sm(int ns) { return ns >= 3 ? 3 : 4; }
 template <int D, int NS>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NS)) attn_int4_kernel(const Int4AttnParams p) {

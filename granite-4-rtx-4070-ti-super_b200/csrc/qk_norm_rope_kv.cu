@@ -189,8 +189,9 @@ __device__ __forceinline__ void copies_wait() {
 // (the products of norm weights and tables for q) is worked out once. A lane's 32 bytes of the next three items are on
 // their way by asynchronous copies into slots of its own, so nothing is synchronised. Arithmetic is on pairs of f32 where
 // it can be. What bounds the kernel is memory, 22 KB a row of 48 heads in and out, and close behind it the issue slots:
-// 16384 such rows with norms into the 4-bit pool take 66 - 69 us, 5.3 TB/s, 2400 warp instructions a row. (With every key
-// in double 79 us, 3080; rows unrolled in the code 210 us, waiting for instructions.)
+// 16384 such rows with norms into the 4-bit pool take 66 - 69 us on the GPU, 5.3 TB/s, 2400 warp instructions a row; six CTAs
+// per SM leave 80 registers a thread, of which 28 - 32 bytes are spilled. (With every key in double 79 us, 3080; rows unrolled in
+// the code 210 us, waiting for instructions.)
 constexpr int kQkDepth = 4, kQkCtas = 6;
 // WHOLE: query heads and key / value heads fill their items, so the items of all rows lie one behind the other in qkv.
 template <int D, int BITS, bool WHOLE>

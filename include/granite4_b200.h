@@ -546,7 +546,11 @@ int granite4_attn_split_int8(const uint16_t* d_q, const int8_t* d_cache_k8, cons
  * position gets zeros; the rows of a group may have any positions. A query head
  * that holds an infinity or a NaN gives NaN, the others are not touched by it; a row
  * scale that is a NaN, or an infinite value scale, gives NaN to the rows that see its
- * position and to no others. The cache is cut into
+ * position and to no others. Held in fewer bits than f32: q in the logits, as the integer
+ * round(q 32639 / max |q|) of its head (off by up to max |q| / 65278, so elements far
+ * under the head's largest keep fewer bits than their own), and each probability times
+ * its v_scale, as fp16 against the largest of those that the row sees (v_scale from 2^-80
+ * to 2^100, or 0; what a row does not see does not count). The cache is cut into
  * equal shares whatever the sequences' lengths, and the order of every sum follows from
  * the arguments and positions alone: the same call gives the same bits. */
 long long granite4_attn_decode_int4_scratch_bytes(int rows, int rows_per_group, int Hq, int Hk, int d,
@@ -566,7 +570,8 @@ int granite4_kernel_attn_decode_int4_paged(const uint16_t* d_q, const uint8_t* d
  * below 64 rows), runs on the decode kernel, where d_scratch is optional (without it no
  * range is split). Those kernels hold V as fp16(code * fp16(v_scale)) after a power of two
  * of each head that puts its largest v_scale under 9360 at 2^12 or more: v_scale down to
- * 2^-26 of that keeps its bits. A position with 7 * v_scale over 65504 gives NaN to the
+ * 2^-26 of that keeps its bits; q is fp16 there after a power of two per 32 (below 64
+ * rows of the chunk) or 64 rows, probabilities are fp16. A position with 7 * v_scale over 65504 gives NaN to the
  * rows that see it, as a scale that is not a number does in both forms. d_scratch must hold
  * granite4_prefill_attention_int4_scratch_bytes(...) bytes, 16-byte aligned. */
 long long granite4_prefill_attention_int4_scratch_bytes(int rows, int base_pos, int Hq, int Hk, int d);
